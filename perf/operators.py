@@ -118,7 +118,8 @@ def draw(rng):
         drafts = rng.randint(17, 64)
         return dict(shape, kind="keep", requests=_log_int(rng, 1, 24), layers=layers,
                     kv_heads=rng.choice([1, 2, 4, 8]), head_dim=rng.choice([64, 80, 128]),
-                    block=rng.choice([1, 12, 16, 32]), drafts=drafts, path=rng.randint(1, 8), lo=0, hi=48, lens_seed=lens_seed)
+                    block=rng.choice([1, 12, 16, 32]), drafts=drafts, path=rng.randint(1, 8), lo=0,
+                    hi=48, lens_seed=lens_seed)
     base = dict(shape, kind="attend", tree=False, empty=rng.random() < 0.2, lens_seed=lens_seed)
     if kind == "decode":
         hi = _log_int(rng, 16, 8192)
