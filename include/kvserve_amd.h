@@ -62,6 +62,8 @@ typedef struct ihipStream_t* kvmi_stream_t;
 #define KVMI_ERR_SYNC 8         /* a one-pass compress barrier timed out or met another call's keys */
 #define KVMI_ERR_BLOCK_ID 16    /* a block id outside its pool (kvmi_check_block_ids) */
 #define KVMI_ERR_SCHEDULE 32    /* a job has more blocks than its one-pass schedule */
+#define KVMI_ERR_NO_BLOCKS 64   /* kvmi_build_tables: a request was refused, too few free blocks */
+#define KVMI_ERR_LENGTH 128     /* a length, slot range, query range or path outside its bounds */
 
 /* Host-visible return codes. */
 #define KVMI_OK 0
@@ -472,6 +474,131 @@ int kvmi_rt_decode(const kvmi_rt_geometry* geom, const kvmi_rt_layer* layers, in
 /* The runtime's normalized bf16-per-stage FWHT of rows [rows, head_dim]
  * (runtime cpp_backend.hadamard_transform); in and out may be equal, not overlap. */
 int kvmi_rt_hadamard(const void* in, void* out, int64_t rows, int32_t head_dim, kvmi_stream_t stream);
+
+/*
+ * ---- Decode-instance operators: block tables, slot writes, attention over the paged
+ * cache, kept drafts.  No counterpart in the reference, whose host (vLLM) does this work
+ * itself; they serve an instance that received its requests through kvmi_decode_paged.
+ */
+
+/*
+ * Block tables, slot map and free blocks brought from one set of request lengths to
+ * another, in one launch.  A request of n tokens holds ceil(n / block_size) blocks.
+ *   lengths, new_lengths  int32 [R] tokens before / after
+ *   tables                int32 [R][columns], a request's blocks in order
+ *   free_blocks           int32 [ring] ring of free block ids: `state` = {head, count}; blocks are
+ *                         taken at the head and returned behind the last
+ * Requests are served in order: one that grows is granted iff the blocks asked for by it and
+ * all before it fit the count (else KVMI_ERR_NO_BLOCKS: it keeps its length and blocks, and its
+ * new tokens get slot -1).  Blocks returned by this call are free for the next one.  A length
+ * outside [0, columns * block_size] sets KVMI_ERR_LENGTH and leaves its request as it is.
+ *   out_tables            may be `tables` itself (then only changed entries are written, the
+ *                         entries given up with -1); else every entry is written, -1 past the end
+ *   out_lengths, out_state   may be `lengths` and `state` (both or neither): then `ticket`, an
+ *                         int32 word that is zero before the first call, is used and left zero
+ *   slots                 int64 [max_tokens]: block * block_size + place of every new token,
+ *                         requests in order; -1 behind the last.  More tokens than that set
+ *                         KVMI_ERR_LENGTH
+ *   starts                int32 [R + 1]: where each request's new tokens begin in `slots`
+ * `err` may be null here and in the entry points below.
+ */
+typedef struct kvmi_tables_args {
+  const int32_t* lengths;
+  const int32_t* new_lengths;
+  const int32_t* tables;
+  int32_t* free_blocks;
+  const int32_t* state;
+  int32_t* out_tables;
+  int32_t* out_lengths;
+  int32_t* out_state;
+  int64_t* slots;
+  int32_t* starts;
+  int32_t* ticket;
+  int32_t* err;
+  int32_t requests, columns, ring, block_size, max_tokens, reserved;
+} kvmi_tables_args;
+int kvmi_build_tables(const kvmi_tables_args* args, kvmi_stream_t stream);
+
+/*
+ * A paged cache of 16-bit elements: element (part, block, token, head, channel) lies at
+ * base + (part * part_stride + block * block_stride + (token * num_heads + head) * head_dim +
+ * channel) * 2 bytes: [2, P, S, H, D] and [P, 2, S, H, D].
+ */
+typedef struct kvmi_cache {
+  void* base; /* kvmi_keep_drafts: see there */
+  int64_t part_stride;
+  int64_t block_stride;
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t num_heads;
+  int32_t head_dim;
+} kvmi_cache;
+
+/*
+ * Rows of new keys and values into the cache: token i's go to block slots[i] / S, place
+ * slots[i] % S.  key / value are [tokens][H][D] with the given strides in elements (channels
+ * adjacent).  Slot -1 is skipped; any other slot outside the cache sets KVMI_ERR_BLOCK_ID.
+ * No two tokens may share a slot.
+ */
+int kvmi_write_kv(const kvmi_cache* cache, const void* key, const void* value, int64_t key_token_stride,
+                  int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride,
+                  const int64_t* slots, int64_t tokens, int32_t* err, kvmi_stream_t stream);
+
+/*
+ * Attention of drafted (or any last) tokens over the paged cache.  Request r has the query rows
+ * starts[r] .. starts[r+1]-1, T of them, and a cache of lengths[r] = L tokens, the queries' own
+ * keys and values included as its last T.  Query i sees every position before L - T, and of the
+ * last T position j where bit j % 64 of mask[row * mask_words + j / 64] is set, or j <= i when
+ * `mask` is null.  Softmax(scale * q.k) is kept in fp32; a query that sees nothing gives zeros
+ * (and lse -inf).  What a query does not see does not touch its result, NaN and infinities
+ * included.
+ *   query, out  [total_queries][query_heads][D], query with strides in elements (channels
+ *               adjacent, 16-byte aligned rows), out contiguous; query head h reads KV head
+ *               h / (query_heads / num_heads)
+ *   lse         fp32 [total_queries][query_heads] natural log of the sums, or null
+ *   max_query   no request may have more queries (KVMI_ERR_LENGTH, the rows past it unwritten)
+ *   max_length  the longest length, for the launch shape only: any value gives the same sums up
+ *               to the order of their parts
+ *   workspace   kvmi_attention_workspace_bytes of the same arguments, 16-byte aligned
+ * D is a multiple of 8 up to 256.  A block id outside the cache sets KVMI_ERR_BLOCK_ID (the
+ * nearest block is read in its place), a length outside [0, columns * S] or a range outside the
+ * queries KVMI_ERR_LENGTH (and is clamped).
+ */
+typedef struct kvmi_attention_args {
+  kvmi_cache cache;
+  const void* query;
+  void* out;
+  float* lse;
+  const int32_t* tables;
+  const int32_t* lengths;
+  const int32_t* starts;
+  const uint64_t* mask;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* err;
+  int64_t query_token_stride;
+  int64_t query_head_stride;
+  float scale;
+  int32_t dtype; /* KVMI_DTYPE_* */
+  int32_t requests, columns, total_queries, query_heads, max_query, max_length, mask_words, reserved;
+} kvmi_attention_args;
+#define KVMI_DTYPE_BF16 0
+#define KVMI_DTYPE_FP16 1
+int64_t kvmi_attention_workspace_bytes(const kvmi_attention_args* args);
+int kvmi_tree_attention(const kvmi_attention_args* args, kvmi_stream_t stream);
+
+/*
+ * The accepted path of each request's drafts moved to the front of the drafted places, in every
+ * layer: row lengths[r] + i <- row lengths[r] + accepted[r][i].  `accepted` is int32 [R][width],
+ * strictly increasing draft numbers, ended by a negative one or the row's end; out_lengths[r] =
+ * lengths[r] + the path's length (not `lengths` itself).  A path that does not increase or leaves
+ * the table sets KVMI_ERR_LENGTH, a bad block id KVMI_ERR_BLOCK_ID; that request is left as it is
+ * and keeps its length.  `bases` is a device array of the layers' cache bases; `cache` gives their
+ * common layout, and `cache->base` the bitwise OR of all bases (their alignment).  width <= 1024.
+ */
+int kvmi_keep_drafts(const kvmi_cache* cache, void* const* bases, int32_t layers, const int32_t* tables,
+                     int32_t columns, const int32_t* lengths, const int32_t* accepted, int32_t requests,
+                     int32_t width, int32_t* out_lengths, int32_t* err, kvmi_stream_t stream);
 
 #ifdef __cplusplus
 }

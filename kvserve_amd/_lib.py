@@ -22,6 +22,8 @@ ERR_CORRUPT = 4
 ERR_SYNC = 8
 ERR_BLOCK_ID = 16
 ERR_SCHEDULE = 32
+ERR_NO_BLOCKS = 64
+ERR_LENGTH = 128
 OK, EINVAL, ELAUNCH, ENOSPC = 0, -22, -5, -28
 # Bytes of the fixed device array behind kvmi_v3_compress_noalloc (per GPU).
 V3_NOALLOC_SCRATCH_BYTES = 4 * 1024 * 1024
@@ -74,6 +76,11 @@ EXPORTS = (
     "kvmi_rt_decode",
     "kvmi_rt_hadamard",
     "kvmi_rt_scratch_bytes",
+    "kvmi_build_tables",
+    "kvmi_write_kv",
+    "kvmi_attention_workspace_bytes",
+    "kvmi_tree_attention",
+    "kvmi_keep_drafts",
 )
 
 
@@ -121,6 +128,31 @@ class RtLayer(ctypes.Structure):
                 ("token_stride", ctypes.c_int64), ("channel_offset", ctypes.c_int64), ("signs", ctypes.c_void_p),
                 ("head_order", ctypes.c_void_p), ("u8_offset", ctypes.c_int64), ("sections", RtSection * 2),
                 ("num_sections", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+DTYPE_BF16, DTYPE_FP16 = 0, 1
+
+
+class TablesArgs(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "lengths", "new_lengths", "tables", "free_blocks", "state", "out_tables", "out_lengths", "out_state", "slots",
+        "starts", "ticket", "err")] + [(name, ctypes.c_int32) for name in (
+            "requests", "columns", "ring", "block_size", "max_tokens", "reserved")]
+
+
+class Cache(ctypes.Structure):
+    _fields_ = [("base", ctypes.c_void_p), ("part_stride", ctypes.c_int64), ("block_stride", ctypes.c_int64),
+                ("num_blocks", ctypes.c_int32), ("block_size", ctypes.c_int32), ("num_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32)]
+
+
+class AttentionArgs(ctypes.Structure):
+    _fields_ = [("cache", Cache)] + [(name, ctypes.c_void_p) for name in (
+        "query", "out", "lse", "tables", "lengths", "starts", "mask", "workspace")] + [
+            ("workspace_bytes", ctypes.c_int64), ("err", ctypes.c_void_p), ("query_token_stride", ctypes.c_int64),
+            ("query_head_stride", ctypes.c_int64), ("scale", ctypes.c_float)] + [(name, ctypes.c_int32) for name in (
+                "dtype", "requests", "columns", "total_queries", "query_heads", "max_query", "max_length",
+                "mask_words", "reserved")]
 
 
 # kvmi_layer_job: 8 pointers, 4 int64, 2 int32 -> 104 bytes, 8-byte aligned.  It is
@@ -171,6 +203,12 @@ _SIGNATURES = {
     "kvmi_rt_decode": ([ctypes.POINTER(RtGeometry), _vp, _i32, _vp, _i64, _vp, _vp, _vp], ctypes.c_int),
     "kvmi_rt_hadamard": ([_vp, _vp, _i64, _i32, _vp], ctypes.c_int),
     "kvmi_rt_scratch_bytes": ([_i32, _i64, _i32, _i32], _i64),
+    "kvmi_build_tables": ([ctypes.POINTER(TablesArgs), _vp], ctypes.c_int),
+    "kvmi_write_kv": ([ctypes.POINTER(Cache), _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp], ctypes.c_int),
+    "kvmi_attention_workspace_bytes": ([ctypes.POINTER(AttentionArgs)], _i64),
+    "kvmi_tree_attention": ([ctypes.POINTER(AttentionArgs), _vp], ctypes.c_int),
+    "kvmi_keep_drafts": ([ctypes.POINTER(Cache), _vp, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp],
+                         ctypes.c_int),
 }
 
 

@@ -1,0 +1,355 @@
+// Decode-instance upkeep of the paged cache: block tables and slot maps from request
+// lengths, new keys and values written by slot, accepted drafts kept.
+#include "kvmi_common.hpp"
+
+namespace kvmi {
+namespace {
+
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ void flag_error(int32_t* err, int32_t bits) {
+  if (err && bits) atomicOr(err, bits);
+}
+
+// Sum over the workgroup, given to every thread.
+__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* lds) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return lds[0] + lds[1] + lds[2] + lds[3];
+}
+
+// ---------------------------------------------------------------- block tables
+struct Need {  // what one request's change of length asks for
+  int now, next, have, want;
+  bool bad;
+  __device__ int take() const { return want > have ? want - have : 0; }
+  __device__ int give() const { return have > want ? have - want : 0; }
+  __device__ int tokens() const { return next > now ? next - now : 0; }
+};
+__device__ __forceinline__ Need need_of(const kvmi_tables_args& a, int r) {
+  Need n;
+  const int64_t top = (int64_t)a.columns * a.block_size;
+  n.now = a.lengths[r];
+  n.next = a.new_lengths[r];
+  n.bad = n.now < 0 || n.now > top || n.next < 0 || n.next > top;
+  if (n.bad) n.next = n.now = n.now < 0 ? 0 : n.now > top ? (int)top : n.now;
+  n.have = (int)(((int64_t)n.now + a.block_size - 1) / a.block_size);
+  n.want = (int)(((int64_t)n.next + a.block_size - 1) / a.block_size);
+  return n;
+}
+
+// Workgroup (r, y) makes part y of request r's table row and slots.  No workgroup waits for
+// another: each adds up what the requests before its own ask for and give back (R lengths out
+// of the L2, a few microseconds less than a scan kernel and a second launch would take), and
+// from those sums it knows its place in the ring, so that a slot needs no table entry that
+// another workgroup writes.  A ring holds every block of the pool, so the places behind the
+// last free block never reach the head's: blocks returned here are not read here.
+__global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a) {
+  __shared__ int64_t lds[4];
+  __shared__ int last;
+  const int r = blockIdx.x, tid = threadIdx.x;
+  int64_t take = 0, give = 0, tokens = 0;
+  for (int i = tid; i < r; i += kThreads) {
+    const Need n = need_of(a, i);
+    take += n.take();
+    give += n.give();
+    tokens += n.tokens();
+  }
+  take = block_sum(take, lds);
+  give = block_sum(give, lds);
+  tokens = block_sum(tokens, lds);
+  const Need n = need_of(a, r);
+  const int N = a.ring;
+  const int head = (int)((uint32_t)a.state[0] % (uint32_t)N);
+  const int count = a.state[1] < 0 ? 0 : a.state[1] > N ? N : a.state[1];
+  const bool fits = take + n.take() <= count;
+  const bool granted = fits || n.take() == 0;
+  const int keep = granted ? n.want : n.have;
+  const bool in_place = a.out_tables == a.tables;
+  const int64_t row = (int64_t)r * a.columns;
+  const int64_t step = (int64_t)kThreads * gridDim.y;
+  const int64_t lane = (int64_t)blockIdx.y * kThreads + tid;
+
+  // the table row: blocks kept, blocks taken, and -1 behind them; the blocks given back go
+  // behind the last free one
+  const int lo = in_place ? (n.have < keep ? n.have : keep) : 0;
+  const int hi = in_place ? (n.have > keep ? n.have : keep) : a.columns;
+  for (int64_t k = lo + lane; k < hi; k += step) {
+    const int32_t old = k < n.have ? a.tables[row + k] : -1;
+    int32_t id = old;
+    if (k >= keep) {
+      if (k < n.have) a.free_blocks[(head + count + give + (k - keep)) % N] = old;
+      id = -1;
+    } else if (k >= n.have) {
+      id = a.free_blocks[(head + take + (k - n.have)) % N];
+    }
+    a.out_tables[row + k] = id;
+  }
+
+  // the new tokens' slots
+  for (int64_t i = lane; i < n.tokens(); i += step) {
+    const int64_t at = tokens + i;
+    if (at >= a.max_tokens) break;
+    int64_t slot = -1;
+    if (granted) {
+      const int p = n.now + (int)i, k = p / a.block_size;
+      const int32_t id = k < n.have ? a.tables[row + k] : a.free_blocks[(head + take + (k - n.have)) % N];
+      slot = (int64_t)id * a.block_size + p % a.block_size;
+    }
+    a.slots[at] = slot;
+  }
+  const int64_t upto = tokens + n.tokens();
+  if (r == a.requests - 1)
+    for (int64_t i = upto + lane; i < a.max_tokens; i += step) a.slots[i] = -1;
+  if (blockIdx.y == 0 && tid == 0) {
+    if (r == 0) a.starts[0] = 0;
+    a.starts[r + 1] = upto > 0x7fffffff ? 0x7fffffff : (int)upto;
+    flag_error(a.err, (granted ? 0 : KVMI_ERR_NO_BLOCKS) | (n.bad || upto > a.max_tokens ? KVMI_ERR_LENGTH : 0));
+  }
+
+  // Lengths and ring state.  They may lie over the inputs that other workgroups still read:
+  // then the last workgroup to arrive here writes them all.  Else each request's first
+  // workgroup writes its length, and the last request's the state.
+  const bool over = a.out_lengths == a.lengths;
+  if (over) {
+    __syncthreads();
+    if (tid == 0) last = atomicAdd(a.ticket, 1) == (int)(gridDim.x * gridDim.y) - 1;
+    __syncthreads();
+    if (!last) return;
+  } else {
+    if (blockIdx.y) return;
+    if (tid == 0) a.out_lengths[r] = granted ? (n.bad ? a.lengths[r] : n.next) : n.now;
+    if (r != a.requests - 1) return;
+  }
+  // taken = the asked-for sum up to the last request that fits; only where blocks ran short,
+  // or where all lengths are still to be written, are the sums needed request by request
+  const int64_t all_give = give + (granted ? n.give() : 0);
+  int64_t taken = take + n.take(), returned = all_give;
+  if (over || !fits) {
+    int64_t before = 0, fit = 0;
+    returned = 0;
+    for (int base = 0; base < a.requests; base += kThreads) {
+      const int i = base + tid;
+      Need m{};
+      if (i < a.requests) m = need_of(a, i);
+      // inclusive sum of take over this piece: within the wave, then over the waves
+      int64_t s = m.take();
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int64_t t = __shfl_up(s, d, 64);
+        if ((tid & 63) >= d) s += t;
+      }
+      __syncthreads();
+      if ((tid & 63) == 63) lds[tid >> 6] = s;
+      __syncthreads();
+      int64_t carry = before;
+      for (int w = 0; w < (tid >> 6); ++w) carry += lds[w];
+      const int64_t piece = lds[0] + lds[1] + lds[2] + lds[3];
+      s += carry;
+      const bool ok = s <= count;
+      if (over && i < a.requests && !m.bad) a.out_lengths[i] = ok || m.take() == 0 ? m.next : m.now;
+      fit += i < a.requests && ok ? m.take() : 0;
+      returned += m.give();
+      before += piece;
+    }
+    taken = block_sum(fit, lds);
+    returned = block_sum(returned, lds);
+  }
+  if (tid == 0) {
+    a.out_state[0] = (int)((head + taken) % N);
+    a.out_state[1] = (int)(count - taken + returned);
+    if (over) *a.ticket = 0;
+  }
+}
+
+// ---------------------------------------------------------------- slot writes
+struct WriteArgs {
+  kvmi_cache cache;
+  const uint16_t* rows[2];
+  int64_t token_stride[2], head_stride[2];
+  const int64_t* slots;
+  int64_t tokens;
+  int32_t* err;
+  int lanes_log2;  // lanes of a token, a power of two up to the workgroup
+};
+
+// A group of 2^lanes_log2 lanes copies one token's K and V rows in units of V (16 bytes, or 2
+// where a stride or an address is not aligned): copies, bound by memory.
+template <class V>
+__global__ __launch_bounds__(kThreads) void write_kernel(WriteArgs a) {
+  constexpr int U = sizeof(V) / 2;
+  const int per_head = a.cache.head_dim / U, per_part = a.cache.num_heads * per_head;
+  const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
+  const int64_t tok = ((int64_t)blockIdx.x << (8 - a.lanes_log2)) + (threadIdx.x >> a.lanes_log2);
+  if (tok >= a.tokens) return;
+  const int64_t slot = a.slots[tok];
+  const int S = a.cache.block_size;
+  if (slot < 0 || slot >= (int64_t)a.cache.num_blocks * S) {
+    if (slot != -1 && lane == 0) flag_error(a.err, KVMI_ERR_BLOCK_ID);
+    return;
+  }
+  const int64_t place = (slot / S) * a.cache.block_stride + (slot % S) * a.cache.num_heads * a.cache.head_dim;
+  for (int p = lane; p < 2 * per_part; p += lanes) {
+    const int part = p >= per_part, q = p - part * per_part;
+    const int head = q / per_head;
+    const uint16_t* src = a.rows[part] + tok * a.token_stride[part] + head * a.head_stride[part] +
+                          (int64_t)(q - head * per_head) * U;
+    uint16_t* dst = (uint16_t*)a.cache.base + part * a.cache.part_stride + place + (int64_t)q * U;
+    gst((V*)dst, gld((const V*)src));
+  }
+}
+
+// ---------------------------------------------------------------- kept drafts
+struct KeepArgs {
+  kvmi_cache cache;
+  void* const* bases;
+  const int32_t* tables;
+  const int32_t* lengths;
+  const int32_t* accepted;
+  int32_t* out_lengths;
+  int32_t* err;
+  int columns, width, layers;
+};
+constexpr int kMaxPath = 1024;
+
+// Workgroup (request, layer).  The path is checked as a whole before anything moves.  A thread
+// owns one 16-byte (or 2-byte) column of the row and walks the path in order, so no thread waits
+// for another: path[i] >= i and the path increases, hence a row is read before, or in the same
+// step as, it is overwritten.
+template <class V>
+__global__ __launch_bounds__(kThreads) void keep_kernel(KeepArgs a) {
+  constexpr int U = sizeof(V) / 2, kStep = 8;
+  __shared__ int64_t src[kMaxPath], dst[kMaxPath];
+  __shared__ int count;
+  const int r = blockIdx.x, layer = blockIdx.y, tid = threadIdx.x;
+  const int32_t* path = a.accepted + (int64_t)r * a.width;
+  const int S = a.cache.block_size;
+  const int64_t base = a.lengths[r], top = (int64_t)a.columns * S;
+  if (tid == 0) count = a.width;
+  __syncthreads();
+  for (int i = tid; i < a.width; i += kThreads)
+    if (path[i] < 0) atomicMin(&count, i);
+  __syncthreads();
+  const int n = count;
+  int bad = base < 0 || base > top ? KVMI_ERR_LENGTH : 0;
+  if (!bad)
+    for (int i = tid; i < n; i += kThreads) {
+      const int64_t from = base + path[i], to = base + i;
+      if ((i && path[i] <= path[i - 1]) || from >= top) {
+        bad |= KVMI_ERR_LENGTH;
+        continue;
+      }
+      const int32_t fb = a.tables[(int64_t)r * a.columns + from / S], tb = a.tables[(int64_t)r * a.columns + to / S];
+      if (fb < 0 || fb >= a.cache.num_blocks || tb < 0 || tb >= a.cache.num_blocks) bad |= KVMI_ERR_BLOCK_ID;
+      const int64_t row = (int64_t)a.cache.num_heads * a.cache.head_dim;
+      src[i] = (int64_t)fb * a.cache.block_stride + (from % S) * row;
+      dst[i] = (int64_t)tb * a.cache.block_stride + (to % S) * row;
+    }
+  if (bad && layer == 0) flag_error(a.err, bad);
+  const int any = __syncthreads_or(bad);
+  if (layer == 0 && tid == 0) a.out_lengths[r] = (int)base + (any ? 0 : n);
+  if (any) return;
+  const int per_part = a.cache.num_heads * a.cache.head_dim / U;
+  for (int p = tid; p < 2 * per_part; p += kThreads) {
+    const int part = p >= per_part;
+    uint16_t* col = (uint16_t*)a.bases[layer] + part * a.cache.part_stride + (int64_t)(p - part * per_part) * U;
+    for (int i0 = 0; i0 < n; i0 += kStep) {
+      V held[kStep];
+#pragma unroll
+      for (int i = 0; i < kStep; ++i)
+        if (i0 + i < n && src[i0 + i] != dst[i0 + i]) held[i] = gld((const V*)(col + src[i0 + i]));
+#pragma unroll
+      for (int i = 0; i < kStep; ++i)
+        if (i0 + i < n && src[i0 + i] != dst[i0 + i]) gst((V*)(col + dst[i0 + i]), held[i]);
+    }
+  }
+}
+
+bool cache_ok(const kvmi_cache* c, bool base) {
+  return c && (!base || c->base) && c->num_blocks >= 1 && c->block_size >= 1 && c->num_heads >= 1 && c->head_dim >= 1 &&
+         c->part_stride >= 0 && c->block_stride >= (int64_t)c->block_size * c->num_heads * c->head_dim &&
+         (int64_t)c->num_blocks * c->block_size < 0x7fffffffLL && (int64_t)c->num_heads * c->head_dim < (1 << 24);
+}
+bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+bool strides16(const kvmi_cache* c) {
+  return c->head_dim % 8 == 0 && c->part_stride % 8 == 0 && c->block_stride % 8 == 0;
+}
+int launched() { return hipGetLastError() == hipSuccess ? KVMI_OK : KVMI_ELAUNCH; }
+
+}  // namespace
+}  // namespace kvmi
+
+extern "C" int kvmi_build_tables(const kvmi_tables_args* args, kvmi_stream_t stream) {
+  using namespace kvmi;
+  if (!args) return KVMI_EINVAL;
+  const kvmi_tables_args& a = *args;
+  if (a.requests < 0 || a.columns < 1 || a.ring < 1 || a.block_size < 1 || a.max_tokens < 0) return KVMI_EINVAL;
+  if ((int64_t)a.columns * a.block_size > 0x7fffffffLL || (int64_t)a.ring * a.block_size > 0x7fffffffLL)
+    return KVMI_EINVAL;
+  if (a.requests == 0) return KVMI_OK;
+  if (!a.lengths || !a.new_lengths || !a.tables || !a.free_blocks || !a.state || !a.out_tables || !a.out_lengths ||
+      !a.out_state || !a.starts || (a.max_tokens && !a.slots))
+    return KVMI_EINVAL;
+  const bool over = a.out_lengths == a.lengths;
+  if (over != (a.out_state == a.state) || (over && !a.ticket) || a.new_lengths == a.out_lengths) return KVMI_EINVAL;
+  // one request may own most of the tokens: parts of 4096 slots, up to 64 of them
+  int64_t parts = ((int64_t)a.max_tokens + 4095) / 4096;
+  parts = parts < 1 ? 1 : parts > 64 ? 64 : parts;
+  hipLaunchKernelGGL(tables_kernel, dim3((unsigned)a.requests, (unsigned)parts), dim3(kThreads), 0,
+                     reinterpret_cast<hipStream_t>(stream), a);
+  return launched();
+}
+
+extern "C" int kvmi_write_kv(const kvmi_cache* cache, const void* key, const void* value, int64_t key_token_stride,
+                             int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride,
+                             const int64_t* slots, int64_t tokens, int32_t* err, kvmi_stream_t stream) {
+  using namespace kvmi;
+  if (!cache_ok(cache, true) || tokens < 0) return KVMI_EINVAL;
+  if (tokens == 0) return KVMI_OK;
+  if (!key || !value || !slots) return KVMI_EINVAL;
+  WriteArgs a{*cache,
+              {(const uint16_t*)key, (const uint16_t*)value},
+              {key_token_stride, value_token_stride},
+              {key_head_stride, value_head_stride},
+              slots,
+              tokens,
+              err,
+              8};
+  const bool wide = strides16(cache) && aligned16(cache->base) && aligned16(key) && aligned16(value) &&
+                    key_token_stride % 8 == 0 && key_head_stride % 8 == 0 && value_token_stride % 8 == 0 &&
+                    value_head_stride % 8 == 0;
+  const int units = 2 * cache->num_heads * cache->head_dim / (wide ? 8 : 1);
+  while (a.lanes_log2 > 0 && (1 << (a.lanes_log2 - 1)) >= units) --a.lanes_log2;
+  const int64_t per_wg = kThreads >> a.lanes_log2, grid = (tokens + per_wg - 1) / per_wg;
+  if (grid > 0x7fffffffLL) return KVMI_EINVAL;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (wide)
+    hipLaunchKernelGGL((write_kernel<uint4>), dim3((unsigned)grid), dim3(kThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((write_kernel<uint16_t>), dim3((unsigned)grid), dim3(kThreads), 0, st, a);
+  return launched();
+}
+
+extern "C" int kvmi_keep_drafts(const kvmi_cache* cache, void* const* bases, int32_t layers, const int32_t* tables,
+                                int32_t columns, const int32_t* lengths, const int32_t* accepted, int32_t requests,
+                                int32_t width, int32_t* out_lengths, int32_t* err, kvmi_stream_t stream) {
+  using namespace kvmi;
+  if (!cache_ok(cache, false) || layers < 1 || layers > 65535 || columns < 1 || requests < 0 || width < 0 ||
+      width > kMaxPath || (int64_t)columns * cache->block_size > 0x7fffffffLL)
+    return KVMI_EINVAL;
+  if (requests == 0) return KVMI_OK;
+  if (!bases || !tables || !lengths || !out_lengths || (width && !accepted) || lengths == out_lengths)
+    return KVMI_EINVAL;
+  KeepArgs a{*cache, bases, tables, lengths, accepted, out_lengths, err, columns, width, layers};
+  const dim3 grid((unsigned)requests, (unsigned)layers);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  // `cache->base` tells how the bases are aligned: the caller passes the OR of all of them
+  if (strides16(cache) && aligned16(cache->base))
+    hipLaunchKernelGGL((keep_kernel<uint4>), grid, dim3(kThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((keep_kernel<uint16_t>), grid, dim3(kThreads), 0, st, a);
+  return launched();
+}

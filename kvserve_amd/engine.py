@@ -676,6 +676,10 @@ def packet_groups(packet: Packet) -> int:
 
 def raise_device_error(code: int) -> None:
     """Raise the reference's device-assert messages (bitpack_codec.py:32, :38, :60)."""
+    if code & _lib.ERR_NO_BLOCKS:
+        raise RuntimeError("too few free blocks: a request was refused")
+    if code & _lib.ERR_LENGTH:  # before the block ids: a length too long reads past its blocks
+        raise ValueError("a length, token range or path is out of range")
     if code & _lib.ERR_SYMBOL_RANGE:
         raise RuntimeError("symbol exceeds bitpack_bits")
     if code & _lib.ERR_BAD_HEADER:
