@@ -1,99 +1,333 @@
-// Attention of drafted (or any last) tokens over the paged cache.
-#include "kvmi_common.hpp"
+// Attention of drafted (or any last) tokens over the paged cache: the kernel for few rows, the
+// joining of split sums, and the entry points.
+#include "kvmi_attention.hpp"
+
+#include <algorithm>
 
 namespace kvmi {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kStep = 32;  // keys a wave takes at a time
 
-template <int DT>
-__device__ __forceinline__ float to_f32(uint16_t x) {
-  if constexpr (DT == KVMI_DTYPE_BF16) return bf16_to_f32(x);
-  return (float)__builtin_bit_cast(_Float16, x);
-}
-template <int DT>
-__device__ __forceinline__ uint16_t from_f32(float x) {
-  if constexpr (DT == KVMI_DTYPE_BF16) return (uint16_t)f32_to_bf16_bits(x);
-  return __builtin_bit_cast(uint16_t, (_Float16)x);
-}
+// Few rows (16 * R at most a KV head): bound by reading the cache.  Each wave takes every NW-th
+// 32 keys of the workgroup's part straight from memory into registers:
+//   S^T = K Q^T     a lane has 16 bytes of key l % 16, four lanes 64 bytes of one
+//   O^T += V^T P^T  a lane loads 16 bytes of each of its 8 keys, 16 lanes a whole row of 128
+//                   channels; pairs of keys are brought together by byte permutes, and the
+//                   output row of tile j is channel 8 * row + j
+// so that nothing goes through LDS before the waves' sums are joined at the end.
+// N8 / N4: panels of 128 / 64 channels.
+template <int DT, int N8, int N4, int R>
+__global__ __launch_bounds__(512, 2) void attend_rows_kernel(kvmi_attention_args a, AttendPlan plan) {
+  constexpr int KS = 4 * N8 + 2 * N4, OT = 8 * N8 + 4 * N4;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // [waves][rows][D] sums
+  __shared__ int64_t offs[8][2][kStep];
+  __shared__ float2 stat[8][16 * R];
 
-// One wave a query row: 64 keys at a time, a lane a key for the scores, a lane four channels
-// for the sums.
-template <int DT>
-__global__ __launch_bounds__(64) void attend_kernel(kvmi_attention_args a) {
-  __shared__ float q[256], w[64];
-  __shared__ int64_t at[64];
-  const int lane = threadIdx.x, r = blockIdx.y;
-  const int i = blockIdx.x / a.query_heads, head = blockIdx.x % a.query_heads;
-  const int D = a.cache.head_dim, S = a.cache.block_size;
-  int s0 = a.starts[r], s1 = a.starts[r + 1], err = 0;
-  if (s0 < 0 || s1 < s0 || s1 > a.total_queries || s1 - s0 > a.max_query) err |= KVMI_ERR_LENGTH;
-  s0 = min(max(s0, 0), a.total_queries);
-  s1 = min(max(s1, s0), a.total_queries);
-  int L = a.lengths[r];
-  const int top = a.columns * S;
-  if (L < 0 || L > top) err |= KVMI_ERR_LENGTH;
-  L = min(max(L, 0), top);
-  if (err && a.err && lane == 0) atomicOr(a.err, err);
-  const int T = s1 - s0, prefix = L - T;
-  if (i >= T) return;
-  const int64_t row = s0 + i;
-  const uint16_t* qp = (const uint16_t*)a.query + row * a.query_token_stride + head * a.query_head_stride;
-  for (int d = lane; d < D; d += 64) q[d] = to_f32<DT>(qp[d]);
-  __syncthreads();
-  const uint16_t* base = (const uint16_t*)a.cache.base + (head / (a.query_heads / a.cache.num_heads)) * D;
-  const float c = a.scale * kLog2e;
-  float m = -INFINITY, l = 0, o[4] = {0, 0, 0, 0};
-  const int end = a.mask ? L : min(L, prefix + i + 1);
-  for (int p0 = 0; p0 < end; p0 += 64) {
-    const int p = p0 + lane;
-    bool seen = p < end;
-    int64_t off = 0;
-    float s = -INFINITY;
-    if (seen) {
-      int id = a.tables[(int64_t)r * a.columns + p / S];
-      if (id < 0 || id >= a.cache.num_blocks) {
-        if (a.err) atomicOr(a.err, KVMI_ERR_BLOCK_ID);
-        id = min(max(id, 0), a.cache.num_blocks - 1);
-      }
-      off = (int64_t)id * a.cache.block_stride + (int64_t)(p % S) * a.cache.num_heads * D;
-      const int j = p - prefix;
-      if (a.mask && j >= 0)
-        seen = j < a.mask_words * 64 && ((a.mask[row * a.mask_words + j / 64] >> (j % 64)) & 1);
-    }
-    if (seen) {
-      s = 0;
-      for (int d = 0; d < D; ++d) s += q[d] * to_f32<DT>(base[off + d]);
-      s *= c;
-    }
-    float mx = s;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int col = lane & 15, g = lane >> 4;
+  const int head = blockIdx.x, part = blockIdx.y, r = blockIdx.z;
+  const Request q = request_of(a, r, threadIdx.x == 0);
+  const int D = a.cache.head_dim, H = a.cache.num_heads, G = a.query_heads / H;
+  const int M = min(q.queries, a.max_query) * G;
+  if (M == 0) return;
+  const int parts = parts_of(plan, q.length);
+  if (part >= parts) return;
+  const uint16_t* const keys = (const uint16_t*)a.cache.base + head * D;
+  const uint16_t* const values = keys + a.cache.part_stride;
+
+  u32x4v qf[R][KS];
+  int qi[R];
+  const uint64_t* mask[R];
 #pragma unroll
-    for (int d = 32; d; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
-    const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.0f : mn;
-    const float f = __builtin_amdgcn_exp2f(m - ms), x = seen ? __builtin_amdgcn_exp2f(s - ms) : 0.0f;
-    m = mn;
-    l = l * f + x;
-    __syncthreads();
-    w[lane] = x;
-    at[lane] = seen ? off : -1;
-    __syncthreads();
+  for (int x = 0; x < R; ++x) {
+    const int m = min(16 * x + col, M - 1);
+    qi[x] = m / G;
+    const int64_t row = q.first + qi[x];
+    mask[x] = a.mask ? a.mask + row * a.mask_words : nullptr;
+    const uint16_t* qp = (const uint16_t*)a.query + row * a.query_token_stride +
+                         (head * G + m - qi[x] * G) * a.query_head_stride;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] *= f;
-    for (int t = 0; t < 64; ++t) {
-      if (at[t] < 0) continue;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (lane + 64 * k < D) o[k] += w[t] * to_f32<DT>(base[a.cache.part_stride + at[t] + lane + 64 * k]);
+    for (int k = 0; k < KS; ++k) {
+      const int d = 32 * k + 8 * g;
+      qf[x][k] = d < D ? ld16(qp + d) : u32x4v{0, 0, 0, 0};
     }
   }
+  const float c = a.scale * kLog2e;
+  float mx[R], l[R];
+  f32x4 o[R][OT];
 #pragma unroll
-  for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d, 64);
-  uint16_t* out = (uint16_t*)a.out + (row * a.query_heads + head) * D;
+  for (int x = 0; x < R; ++x) {
+    mx[x] = -INFINITY;
+    l[x] = 0;
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (lane + 64 * k < D) out[lane + 64 * k] = from_f32<DT>(l == 0 ? 0.0f : o[k] / l);
-  if (a.lse && lane == 0)
-    a.lse[row * a.query_heads + head] = l == 0 ? -INFINITY : (m + __builtin_amdgcn_logf(l)) / kLog2e;
+    for (int j = 0; j < OT; ++j) o[x][j] = f32x4{0, 0, 0, 0};
+  }
+
+  const int end = q.length, all = a.mask ? q.prefix : q.prefix + 1;  // seen by some row, by all
+  const int steps = (q.length + kStep - 1) / kStep;
+  const int t0 = (int)((int64_t)steps * part / parts) + wave, t1 = (int)((int64_t)steps * (part + 1) / parts);
+
+  auto lookup = [&](int t) -> int64_t {
+    const int p = t * kStep + (lane & 31);
+    return t < t1 && p < end ? token_offset(a, r, p) : 0;
+  };
+  u32x4v kf[2][KS], v8[8][N8 ? N8 : 1];
+  u32x2v v4[8];
+  auto load_keys = [&](const int64_t* at) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const uint16_t* kp = keys + at[16 * b + col];
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int d = 32 * k + 8 * g;
+        kf[b][k] = ld16(kp + (d < D ? d : 0));
+      }
+    }
+  };
+  auto load_values = [&](const int64_t* at) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint16_t* vp = values + at[16 * (i >> 2) + 4 * g + (i & 3)];
+#pragma unroll
+      for (int n = 0; n < N8; ++n) {
+        const int d = 128 * n + 8 * col;
+        v8[i][n] = ld16(vp + (d < D ? d : 0));
+      }
+      if constexpr (N4 != 0) {
+        const int d = 128 * N8 + 4 * col;
+        v4[i] = ld8(vp + (d < D ? d : 0));
+      }
+    }
+  };
+
+  int64_t* const mine = offs[wave][0];
+  if (t0 < t1) {
+    if (lane < kStep) mine[lane] = lookup(t0);
+    __builtin_amdgcn_wave_barrier();
+    load_keys(mine);
+    load_values(mine);
+  }
+  int buf = 0;
+  for (int t = t0; t < t1; t += waves) {
+    const int p0 = t * kStep;
+    if (lane < kStep) mine[(buf ^ 1) * kStep + lane] = lookup(t + waves);
+    f32x4 s[R][2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int x = 0; x < R; ++x) {
+        s[x][b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) s[x][b] = mma16<DT>(kf[b][k], qf[x][k], s[x][b]);
+      }
+    __builtin_amdgcn_wave_barrier();
+    const int64_t* const next = mine + (buf ^ 1) * kStep;
+    load_keys(next);
+    const bool masked = p0 + kStep > all || p0 + kStep > end;
+    uint32_t seen[R];
+#pragma unroll
+    for (int x = 0; x < R; ++x) {
+      seen[x] = ~0u;
+      if (masked) {
+        seen[x] = (uint32_t)seen_bits(q, mask[x], a.mask_words, qi[x], p0);
+        const uint32_t v = seen[x] >> (4 * g);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[x][b][i] = (v >> (16 * b + i)) & 1 ? s[x][b][i] : -INFINITY;
+      }
+    }
+    u32x4v pf[R];
+#pragma unroll
+    for (int x = 0; x < R; ++x) {
+      float top = fmaxf(fmaxf(fmaxf(s[x][0][0], s[x][0][1]), fmaxf(s[x][0][2], s[x][0][3])),
+                        fmaxf(fmaxf(s[x][1][0], s[x][1][1]), fmaxf(s[x][1][2], s[x][1][3])));
+      top = join32(join16(top, Larger()), Larger()) * c;
+      const bool raise = top > mx[x] + kRaise;
+      if (__ballot(raise)) {
+        const float f = raise ? __builtin_amdgcn_exp2f(mx[x] - top) : 1.0f;
+        mx[x] = raise ? top : mx[x];
+        l[x] *= f;
+#pragma unroll
+        for (int j = 0; j < OT; ++j) o[x][j] *= f;
+      }
+      const float ms = mx[x] == -INFINITY ? 0.0f : mx[x];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[x][b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][b][i], c, -ms));
+        l[x] += (s[x][b][0] + s[x][b][1]) + (s[x][b][2] + s[x][b][3]);
+        pf[x][2 * b] = pack2<DT>(s[x][b][0], s[x][b][1]);
+        pf[x][2 * b + 1] = pack2<DT>(s[x][b][2], s[x][b][3]);
+      }
+    }
+    if (masked) {
+      // a weight of zero has to give zero: values past the end, and those that are not finite,
+      // leave the product; the latter then go to the rows that see them
+      uint32_t bad = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = 16 * (i >> 2) + 4 * g + (i & 3);
+        bool odd = false;
+        const bool in = p0 + key < end;
+#pragma unroll
+        for (int n = 0; n < N8; ++n)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t f = in ? finite2<DT>(v8[i][n][w]) : 0;
+            odd |= in && f != v8[i][n][w];
+            v8[i][n][w] = f;
+          }
+        if constexpr (N4 != 0) {
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t f = in ? finite2<DT>(v4[i][w]) : 0;
+            odd |= in && f != v4[i][w];
+            v4[i][w] = f;
+          }
+        }
+        const uint64_t b = __ballot(odd);
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if ((b >> (16 * y)) & 0xffff) bad |= 1u << (16 * (i >> 2) + 4 * y + (i & 3));
+      }
+      bad = __builtin_amdgcn_readfirstlane(bad);
+#pragma unroll 1
+      while (bad) {
+        const int key = __builtin_ctz(bad), at = (key >> 4) * 4 + (key & 3);
+        bad &= bad - 1;
+        const uint16_t* const vp = values + mine[buf * kStep + key];
+#pragma unroll
+        for (int x = 0; x < R; ++x) {
+          float p = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p = i == at ? s[x][i >> 2][i & 3] : p;
+          p = __shfl(p, col + 16 * ((key >> 2) & 3), 64);
+          const bool sees = (seen[x] >> key) & 1;
+          const int g0 = here(g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int n = 0; n < N8; ++n) {
+              const u32x4v v = ld16(vp + min(128 * n + 8 * (4 * g0 + i), D - 8));
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                o[x][8 * n + j][i] += sees ? odd_term<DT>(p, v[j >> 1] >> (16 * (j & 1))) : 0.0f;
+            }
+            if constexpr (N4 != 0) {
+              const u32x2v v = ld8(vp + min(128 * N8 + 4 * (4 * g0 + i), D - 4));
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                o[x][8 * N8 + j][i] += sees ? odd_term<DT>(p, v[j >> 1] >> (16 * (j & 1))) : 0.0f;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < OT; ++j) {
+      const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
+      u32x4v f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if (j < 8 * N8)
+          f[w] = __builtin_amdgcn_perm(v8[2 * w + 1][j >> 3][(j & 7) >> 1], v8[2 * w][j >> 3][(j & 7) >> 1], sel);
+        else
+          f[w] = __builtin_amdgcn_perm(v4[2 * w + 1][(j & 3) >> 1], v4[2 * w][(j & 3) >> 1], sel);
+      }
+#pragma unroll
+      for (int x = 0; x < R; ++x) o[x][j] = mma16<DT>(f, pf[x], o[x][j]);
+    }
+    load_values(next);
+    buf ^= 1;
+  }
+
+  // the waves' sums, brought to their common maximum and added up in the waves' order
+  const int rows = min(M, 16 * R), DP = D + 4;
+  float* const sums = (float*)lds;
+#pragma unroll
+  for (int x = 0; x < R; ++x) {
+    l[x] = join32(join16(l[x], Plus()), Plus());
+    if (g == 0) stat[wave][16 * x + col] = make_float2(mx[x], l[x]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < R; ++x) {
+    const int m = 16 * x + col;
+    float top = -INFINITY;
+    for (int w = 0; w < waves; ++w) top = fmaxf(top, stat[w][m].x);
+    const float f = mx[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx[x] - top);
+    if (m < rows) {
+      float* const dst = sums + (wave * rows + m) * DP;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int n = 0; n < 2 * N8; ++n) {
+          const int d = 128 * (n >> 1) + 8 * (4 * g + i) + 4 * (n & 1), j = 4 * n;
+          if (d < D) *(f32x4*)(dst + d) = f32x4{o[x][j][i], o[x][j + 1][i], o[x][j + 2][i], o[x][j + 3][i]} * f;
+        }
+        if constexpr (N4 != 0) {
+          constexpr int j = 8 * N8;
+          const int d = 128 * N8 + 4 * (4 * g + i);
+          if (d < D) *(f32x4*)(dst + d) = f32x4{o[x][j][i], o[x][j + 1][i], o[x][j + 2][i], o[x][j + 3][i]} * f;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < rows * (D / 4); e += blockDim.x) {
+    const int m = e / (D / 4), d = 4 * (e - m * (D / 4));
+    float top = -INFINITY, total = 0;
+    for (int w = 0; w < waves; ++w) top = fmaxf(top, stat[w][m].x);
+    f32x4 v = {0, 0, 0, 0};
+    for (int w = 0; w < waves; ++w) {
+      const float2 s = stat[w][m];
+      total += s.x == -INFINITY ? 0.0f : s.y * __builtin_amdgcn_exp2f(s.x - top);
+      v += *(const f32x4*)(sums + (w * rows + m) * DP + d);
+    }
+    const int i = m / G;
+    const int64_t out_row = (int64_t)(q.first + i) * a.query_heads + head * G + m - i * G;
+    if (parts == 1) {
+      const float f = total == 0 ? 0.0f : 1.0f / total;
+      gst((uint2*)((uint16_t*)a.out + out_row * D + d),
+          make_uint2(pack2<DT>(v[0] * f, v[1] * f), pack2<DT>(v[2] * f, v[3] * f)));
+      if (a.lse && d == 0) a.lse[out_row] = total == 0 ? -INFINITY : (top + __builtin_amdgcn_logf(total)) / kLog2e;
+    } else {
+      *(KVMI_GLOBAL f32x4*)(plan.sums + (out_row * plan.splits + part) * D + d) = v;
+      if (d == 0) plan.stats[out_row * plan.splits + part] = make_float2(top, total);
+    }
+  }
+}
+
+// The parts of each query head of a request that was split, joined in their order.  D / 4
+// lanes (a power of two at least) a row.
+template <int DT>
+__global__ __launch_bounds__(256) void join_kernel(kvmi_attention_args a, AttendPlan plan, int lanes) {
+  const int r = blockIdx.y, D = a.cache.head_dim;
+  const Request q = request_of(a, r, false);
+  const int parts = parts_of(plan, q.length);
+  if (parts == 1) return;
+  const int e = blockIdx.x * (256 / lanes) + threadIdx.x / lanes, d = 4 * (threadIdx.x % lanes);
+  if (e >= min(q.queries, a.max_query) * a.query_heads || d >= D) return;
+  const int64_t row = (int64_t)q.first * a.query_heads + e;
+  const float2* const stats = plan.stats + row * plan.splits;
+  const float* const sums = plan.sums + row * plan.splits * D + d;
+  float top = -INFINITY, total = 0;
+  for (int s = 0; s < parts; ++s) top = fmaxf(top, stats[s].x);
+  f32x4 v = {0, 0, 0, 0};
+  for (int s = 0; s < parts; ++s) {
+    const float2 st = stats[s];
+    if (st.x == -INFINITY) continue;
+    const float f = __builtin_amdgcn_exp2f(st.x - top);
+    total += st.y * f;
+    v += *(const KVMI_GLOBAL f32x4*)(sums + (int64_t)s * D) * f;
+  }
+  const float f = total == 0 ? 0.0f : 1.0f / total;
+  gst((uint2*)((uint16_t*)a.out + row * D + d),
+      make_uint2(pack2<DT>(v[0] * f, v[1] * f), pack2<DT>(v[2] * f, v[3] * f)));
+  if (a.lse && d == 0) a.lse[row] = total == 0 ? -INFINITY : (top + __builtin_amdgcn_logf(total)) / kLog2e;
 }
 
 bool attention_ok(const kvmi_attention_args* a) {
@@ -108,17 +342,75 @@ bool attention_ok(const kvmi_attention_args* a) {
       (a->dtype != KVMI_DTYPE_BF16 && a->dtype != KVMI_DTYPE_FP16) || !(a->scale > 0) || a->scale > 3.0e38f)
     return false;
   if ((int64_t)a->columns * c.block_size > 0x7fffffffLL || (int64_t)c.num_blocks * c.block_size > 0x7fffffffLL ||
-      (int64_t)a->max_query * a->query_heads > 0x7fffffffLL)
+      (int64_t)a->max_query * a->query_heads > 0x7fffffffLL ||
+      (int64_t)c.block_size * c.num_heads * c.head_dim > 0x7fffffffLL)
     return false;
   if (a->mask && a->mask_words < 1) return false;
   return true;
+}
+
+struct Choice {
+  bool rows;     // the kernel for few rows
+  int waves;     // its waves a workgroup
+  int row_groups;
+  AttendPlan plan;
+};
+int64_t parts_bytes(const kvmi_attention_args& a, int splits) {
+  const int64_t rows = (int64_t)a.total_queries * a.query_heads * splits;
+  return splits == 1 ? 0 : rows * (a.cache.head_dim * 4 + 8);
+}
+Choice choose(const kvmi_attention_args& a) {
+  Choice c{};
+  const int G = a.query_heads / a.cache.num_heads, D = a.cache.head_dim;
+  const int64_t rows = (int64_t)a.max_query * G;
+  c.row_groups = rows <= 16 ? 1 : 2;
+  c.rows = rows <= (D <= 128 ? 32 : 16);
+  const int64_t length = a.max_length < 1 ? 1 : a.max_length;
+  c.plan.row_tiles = c.rows ? 1 : (int)((rows + 127) / 128);
+  const int64_t groups = (int64_t)a.requests * a.cache.num_heads * c.plan.row_tiles;
+  c.plan.chunk = c.rows ? 1024 : 512;
+  int64_t splits = (length + c.plan.chunk - 1) / c.plan.chunk;
+  if (!c.rows) splits = splits < (1024 + groups - 1) / groups ? splits : (1024 + groups - 1) / groups;
+  splits = splits > 64 ? 64 : splits;
+  if (!c.rows && splits > 1) c.plan.chunk = (int)((length + splits - 1) / splits);
+  while (splits > 1 && ((int64_t)c.plan.row_tiles * splits > 65535 || parts_bytes(a, (int)splits) > (1LL << 31))) splits /= 2;
+  c.plan.splits = (int)splits;
+  c.waves = 4;
+  return c;
+}
+
+template <int DT>
+void launch_rows(const kvmi_attention_args& a, const Choice& c, hipStream_t st) {
+  const int D = a.cache.head_dim, G = a.query_heads / a.cache.num_heads;
+  const int rows = std::min(16 * c.row_groups, a.max_query * G);
+  const dim3 grid((unsigned)a.cache.num_heads, (unsigned)c.plan.splits, (unsigned)a.requests);
+  const dim3 threads((unsigned)(64 * c.waves));
+  const size_t lds = (size_t)c.waves * rows * (D + 4) * 4;
+#define KVMI_ROWS(N8, N4, R) \
+  hipLaunchKernelGGL((attend_rows_kernel<DT, N8, N4, R>), grid, threads, lds, st, a, c.plan)
+  if (D > 192)
+    KVMI_ROWS(2, 0, 1);
+  else if (D > 128)
+    KVMI_ROWS(1, 1, 1);
+  else if (D > 64 && c.row_groups == 1)
+    KVMI_ROWS(1, 0, 1);
+  else if (D > 64)
+    KVMI_ROWS(1, 0, 2);
+  else if (c.row_groups == 1)
+    KVMI_ROWS(0, 1, 1);
+  else
+    KVMI_ROWS(0, 1, 2);
+#undef KVMI_ROWS
 }
 
 }  // namespace
 }  // namespace kvmi
 
 extern "C" int64_t kvmi_attention_workspace_bytes(const kvmi_attention_args* args) {
-  return kvmi::attention_ok(args) ? 0 : KVMI_EINVAL;
+  using namespace kvmi;
+  if (!attention_ok(args)) return KVMI_EINVAL;
+  if (args->requests == 0 || args->total_queries == 0 || args->max_query == 0) return 0;
+  return parts_bytes(*args, choose(*args).plan.splits);
 }
 
 extern "C" int kvmi_tree_attention(const kvmi_attention_args* args, kvmi_stream_t stream) {
@@ -127,13 +419,35 @@ extern "C" int kvmi_tree_attention(const kvmi_attention_args* args, kvmi_stream_
   const kvmi_attention_args& a = *args;
   if (a.requests == 0 || a.total_queries == 0 || a.max_query == 0) return KVMI_OK;
   if (!a.query || !a.out || !a.tables || !a.lengths || !a.starts || (uintptr_t)a.query % 16 ||
-      a.query_token_stride % 8 || a.query_head_stride % 8)
+      (uintptr_t)a.out % 16 || a.query_token_stride % 8 || a.query_head_stride % 8)
     return KVMI_EINVAL;
-  const dim3 grid((unsigned)(a.max_query * a.query_heads), (unsigned)a.requests);
+  Choice c = choose(a);
+  const int64_t space = parts_bytes(a, c.plan.splits);
+  if (c.plan.row_tiles * (int64_t)c.plan.splits > 65535 ||
+      (space && (!a.workspace || a.workspace_bytes < space || (uintptr_t)a.workspace % 16)))
+    return KVMI_EINVAL;
+  c.plan.sums = (float*)a.workspace;
+  c.plan.stats = (float2*)((uint8_t*)a.workspace +
+                           (int64_t)a.total_queries * a.query_heads * c.plan.splits * a.cache.head_dim * 4);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (a.dtype == KVMI_DTYPE_BF16)
-    hipLaunchKernelGGL((attend_kernel<KVMI_DTYPE_BF16>), grid, dim3(64), 0, st, a);
-  else
-    hipLaunchKernelGGL((attend_kernel<KVMI_DTYPE_FP16>), grid, dim3(64), 0, st, a);
+  const bool bf16 = a.dtype == KVMI_DTYPE_BF16;
+  if (!c.rows) {
+    const int rc = attend_tiles(a, c.plan, st);
+    if (rc != KVMI_OK) return rc;
+  } else if (bf16) {
+    launch_rows<KVMI_DTYPE_BF16>(a, c, st);
+  } else {
+    launch_rows<KVMI_DTYPE_FP16>(a, c, st);
+  }
+  if (c.plan.splits > 1) {
+    int lanes = 2;
+    while (4 * lanes < a.cache.head_dim) lanes *= 2;
+    const int64_t rows = (int64_t)a.max_query * a.query_heads;
+    const dim3 grid((unsigned)((rows + 256 / lanes - 1) / (256 / lanes)), (unsigned)a.requests);
+    if (bf16)
+      hipLaunchKernelGGL((join_kernel<KVMI_DTYPE_BF16>), grid, dim3(256), 0, st, a, c.plan, lanes);
+    else
+      hipLaunchKernelGGL((join_kernel<KVMI_DTYPE_FP16>), grid, dim3(256), 0, st, a, c.plan, lanes);
+  }
   return hipGetLastError() == hipSuccess ? KVMI_OK : KVMI_ELAUNCH;
 }

@@ -1,0 +1,306 @@
+// Attention over the paged cache for many rows: tiles of 128 query rows against 64 keys.
+//
+// The rows of a KV head are its queries' heads, row m = query m / G, head m % G.  A wave holds
+// 32 rows as the columns of its matrix products:
+//   S^T = K Q^T     [64 keys][32 rows], operands K (LDS, 16 bytes a lane) and Q (registers)
+//   O^T += V^T P^T  [D][32 rows], V^T by transposing reads of V's rows in LDS
+// so that a lane has half of one row's scores, the softmax needs one exchange between the two
+// halves of the wave, and the scores, rounded to the type, are the second product's operand
+// where they lie: its key order within 16 is the one in which the first product left them.
+#include "kvmi_attention.hpp"
+
+namespace kvmi {
+namespace {
+
+constexpr int kRows = 128, kKeys = 64;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ u32x2v read_transposed(const uint8_t* p) {
+  return __builtin_bit_cast(
+      u32x2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+
+// NT: 32-channel tiles of a head, D <= 32 * NT.
+template <int DT, int NT>
+__global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi_attention_args a, AttendPlan plan) {
+  // K rows an odd number of 16 bytes apart, V rows an odd number of 64: reads of 16 rows in
+  // one column, and of 4 rows by 64 bytes, then meet every bank once
+  constexpr int KS = 64 * NT + 16, VS = 64 * (NT | 1), kBuf = kKeys * (KS + VS), PC = 4 * NT;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kBuf];
+  // of tile t in place t % 3: each key's offset in the cache (looked up two tiles ahead), and the
+  // keys with a value that is not finite
+  __shared__ int64_t offs[3][kKeys];
+  __shared__ uint32_t odd[3][2];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int head = blockIdx.x, r = blockIdx.z;
+  const int tile = plan.row_tiles - 1 - (int)blockIdx.y % plan.row_tiles, part = blockIdx.y / plan.row_tiles;
+  const Request q = request_of(a, r, tid == 0);
+  const int D = a.cache.head_dim, H = a.cache.num_heads, G = a.query_heads / H;
+  const int M = min(q.queries, a.max_query) * G, m0 = tile * kRows;
+  if (m0 >= M) return;
+  const int parts = parts_of(plan, q.length);
+  if (part >= parts) return;
+  const uint64_t* const masks = a.mask;
+  const uint16_t* const keys = (const uint16_t*)a.cache.base + head * D;
+  const uint16_t* const values = keys + a.cache.part_stride;
+
+  // keys that any row of the workgroup sees end at `end`; those before `all` are seen by all
+  const int last_row = min(m0 + kRows, M) - 1;
+  const int end = masks ? q.length : min(q.length, q.prefix + last_row / G + 1);
+  const int all = masks ? q.prefix : q.prefix + m0 / G + 1;
+  const int w0 = m0 + 32 * wave;
+  const bool idle = w0 >= M;
+  const int w_all = masks ? q.prefix : q.prefix + w0 / G + 1;
+  const int w_end = masks ? end : min(end, q.prefix + min(w0 + 31, M - 1) / G + 1);
+  const int tiles = (q.length + kKeys - 1) / kKeys;
+  const int t0 = (int)((int64_t)tiles * part / parts);
+  const int t1 = min((int)((int64_t)tiles * (part + 1) / parts), (end + kKeys - 1) / kKeys);
+
+  // this lane's row
+  const int m = min(w0 + col, M - 1), qi = m / G, qh = head * G + m - qi * G;
+  const int64_t row = q.first + qi;
+  const uint64_t* const mask = masks ? masks + row * a.mask_words : nullptr;
+  u32x4v qf[2 * NT];
+  {
+    const uint16_t* qp = (const uint16_t*)a.query + row * a.query_token_stride + qh * a.query_head_stride;
+#pragma unroll
+    for (int k = 0; k < 2 * NT; ++k) {
+      const int d = 16 * k + 8 * half;
+      qf[k] = d < D ? ld16(qp + d) : u32x4v{0, 0, 0, 0};
+    }
+  }
+  const float c = a.scale * kLog2e;
+  float mx = -INFINITY, l = 0;
+  f32x16 o[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) o[n][x] = 0;
+
+  auto lookup = [&](int t) -> int64_t {  // the first wave's lanes, a key each
+    const int p = t * kKeys + lane;
+    return p < end ? token_offset(a, r, p) : 0;
+  };
+  u32x4v rk[NT], rv[NT];
+  auto load = [&](int t) {
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+      const int idx = tid + 256 * k, key = idx / PC, d = (idx - key * PC) * 8;
+      const int64_t off = offs[t % 3][key] + (d < D ? d : 0);
+      rk[k] = ld16(keys + off);
+      rv[k] = ld16(values + off);
+    }
+  };
+  auto store = [&](int t) {
+    uint8_t* const kb = lds + (t & 1) * kBuf;
+    uint8_t* const vb = kb + kKeys * KS;
+    const int left = end - t * kKeys;
+    if (left < kKeys || t * kKeys + kKeys > all) {
+      // some row does not see some key here: its weight is zero, and so must its product be
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        const int idx = tid + 256 * k, key = idx / PC, d = (idx - key * PC) * 8;
+        if (key >= left) rv[k] = u32x4v{0, 0, 0, 0};
+        u32x4v f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) f[x] = finite2<DT>(rv[k][x]);
+        if (d < D && (f[0] != rv[k][0] || f[1] != rv[k][1] || f[2] != rv[k][2] || f[3] != rv[k][3]))
+          atomicOr(&odd[t % 3][key >> 5], 1u << (key & 31));
+        rv[k] = f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+      const int idx = tid + 256 * k, key = idx / PC, ch = idx - key * PC;
+      if (ch * 8 < D) {
+        *(u32x4v*)(kb + key * KS + ch * 16) = rk[k];
+        *(u32x4v*)(vb + key * VS + ch * 16) = rv[k];
+      }
+    }
+  };
+
+  if (t0 < t1) {
+    if (D < 32 * NT) {  // channels behind the head's are zero once and for all
+      for (int x = tid; x < 2 * kKeys * PC; x += 256) {
+        const int key = x / PC, ch = x - key * PC;
+        uint8_t* const kb = lds + (key >> 6) * kBuf;
+        if (ch * 8 >= D) {
+          *(u32x4v*)(kb + (key & 63) * KS + ch * 16) = u32x4v{0, 0, 0, 0};
+          *(u32x4v*)(kb + kKeys * KS + (key & 63) * VS + ch * 16) = u32x4v{0, 0, 0, 0};
+        }
+      }
+    }
+    if (tid < 6) odd[tid >> 1][tid & 1] = 0;
+    if (wave == 0) {
+      offs[t0 % 3][lane] = lookup(t0);
+      offs[(t0 + 1) % 3][lane] = lookup(t0 + 1);
+    }
+    __syncthreads();
+    load(t0);
+    store(t0);
+    __syncthreads();
+  }
+  for (int t = t0; t < t1; ++t) {
+    int64_t ahead = 0;
+    if (t + 1 < t1) load(t + 1);
+    if (wave == 0) ahead = lookup(t + 2);
+    if (tid < 2) odd[(t + 2) % 3][tid] = 0;
+    const int p0 = t * kKeys;
+    if (!idle && p0 < w_end) {
+      const uint8_t* const kb = lds + (t & 1) * kBuf;
+      const uint8_t* const vb = kb + kKeys * KS;
+      f32x16 s[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) s[b][x] = 0;
+#pragma unroll
+        for (int k = 0; k < 2 * NT; ++k)
+          s[b] = mma32<DT>(*(const u32x4v*)(kb + (32 * b + col) * KS + (2 * k + half) * 16), qf[k], s[b]);
+      }
+      uint64_t seen = ~0ull;
+      if (p0 + kKeys > w_all || p0 + kKeys > q.length) {
+        seen = seen_bits(q, mask, a.mask_words, qi, p0);
+        const uint64_t mine = seen >> (4 * half);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            s[b][x] = (mine >> (32 * b + 8 * (x / 4) + x % 4)) & 1 ? s[b][x] : -INFINITY;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) top = fmaxf(top, s[b][x]);
+      top = join32(top, Larger()) * c;
+      const bool raise = top > mx + kRaise;
+      if (__ballot(raise)) {
+        const float f = raise ? __builtin_amdgcn_exp2f(mx - top) : 1.0f;
+        mx = raise ? top : mx;
+        l *= f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[n][x] *= f;
+      }
+      const float ms = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) s[b][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][x], c, -ms));
+      float sum[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) sum[x & 3] += s[b][x];
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      u32x4v pf[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          pf[k][x] = pack2<DT>(s[k >> 1][8 * (k & 1) + 2 * x], s[k >> 1][8 * (k & 1) + 2 * x + 1]);
+      uint64_t bad = odd[t % 3][0] | (uint64_t)odd[t % 3][1] << 32;
+      bad = __builtin_amdgcn_readfirstlane((uint32_t)bad) |
+            (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(bad >> 32)) << 32;
+#pragma unroll 1
+      while (bad) {  // values that are not finite, to the rows that see them only
+        const int key = __builtin_ctzll(bad), at = (key >> 5) * 16 + ((key >> 3) & 3) * 4 + (key & 3);
+        bad &= bad - 1;
+        float p = 0;
+#pragma unroll
+        for (int x = 0; x < 32; ++x) p = x == at ? s[x >> 4][x & 15] : p;
+        p = __shfl(p, col + 32 * ((key >> 2) & 1), 64);
+        const bool sees = (seen >> key) & 1;
+        const uint16_t* const vp = values + offs[t % 3][key];
+        const int d0 = 4 * here(half);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const u32x2v v = ld8(vp + min(d0 + 32 * n + 8 * x, D - 4));
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              o[n][4 * x + y] += sees ? odd_term<DT>(p, v[y >> 1] >> (16 * (y & 1))) : 0.0f;
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      const uint8_t* const vl = vb + (4 * half + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const u32x2v lo = read_transposed(vl + 16 * k * VS + 64 * n);
+          const u32x2v hi = read_transposed(vl + (16 * k + 8) * VS + 64 * n);
+          o[n] = mma32<DT>(u32x4v{lo.x, lo.y, hi.x, hi.y}, pf[k], o[n]);
+        }
+    }
+    if (t + 1 < t1) store(t + 1);
+    if (wave == 0) offs[(t + 2) % 3][lane] = ahead;
+    __syncthreads();
+  }
+
+  l = join32(l, Plus());
+  if (idle || w0 + col >= M) return;
+  const int64_t out_row = row * a.query_heads + qh;
+  if (parts == 1) {
+    const float f = l == 0 ? 0.0f : 1.0f / l;
+    uint16_t* const op = (uint16_t*)a.out + out_row * D;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int d = 32 * n + 8 * x + 4 * half;
+        if (d < D)
+          gst((uint2*)(op + d), make_uint2(pack2<DT>(o[n][4 * x] * f, o[n][4 * x + 1] * f),
+                                           pack2<DT>(o[n][4 * x + 2] * f, o[n][4 * x + 3] * f)));
+      }
+    if (a.lse && half == 0) a.lse[out_row] = l == 0 ? -INFINITY : (mx + __builtin_amdgcn_logf(l)) / kLog2e;
+  } else {
+    float* const op = plan.sums + (out_row * plan.splits + part) * D;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int d = 32 * n + 8 * x + 4 * half;
+        if (d < D)
+          *(KVMI_GLOBAL f32x4*)(op + d) = f32x4{o[n][4 * x], o[n][4 * x + 1], o[n][4 * x + 2], o[n][4 * x + 3]};
+      }
+    if (half == 0) plan.stats[out_row * plan.splits + part] = make_float2(mx, l);
+  }
+}
+
+template <int DT>
+void launch(const kvmi_attention_args& a, const AttendPlan& p, hipStream_t st) {
+  const dim3 grid((unsigned)a.cache.num_heads, (unsigned)(p.row_tiles * p.splits), (unsigned)a.requests);
+  const int tiles = (a.cache.head_dim + 31) / 32;
+#define KVMI_TILES(N) hipLaunchKernelGGL((attend_tiles_kernel<DT, N>), grid, dim3(256), 0, st, a, p)
+  if (tiles <= 2)
+    KVMI_TILES(2);
+  else if (tiles == 3)
+    KVMI_TILES(3);
+  else if (tiles == 4)
+    KVMI_TILES(4);
+  else if (tiles == 5)
+    KVMI_TILES(5);
+  else if (tiles == 6)
+    KVMI_TILES(6);
+  else
+    KVMI_TILES(8);
+#undef KVMI_TILES
+}
+
+}  // namespace
+
+int attend_tiles(const kvmi_attention_args& a, const AttendPlan& plan, hipStream_t st) {
+  if (a.dtype == KVMI_DTYPE_BF16)
+    launch<KVMI_DTYPE_BF16>(a, plan, st);
+  else
+    launch<KVMI_DTYPE_FP16>(a, plan, st);
+  return hipGetLastError() == hipSuccess ? KVMI_OK : KVMI_ELAUNCH;
+}
+
+}  // namespace kvmi
