@@ -20,17 +20,36 @@ __device__ __forceinline__ u32x2v read_transposed(const uint8_t* p) {
       u32x2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
 
+// Where chunk c (8 channels) of a key's row lies in its row in LDS.  The rows are PC chunks
+// without gaps, since loads that go straight to LDS write 1 KiB in order, and are turned so that
+// the reads meet every bank once: K's, one chunk of 16 keys, by single chunks, V's, 4 chunks of
+// 4 keys, by 4.
+template <int PC>
+struct Turn {
+  static constexpr int kPer = PC % 16 == 0 ? 16 : PC % 8 == 0 ? 8 : 4;  // gcd(PC, 16)
+  static constexpr bool kPow2 = (PC & (PC - 1)) == 0;
+  static __device__ __forceinline__ int key(int row) { return row / (16 / kPer) % kPer; }
+  static __device__ __forceinline__ int value(int row) { return kPer < 8 ? 0 : kPer == 8 ? row / 2 % 2 * 4 : row % 4 * 4; }
+  static __device__ __forceinline__ int place(int c, int turn) {
+    if (kPow2) return c ^ turn;
+    return c + turn >= PC ? c + turn - PC : c + turn;
+  }
+  static __device__ __forceinline__ int chunk(int place, int turn) {
+    if (kPow2) return place ^ turn;
+    return place < turn ? place - turn + PC : place - turn;
+  }
+};
+
 // NT: 32-channel tiles of a head, D <= 32 * NT.
 template <int DT, int NT>
 __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi_attention_args a, AttendPlan plan) {
-  // K rows an odd number of 16 bytes apart, V rows an odd number of 64: reads of 16 rows in
-  // one column, and of 4 rows by 64 bytes, then meet every bank once
-  constexpr int KS = 64 * NT + 16, VS = 64 * (NT | 1), kBuf = kKeys * (KS + VS), PC = 4 * NT;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kBuf];
-  // of tile t in place t % 3: each key's offset in the cache (looked up two tiles ahead), and the
-  // keys with a value that is not finite
+  constexpr int PC = 4 * NT, RS = 16 * PC, kPart = kKeys * RS;  // chunks and bytes of a row, bytes of a tile
+  using T = Turn<PC>;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kPart];  // K and V of two tiles
+  // of tile t in place t % 3 each key's offset in the cache (looked up two tiles ahead), in
+  // place t % 2 the keys with a value that is not finite
   __shared__ int64_t offs[3][kKeys];
-  __shared__ uint32_t odd[3][2];
+  __shared__ uint32_t odd[2][2];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
   const int head = blockIdx.x, r = blockIdx.z;
@@ -82,82 +101,82 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
     const int p = t * kKeys + lane;
     return p < end ? token_offset(a, r, p) : 0;
   };
-  u32x4v rk[NT], rv[NT];
-  auto load = [&](int t) {
+  // pieces of 16 bytes in the order of LDS, NT of K's and of V's a lane
+  auto load = [&](int t, int slot) {
+    uint8_t* const kb = lds + (t & 1) * 2 * kPart + wave * NT * 1024;
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
-      const int idx = tid + 256 * k, key = idx / PC, d = (idx - key * PC) * 8;
-      const int64_t off = offs[t % 3][key] + (d < D ? d : 0);
-      rk[k] = ld16(keys + off);
-      rv[k] = ld16(values + off);
-    }
-  };
-  auto store = [&](int t) {
-    uint8_t* const kb = lds + (t & 1) * kBuf;
-    uint8_t* const vb = kb + kKeys * KS;
-    const int left = end - t * kKeys;
-    if (left < kKeys || t * kKeys + kKeys > all) {
-      // some row does not see some key here: its weight is zero, and so must its product be
-#pragma unroll
-      for (int k = 0; k < NT; ++k) {
-        const int idx = tid + 256 * k, key = idx / PC, d = (idx - key * PC) * 8;
-        if (key >= left) rv[k] = u32x4v{0, 0, 0, 0};
-        u32x4v f;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) f[x] = finite2<DT>(rv[k][x]);
-        if (d < D && (f[0] != rv[k][0] || f[1] != rv[k][1] || f[2] != rv[k][2] || f[3] != rv[k][3]))
-          atomicOr(&odd[t % 3][key >> 5], 1u << (key & 31));
-        rv[k] = f;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < NT; ++k) {
-      const int idx = tid + 256 * k, key = idx / PC, ch = idx - key * PC;
-      if (ch * 8 < D) {
-        *(u32x4v*)(kb + key * KS + ch * 16) = rk[k];
-        *(u32x4v*)(vb + key * VS + ch * 16) = rv[k];
-      }
+      const int idx = (wave * NT + k) * 64 + lane, key = idx / PC, place = idx - key * PC;
+      const int64_t off = offs[slot][key];
+      const int ck = T::chunk(place, T::key(key)), cv = T::chunk(place, T::value(key));
+      if (ck * 8 < D)
+        __builtin_amdgcn_global_load_lds((const KVMI_GLOBAL void*)(keys + off + ck * 8),
+                                         (__attribute__((address_space(3))) void*)(kb + k * 1024), 16, 0, 0);
+      if (cv * 8 < D)
+        __builtin_amdgcn_global_load_lds((const KVMI_GLOBAL void*)(values + off + cv * 8),
+                                         (__attribute__((address_space(3))) void*)(kb + kPart + k * 1024), 16, 0, 0);
     }
   };
 
+  int slot = 0;  // t % 3
   if (t0 < t1) {
     if (D < 32 * NT) {  // channels behind the head's are zero once and for all
-      for (int x = tid; x < 2 * kKeys * PC; x += 256) {
-        const int key = x / PC, ch = x - key * PC;
-        uint8_t* const kb = lds + (key >> 6) * kBuf;
-        if (ch * 8 >= D) {
-          *(u32x4v*)(kb + (key & 63) * KS + ch * 16) = u32x4v{0, 0, 0, 0};
-          *(u32x4v*)(kb + kKeys * KS + (key & 63) * VS + ch * 16) = u32x4v{0, 0, 0, 0};
-        }
+      for (int x = tid; x < 4 * kKeys * PC; x += 256) {
+        const int row = x / PC, place = x - row * PC, key = row & 63;
+        if (T::chunk(place, row & 64 ? T::value(key) : T::key(key)) * 8 >= D)
+          *(u32x4v*)(lds + x * 16) = u32x4v{0, 0, 0, 0};
       }
     }
-    if (tid < 6) odd[tid >> 1][tid & 1] = 0;
+    if (tid < 4) odd[tid >> 1][tid & 1] = 0;
     if (wave == 0) {
-      offs[t0 % 3][lane] = lookup(t0);
-      offs[(t0 + 1) % 3][lane] = lookup(t0 + 1);
+      offs[0][lane] = lookup(t0);
+      offs[1][lane] = lookup(t0 + 1);
     }
     __syncthreads();
-    load(t0);
-    store(t0);
+    load(t0, 0);
     __syncthreads();
   }
   for (int t = t0; t < t1; ++t) {
     int64_t ahead = 0;
-    if (t + 1 < t1) load(t + 1);
+    if (t + 1 < t1) load(t + 1, slot == 2 ? 0 : slot + 1);
     if (wave == 0) ahead = lookup(t + 2);
-    if (tid < 2) odd[(t + 2) % 3][tid] = 0;
+    uint32_t bad0 = 0, bad1 = 0;
+    if (t * kKeys + kKeys > min(all, end)) {
+      // some row does not see some key here: its weight is zero, and so must its product be.
+      // Values that are not finite leave the tile, and go to the rows that see them below.
+      uint8_t* const vb = lds + (t & 1) * 2 * kPart + kPart;
+#pragma unroll 1
+      for (int x = tid; x < kKeys * PC; x += 256) {
+        const int key = x / PC;
+        const u32x4v v = *(const u32x4v*)(vb + x * 16);
+        u32x4v f = {0, 0, 0, 0};
+        if (t * kKeys + key < end) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) f[y] = finite2<DT>(v[y]);
+          if (f[0] != v[0] || f[1] != v[1] || f[2] != v[2] || f[3] != v[3])
+            atomicOr(&odd[t & 1][key >> 5], 1u << (key & 31));
+        }
+        *(u32x4v*)(vb + x * 16) = f;
+      }
+      __syncthreads();
+      bad0 = __builtin_amdgcn_readfirstlane(odd[t & 1][0]);
+      bad1 = __builtin_amdgcn_readfirstlane(odd[t & 1][1]);
+    }
+    if (tid < 2) odd[(t + 1) & 1][tid] = 0;
     const int p0 = t * kKeys;
     if (!idle && p0 < w_end) {
-      const uint8_t* const kb = lds + (t & 1) * kBuf;
-      const uint8_t* const vb = kb + kKeys * KS;
+      const uint8_t* const kb = lds + (t & 1) * 2 * kPart;
+      const uint8_t* const vb = kb + kPart;
       f32x16 s[2];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int x = 0; x < 16; ++x) s[b][x] = 0;
 #pragma unroll
-        for (int k = 0; k < 2 * NT; ++k)
-          s[b] = mma32<DT>(*(const u32x4v*)(kb + (32 * b + col) * KS + (2 * k + half) * 16), qf[k], s[b]);
+      for (int k = 0; k < 2 * NT; ++k) {
+        const uint8_t* const kp = kb + col * RS + T::place(2 * k + half, T::key(col)) * 16;  // key + 32 turns alike
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s[b] = mma32<DT>(*(const u32x4v*)(kp + 32 * b * RS), qf[k], s[b]);
       }
       uint64_t seen = ~0ull;
       if (p0 + kKeys > w_all || p0 + kKeys > q.length) {
@@ -202,9 +221,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
 #pragma unroll
         for (int x = 0; x < 4; ++x)
           pf[k][x] = pack2<DT>(s[k >> 1][8 * (k & 1) + 2 * x], s[k >> 1][8 * (k & 1) + 2 * x + 1]);
-      uint64_t bad = odd[t % 3][0] | (uint64_t)odd[t % 3][1] << 32;
-      bad = __builtin_amdgcn_readfirstlane((uint32_t)bad) |
-            (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(bad >> 32)) << 32;
+      uint64_t bad = bad0 | (uint64_t)bad1 << 32;
 #pragma unroll 1
       while (bad) {  // values that are not finite, to the rows that see them only
         const int key = __builtin_ctzll(bad), at = (key >> 5) * 16 + ((key >> 3) & 3) * 4 + (key & 3);
@@ -214,7 +231,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
         for (int x = 0; x < 32; ++x) p = x == at ? s[x >> 4][x & 15] : p;
         p = __shfl(p, col + 32 * ((key >> 2) & 1), 64);
         const bool sees = (seen >> key) & 1;
-        const uint16_t* const vp = values + offs[t % 3][key];
+        const uint16_t* const vp = values + offs[slot][key];
         const int d0 = 4 * here(half);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -228,18 +245,19 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      const uint8_t* const vl = vb + (4 * half + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+      const int vrow = 4 * half + (lane & 15) / 4;
+      const uint8_t* const vl = vb + vrow * RS + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const u32x2v lo = read_transposed(vl + 16 * k * VS + 64 * n);
-          const u32x2v hi = read_transposed(vl + (16 * k + 8) * VS + 64 * n);
+        for (int n = 0; n < NT; ++n) {  // key + 4 turns alike
+          const uint8_t* const vp = vl + T::place(4 * n, T::value(vrow)) * 16 + 16 * k * RS;
+          const u32x2v lo = read_transposed(vp), hi = read_transposed(vp + 8 * RS);
           o[n] = mma32<DT>(u32x4v{lo.x, lo.y, hi.x, hi.y}, pf[k], o[n]);
         }
     }
-    if (t + 1 < t1) store(t + 1);
-    if (wave == 0) offs[(t + 2) % 3][lane] = ahead;
+    if (wave == 0) offs[slot == 0 ? 2 : slot - 1][lane] = ahead;
+    slot = slot == 2 ? 0 : slot + 1;
     __syncthreads();
   }
 
