@@ -49,16 +49,26 @@ __device__ __forceinline__ int parts_of(const AttendPlan& p, int length) {
   return min(p.splits, max(1, (length + p.chunk - 1) / p.chunk));
 }
 
-// Element offset of token p's row of this request, from the part's base.  A bad block id is
-// reported and the nearest block read in its place.
-__device__ __forceinline__ int64_t token_offset(const kvmi_attention_args& a, int r, int p) {
-  const uint32_t S = a.cache.block_size, col = (uint32_t)p / S, place = (uint32_t)p - col * S;
-  int id = gld(a.tables + (int64_t)r * a.columns + col);
+// Where token p's block and place in it are: its column of the table, and the element offset of
+// its row from the part's base.  A bad block id is reported and the nearest block read in its
+// place.
+struct Place {
+  uint32_t column, place;
+};
+__device__ __forceinline__ Place place_of(const kvmi_attention_args& a, int p) {
+  const uint32_t S = a.cache.block_size, col = (uint32_t)p / S;
+  return Place{col, (uint32_t)p - col * S};
+}
+__device__ __forceinline__ int64_t row_offset(const kvmi_attention_args& a, int id, uint32_t place) {
   if (id < 0 || id >= a.cache.num_blocks) {
     if (a.err) atomicOr(a.err, KVMI_ERR_BLOCK_ID);
     id = min(max(id, 0), a.cache.num_blocks - 1);
   }
   return (int64_t)id * a.cache.block_stride + (int64_t)(place * (uint32_t)(a.cache.num_heads * a.cache.head_dim));
+}
+__device__ __forceinline__ int64_t token_offset(const kvmi_attention_args& a, int r, int p) {
+  const Place at = place_of(a, p);
+  return row_offset(a, gld(a.tables + (int64_t)r * a.columns + at.column), at.place);
 }
 
 // Bit k: query i of the request (its mask row at `mask`, or null: the causal chain) sees token
@@ -107,6 +117,9 @@ __device__ __forceinline__ float odd_term(float p, uint32_t x) {
   constexpr uint32_t e = DT == KVMI_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
   return (x & e) == e ? p * to_f32<DT>(x & 0xffffu) : 0.0f;
 }
+// A value needed from here on: a load of it is waited for here, not at a first use inside a loop,
+// where the wait would be for the loop's own loads too.
+__device__ __forceinline__ void arrive(u32x4v& v) { asm volatile("" : "+v"(v)); }
 // A value that is taken anew where it stands: keeps what a rare path computes from it inside
 // that path.
 __device__ __forceinline__ int here(int x) {

@@ -20,6 +20,25 @@ __device__ __forceinline__ u32x2v read_transposed(const uint8_t* p) {
       u32x2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
 
+__device__ __forceinline__ void to_lds(const uint16_t* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((const KVMI_GLOBAL void*)from, (__attribute__((address_space(3))) void*)to, 16, 0,
+                                   0);
+}
+
+// The order of a product's N instructions: AHEAD of their operands, READS reads of LDS each, are
+// on their way before the first, then one more behind each.  (Left to itself the scheduler reads
+// two and waits for both: 5 % slower.)
+template <int N, int READS, int AHEAD>
+__device__ __forceinline__ void interleave() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * READS, 0);
+#pragma unroll
+  for (int k = 0; k < N - AHEAD; ++k) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x8, AHEAD, 0);
+}
+
 // Where chunk c (8 channels) of a key's row lies in its row in LDS.  The rows are PC chunks
 // without gaps, since loads that go straight to LDS write 1 KiB in order, and are turned so that
 // the reads meet every bank once: K's, one chunk of 16 keys, by single chunks, V's, 4 chunks of
@@ -51,7 +70,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
   __shared__ int64_t offs[3][kKeys];
   __shared__ uint32_t odd[2][2];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int head = blockIdx.x, r = blockIdx.z;
   const int tile = plan.row_tiles - 1 - (int)blockIdx.y % plan.row_tiles, part = blockIdx.y / plan.row_tiles;
   const Request q = request_of(a, r, tid == 0);
@@ -89,6 +108,8 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
       qf[k] = d < D ? ld16(qp + d) : u32x4v{0, 0, 0, 0};
     }
   }
+#pragma unroll
+  for (int k = 0; k < 2 * NT; ++k) arrive(qf[k]);
   const float c = a.scale * kLog2e;
   float mx = -INFINITY, l = 0;
   f32x16 o[NT];
@@ -97,24 +118,24 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
 #pragma unroll
     for (int x = 0; x < 16; ++x) o[n][x] = 0;
 
-  auto lookup = [&](int t) -> int64_t {  // the first wave's lanes, a key each
+  // the first wave's lanes look a key each up: the id is loaded ahead of a tile's loads, and
+  // waited for without waiting for those
+  const int32_t* const table = a.tables + (int64_t)r * a.columns;
+  auto find = [&](int t) -> Place {
     const int p = t * kKeys + lane;
-    return p < end ? token_offset(a, r, p) : 0;
+    return place_of(a, p < end ? p : 0);
   };
   // pieces of 16 bytes in the order of LDS, NT of K's and of V's a lane
   auto load = [&](int t, int slot) {
     uint8_t* const kb = lds + (t & 1) * 2 * kPart + wave * NT * 1024;
+    const bool whole = D == 32 * NT;
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
       const int idx = (wave * NT + k) * 64 + lane, key = idx / PC, place = idx - key * PC;
       const int64_t off = offs[slot][key];
       const int ck = T::chunk(place, T::key(key)), cv = T::chunk(place, T::value(key));
-      if (ck * 8 < D)
-        __builtin_amdgcn_global_load_lds((const KVMI_GLOBAL void*)(keys + off + ck * 8),
-                                         (__attribute__((address_space(3))) void*)(kb + k * 1024), 16, 0, 0);
-      if (cv * 8 < D)
-        __builtin_amdgcn_global_load_lds((const KVMI_GLOBAL void*)(values + off + cv * 8),
-                                         (__attribute__((address_space(3))) void*)(kb + kPart + k * 1024), 16, 0, 0);
+      if (whole || ck * 8 < D) to_lds(keys + off + ck * 8, kb + k * 1024);
+      if (whole || cv * 8 < D) to_lds(values + off + cv * 8, kb + kPart + k * 1024);
     }
   };
 
@@ -129,17 +150,23 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
     }
     if (tid < 4) odd[tid >> 1][tid & 1] = 0;
     if (wave == 0) {
-      offs[0][lane] = lookup(t0);
-      offs[1][lane] = lookup(t0 + 1);
+      for (int x = 0; x < 2; ++x) {
+        const Place at = find(t0 + x);
+        offs[x][lane] = row_offset(a, gld(table + at.column), at.place);
+      }
     }
     __syncthreads();
     load(t0, 0);
     __syncthreads();
   }
   for (int t = t0; t < t1; ++t) {
-    int64_t ahead = 0;
+    Place at{};
+    int id = 0;
+    if (wave == 0) {
+      at = find(t + 2);
+      id = gld(table + at.column);
+    }
     if (t + 1 < t1) load(t + 1, slot == 2 ? 0 : slot + 1);
-    if (wave == 0) ahead = lookup(t + 2);
     uint32_t bad0 = 0, bad1 = 0;
     if (t * kKeys + kKeys > min(all, end)) {
       // some row does not see some key here: its weight is zero, and so must its product be.
@@ -178,6 +205,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
 #pragma unroll
         for (int b = 0; b < 2; ++b) s[b] = mma32<DT>(*(const u32x4v*)(kp + 32 * b * RS), qf[k], s[b]);
       }
+      interleave<4 * NT, 1, 4>();
       uint64_t seen = ~0ull;
       if (p0 + kKeys > w_all || p0 + kKeys > q.length) {
         seen = seen_bits(q, mask, a.mask_words, qi, p0);
@@ -245,6 +273,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
           __builtin_amdgcn_sched_barrier(0);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
       const int vrow = 4 * half + (lane & 15) / 4;
       const uint8_t* const vl = vb + vrow * RS + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
 #pragma unroll
@@ -255,8 +284,9 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
           const u32x2v lo = read_transposed(vp), hi = read_transposed(vp + 8 * RS);
           o[n] = mma32<DT>(u32x4v{lo.x, lo.y, hi.x, hi.y}, pf[k], o[n]);
         }
+      interleave<4 * NT, 2, 2>();
     }
-    if (wave == 0) offs[slot == 0 ? 2 : slot - 1][lane] = ahead;
+    if (wave == 0) offs[slot == 0 ? 2 : slot - 1][lane] = row_offset(a, id, at.place);
     slot = slot == 2 ? 0 : slot + 1;
     __syncthreads();
   }
