@@ -2,6 +2,8 @@
 // lengths, new keys and values written by slot, accepted drafts kept.
 #include "kvmi_common.hpp"
 
+#include <algorithm>
+
 namespace kvmi {
 namespace {
 
@@ -22,6 +24,19 @@ __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* lds) {
 }
 
 // ---------------------------------------------------------------- block tables
+// x / S for 0 <= x < 2^31: with 2^(l-1) < S <= 2^l and m = ceil(2^(31+l) / S) < 2^32, x m / 2^(31+l)
+// is over the quotient by less than x S / (2^(31+l) S) < 1 / S, so its floor is the quotient's.
+struct BlockOf {
+  uint32_t m;
+  int shift;
+  __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> shift); }
+};
+BlockOf block_of(int block_size) {
+  int l = 0;
+  while ((1LL << l) < block_size) ++l;
+  return BlockOf{(uint32_t)(((1ULL << (31 + l)) + block_size - 1) / block_size), 31 + l};
+}
+
 struct Need {  // what one request's change of length asks for
   int now, next, have, want;
   bool bad;
@@ -29,16 +44,23 @@ struct Need {  // what one request's change of length asks for
   __device__ int give() const { return have > want ? have - want : 0; }
   __device__ int tokens() const { return next > now ? next - now : 0; }
 };
-__device__ __forceinline__ Need need_of(const kvmi_tables_args& a, int r) {
+__device__ __forceinline__ Need need_of(const kvmi_tables_args& a, const BlockOf& div, int r) {
   Need n;
-  const int64_t top = (int64_t)a.columns * a.block_size;
+  const int top = a.columns * a.block_size;
   n.now = a.lengths[r];
   n.next = a.new_lengths[r];
   n.bad = n.now < 0 || n.now > top || n.next < 0 || n.next > top;
-  if (n.bad) n.next = n.now = n.now < 0 ? 0 : n.now > top ? (int)top : n.now;
-  n.have = (int)(((int64_t)n.now + a.block_size - 1) / a.block_size);
-  n.want = (int)(((int64_t)n.next + a.block_size - 1) / a.block_size);
+  if (n.bad) n.next = n.now = n.now < 0 ? 0 : n.now > top ? top : n.now;
+  n.have = n.now ? div(n.now - 1) + 1 : 0;
+  n.want = n.next ? div(n.next - 1) + 1 : 0;
   return n;
+}
+// Place of the i-th entry behind `base` (< N) in a ring of N; past 2 N only where the free count
+// and the blocks given back exceed the ring.
+__device__ __forceinline__ uint32_t ring_at(uint32_t base, uint32_t i, uint32_t N) {
+  uint32_t x = base + i;
+  if (x >= N) x -= N;
+  return x < N ? x : x % N;
 }
 
 // Workgroup (r, y) makes part y of request r's table row and slots.  No workgroup waits for
@@ -47,13 +69,13 @@ __device__ __forceinline__ Need need_of(const kvmi_tables_args& a, int r) {
 // from those sums it knows its place in the ring, so that a slot needs no table entry that
 // another workgroup writes.  A ring holds every block of the pool, so the places behind the
 // last free block never reach the head's: blocks returned here are not read here.
-__global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a) {
+__global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a, BlockOf div) {
   __shared__ int64_t lds[4];
   __shared__ int last;
   const int r = blockIdx.x, tid = threadIdx.x;
   int64_t take = 0, give = 0, tokens = 0;
   for (int i = tid; i < r; i += kThreads) {
-    const Need n = need_of(a, i);
+    const Need n = need_of(a, div, i);
     take += n.take();
     give += n.give();
     tokens += n.tokens();
@@ -61,7 +83,7 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a) {
   take = block_sum(take, lds);
   give = block_sum(give, lds);
   tokens = block_sum(tokens, lds);
-  const Need n = need_of(a, r);
+  const Need n = need_of(a, div, r);
   const int N = a.ring;
   const int head = (int)((uint32_t)a.state[0] % (uint32_t)N);
   const int count = a.state[1] < 0 ? 0 : a.state[1] > N ? N : a.state[1];
@@ -72,6 +94,9 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a) {
   const int64_t row = (int64_t)r * a.columns;
   const int64_t step = (int64_t)kThreads * gridDim.y;
   const int64_t lane = (int64_t)blockIdx.y * kThreads + tid;
+  // where this request takes blocks (looked at only where it fits: take <= N) and gives them back
+  const uint32_t from = ring_at(head, fits ? (uint32_t)take : 0, N);
+  const uint32_t to = (uint32_t)((uint64_t)(head + (int64_t)count + give) % (uint32_t)N);
 
   // the table row: blocks kept, blocks taken, and -1 behind them; the blocks given back go
   // behind the last free one
@@ -81,10 +106,10 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a) {
     const int32_t old = k < n.have ? a.tables[row + k] : -1;
     int32_t id = old;
     if (k >= keep) {
-      if (k < n.have) a.free_blocks[(head + count + give + (k - keep)) % N] = old;
+      if (k < n.have) a.free_blocks[ring_at(to, (uint32_t)(k - keep), N)] = old;
       id = -1;
     } else if (k >= n.have) {
-      id = a.free_blocks[(head + take + (k - n.have)) % N];
+      id = a.free_blocks[ring_at(from, (uint32_t)(k - n.have), N)];
     }
     a.out_tables[row + k] = id;
   }
@@ -95,9 +120,9 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a) {
     if (at >= a.max_tokens) break;
     int64_t slot = -1;
     if (granted) {
-      const int p = n.now + (int)i, k = p / a.block_size;
-      const int32_t id = k < n.have ? a.tables[row + k] : a.free_blocks[(head + take + (k - n.have)) % N];
-      slot = (int64_t)id * a.block_size + p % a.block_size;
+      const int p = n.now + (int)i, k = div(p);
+      const int32_t id = k < n.have ? a.tables[row + k] : a.free_blocks[ring_at(from, k - n.have, N)];
+      slot = (int64_t)id * a.block_size + (p - k * a.block_size);
     }
     a.slots[at] = slot;
   }
@@ -134,7 +159,7 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a) {
     for (int base = 0; base < a.requests; base += kThreads) {
       const int i = base + tid;
       Need m{};
-      if (i < a.requests) m = need_of(a, i);
+      if (i < a.requests) m = need_of(a, div, i);
       // inclusive sum of take over this piece: within the wave, then over the waves
       int64_t s = m.take();
 #pragma unroll
@@ -295,11 +320,13 @@ extern "C" int kvmi_build_tables(const kvmi_tables_args* args, kvmi_stream_t str
     return KVMI_EINVAL;
   const bool over = a.out_lengths == a.lengths;
   if (over != (a.out_state == a.state) || (over && !a.ticket) || a.new_lengths == a.out_lengths) return KVMI_EINVAL;
-  // one request may own most of the tokens: parts of 4096 slots, up to 64 of them
-  int64_t parts = ((int64_t)a.max_tokens + 4095) / 4096;
-  parts = parts < 1 ? 1 : parts > 64 ? 64 : parts;
+  // One request may own most of the tokens: where the requests alone do not fill the chip,
+  // several workgroups share one, 4096 slots each.  Every part adds up the requests before its
+  // own again, so there are no more than that needs (64 parts of 1024 requests took 153 us).
+  const int64_t parts = std::max<int64_t>(
+      1, std::min<int64_t>(((int64_t)a.max_tokens + 4095) / 4096, std::min(64, 1024 / a.requests)));
   hipLaunchKernelGGL(tables_kernel, dim3((unsigned)a.requests, (unsigned)parts), dim3(kThreads), 0,
-                     reinterpret_cast<hipStream_t>(stream), a);
+                     reinterpret_cast<hipStream_t>(stream), a, block_of(a.block_size));
   return launched();
 }
 
