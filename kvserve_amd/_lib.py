@@ -238,6 +238,28 @@ def load(path: Path = LIB_PATH):
         return lib
 
 
+class _NoCalls:
+    """In the place of the module `_calls` where it is not built: every use says so."""
+
+    def __init__(self, why: Exception):
+        self._why = why
+
+    def __getattr__(self, name):
+        raise KvmiError(f"kvserve_amd/_calls.so cannot be loaded ({self._why}): build it with "
+                        "`python -m kvserve_amd.build`")
+
+
+def calls():
+    """The module of the paged operators' unchecked calls (csrc/kvmi_calls.cpp)."""
+    try:
+        import torch  # noqa: F401  (its libraries are the module's)
+
+        from . import _calls
+    except ImportError as e:
+        return _NoCalls(e)
+    return _calls
+
+
 def check(rc: int, what: str) -> None:
     if rc == OK:
         return

@@ -1,7 +1,9 @@
 """Build the gfx950 C-ABI library ``kvserve_amd/libkvserve_amd.so`` with hipcc.
 
 Every ``csrc/*.hip`` file is compiled separately (in parallel) and linked into one
-shared library.  The library is built in-tree so it travels with the source tree.
+shared library; ``csrc/kvmi_calls.cpp``, host code, becomes the Python module
+``kvserve_amd/_calls.so`` that calls it.  Both are built in-tree so they travel with the
+source tree.
 
     python -m kvserve_amd.build
 """
@@ -19,6 +21,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 LIB = PKG / "libkvserve_amd.so"
+CALLS = PKG / "_calls.so"
 OBJ = PKG / "_build"
 
 ARCH = "gfx950"
@@ -53,6 +56,27 @@ def _compile(src: Path, defines=()) -> Path:
     return obj
 
 
+def _build_calls() -> None:
+    """The Python module over the library: the paged operators' unchecked calls."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    rocm = Path(hipcc()).resolve().parents[1]
+    tmp = CALLS.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{root}/include",
+           f"-I{root}/include/torch/csrc/api/include", f"-I{rocm}/include", f"-I{sysconfig.get_paths()['include']}",
+           f"-I{INCLUDE}", str(CSRC / "kvmi_calls.cpp"), "-o", str(tmp), f"-L{PKG}", f"-l:{LIB.name}",
+           "-Wl,-rpath,$ORIGIN", f"-L{root}/lib", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
+           f"-L{rocm}/lib", "-lamdhip64"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on kvmi_calls.cpp:\n{res.stderr}")
+    os.replace(tmp, CALLS)
+
+
 def build(verbose: bool = False, defines=()) -> Path:
     """Compile every HIP source and link the shared library; returns its path.
     `defines`: preprocessor symbols for every source (KVMI_ORDINARY_LAUNCH: the one-pass
@@ -71,8 +95,9 @@ def build(verbose: bool = False, defines=()) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stderr}")
     os.replace(tmp, LIB)
+    _build_calls()
     if verbose:
-        print(f"built {LIB}")
+        print(f"built {LIB} and {CALLS.name}")
     return LIB
 
 

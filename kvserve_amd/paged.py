@@ -32,10 +32,18 @@ from . import _lib
 from .engine import raise_device_error
 from .ops import _check_default
 
+# A call that is not checked goes through this module at once (4 us instead of 13); what it does
+# not take comes back, to the checks and errors here.
+_calls = _lib.calls()
+
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 
 
 # ------------------------------------------------------------------ shared checks
+def _unchecked(check: Optional[bool]) -> bool:
+    return check is False or (check is None and not _check_default())
+
+
 def _tensor(t, name: str, dtype: torch.dtype, shape, device=None) -> int:
     """Address of a contiguous CUDA tensor of this type and shape (None: any size)."""
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
@@ -117,6 +125,11 @@ def build_block_tables(lengths: torch.Tensor, new_lengths: torch.Tensor, tables:
     `out`: the tensors of a `TablesUpdate` to write into.  Tables may be `tables` itself;
     lengths and state may both be `lengths` and `state` themselves, with `ticket`, an int32 word
     of zero."""
+    if type(out) is tuple:
+        out = TablesUpdate(*out)
+    if type(out) is TablesUpdate and _unchecked(check) and _calls.build_block_tables(
+            lengths, new_lengths, tables, free, state, block_size, max_tokens, out, ticket, err):
+        return out
     if type(block_size) is not int or block_size < 1 or type(max_tokens) is not int or max_tokens < 0:
         raise ValueError("block_size must be a positive integer and max_tokens a nonnegative one")
     now = _tensor(lengths, "lengths", torch.int32, (None,))
@@ -209,6 +222,8 @@ def write_kv(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor, slots:
     adjacent channels, so slices of one projection will do) into the paged cache: token i's to
     block slots[i] // S, place slots[i] % S.  `slots` is int64 [tokens]; -1 skips a token.  No
     two tokens may share a slot."""
+    if _unchecked(check) and _calls.write_kv(key, value, cache, slots, err):
+        return
     c = _cache_struct(cache)
     for name, t in (("key", key), ("value", value)):
         if not isinstance(t, torch.Tensor) or t.dtype != cache.dtype:
@@ -314,6 +329,9 @@ def tree_attention(query: torch.Tensor, cache: torch.Tensor, tables: torch.Tenso
         raise TypeError("query must be a CUDA tensor")
     if out is None:
         out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    if not return_lse and _unchecked(check) and _calls.tree_attention(
+            query, cache, tables, lengths, starts, max_query, max_length, tree_mask, scale, out, err):
+        return out
     lse = torch.full(query.shape[:2], -math.inf, dtype=torch.float32, device=query.device) if return_lse else None
     args, query = _attention_args(query, cache, tables, lengths, starts, max_query, max_length, tree_mask, scale, out,
                                   lse)
@@ -351,6 +369,7 @@ class LayerCaches:
         self.struct.base = either
         self.device = first.device
         self.bases = torch.tensor(bases, dtype=torch.int64, device=self.device)
+        self._struct_at = ctypes.addressof(self.struct)
 
 
 def keep_drafts(caches, tables: torch.Tensor, lengths: torch.Tensor, accepted: torch.Tensor, *,
@@ -365,6 +384,9 @@ def keep_drafts(caches, tables: torch.Tensor, lengths: torch.Tensor, accepted: t
     Returns the lengths with the kept drafts, int32 [R] (`out`, not `lengths` itself).  A request
     whose path is not increasing or leaves its blocks is left as it is."""
     layers = caches if isinstance(caches, LayerCaches) else LayerCaches(caches)
+    if out is not None and _unchecked(check) and _calls.keep_drafts(
+            layers._struct_at, layers.bases, tables, lengths, accepted, out, err):
+        return out
     R = lengths.numel() if isinstance(lengths, torch.Tensor) else 0
     now = _tensor(lengths, "lengths", torch.int32, (R,), layers.device)
     tab = _tensor(tables, "tables", torch.int32, (R, None), layers.device)
