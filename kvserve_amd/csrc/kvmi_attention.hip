@@ -70,7 +70,9 @@ __global__ __launch_bounds__(512, 2) void attend_rows_kernel(kvmi_attention_args
 
   auto lookup = [&](int t) -> int64_t {
     const int p = t * kStep + (lane & 31);
-    return t < t1 && p < end ? token_offset(a, r, p) : 0;
+    if (t >= t1 || p >= end) return 0;
+    const int at = plan.block(p);
+    return row_offset(a, gld(a.tables + (int64_t)r * a.columns + at), p - at * a.cache.block_size);
   };
   u32x4v kf[2][KS], v8[8][N8 ? N8 : 1];
   u32x2v v4[8];
@@ -351,7 +353,6 @@ bool attention_ok(const kvmi_attention_args* a) {
 
 struct Choice {
   bool rows;     // the kernel for few rows
-  int waves;     // its waves a workgroup
   int row_groups;
   AttendPlan plan;
 };
@@ -366,16 +367,18 @@ Choice choose(const kvmi_attention_args& a) {
   c.row_groups = rows <= 16 ? 1 : 2;
   c.rows = rows <= (D <= 128 ? 32 : 16);
   const int64_t length = a.max_length < 1 ? 1 : a.max_length;
-  c.plan.row_tiles = c.rows ? 1 : (int)((rows + 127) / 128);
+  c.plan.block = block_of(a.cache.block_size);
+  c.plan.waves = 4;
+  c.plan.row_tiles = 1;
+  if (!c.rows) c.plan.row_tiles = (int)((rows + 127) / 128);
   const int64_t groups = (int64_t)a.requests * a.cache.num_heads * c.plan.row_tiles;
   c.plan.chunk = c.rows ? 1024 : 512;
   int64_t splits = (length + c.plan.chunk - 1) / c.plan.chunk;
-  if (!c.rows) splits = splits < (1024 + groups - 1) / groups ? splits : (1024 + groups - 1) / groups;
-  splits = splits > 64 ? 64 : splits;
+  if (!c.rows) splits = std::min<int64_t>(splits, (1024 + groups - 1) / groups);
+  splits = std::min<int64_t>(splits, 64);
   if (!c.rows && splits > 1) c.plan.chunk = (int)((length + splits - 1) / splits);
   while (splits > 1 && ((int64_t)c.plan.row_tiles * splits > 65535 || parts_bytes(a, (int)splits) > (1LL << 31))) splits /= 2;
   c.plan.splits = (int)splits;
-  c.waves = 4;
   return c;
 }
 
@@ -384,8 +387,8 @@ void launch_rows(const kvmi_attention_args& a, const Choice& c, hipStream_t st) 
   const int D = a.cache.head_dim, G = a.query_heads / a.cache.num_heads;
   const int rows = std::min(16 * c.row_groups, a.max_query * G);
   const dim3 grid((unsigned)a.cache.num_heads, (unsigned)c.plan.splits, (unsigned)a.requests);
-  const dim3 threads((unsigned)(64 * c.waves));
-  const size_t lds = (size_t)c.waves * rows * (D + 4) * 4;
+  const dim3 threads((unsigned)(64 * c.plan.waves));
+  const size_t lds = (size_t)c.plan.waves * rows * (D + 4) * 4;
 #define KVMI_ROWS(N8, N4, R) \
   hipLaunchKernelGGL((attend_rows_kernel<DT, N8, N4, R>), grid, threads, lds, st, a, c.plan)
   if (D > 192)

@@ -21,7 +21,9 @@ constexpr float kRaise = 8.0f;
 
 // How the keys of a request are split over workgroups and where the parts go.
 struct AttendPlan {
-  int row_tiles;  // tiles kernel: row tiles of a KV head
+  BlockOf block;
+  int waves;      // of a workgroup
+  int row_tiles;  // tiles kernel: row tiles of a KV head, 32 rows a wave
   int splits;     // the most parts of a request
   int chunk;      // keys that a part should have
   float* sums;    // [query row][query head][splits][D] unnormalised sums, where splits > 1
@@ -49,26 +51,14 @@ __device__ __forceinline__ int parts_of(const AttendPlan& p, int length) {
   return min(p.splits, max(1, (length + p.chunk - 1) / p.chunk));
 }
 
-// Where token p's block and place in it are: its column of the table, and the element offset of
-// its row from the part's base.  A bad block id is reported and the nearest block read in its
-// place.
-struct Place {
-  uint32_t column, place;
-};
-__device__ __forceinline__ Place place_of(const kvmi_attention_args& a, int p) {
-  const uint32_t S = a.cache.block_size, col = (uint32_t)p / S;
-  return Place{col, (uint32_t)p - col * S};
-}
-__device__ __forceinline__ int64_t row_offset(const kvmi_attention_args& a, int id, uint32_t place) {
+// Element offset of a token's row from the part's base, from its block's id and its place in the
+// block.  A bad id is reported and the nearest block read in its place.
+__device__ __forceinline__ int64_t row_offset(const kvmi_attention_args& a, int id, int place) {
   if (id < 0 || id >= a.cache.num_blocks) {
     if (a.err) atomicOr(a.err, KVMI_ERR_BLOCK_ID);
     id = min(max(id, 0), a.cache.num_blocks - 1);
   }
-  return (int64_t)id * a.cache.block_stride + (int64_t)(place * (uint32_t)(a.cache.num_heads * a.cache.head_dim));
-}
-__device__ __forceinline__ int64_t token_offset(const kvmi_attention_args& a, int r, int p) {
-  const Place at = place_of(a, p);
-  return row_offset(a, gld(a.tables + (int64_t)r * a.columns + at.column), at.place);
+  return (int64_t)id * a.cache.block_stride + (int64_t)((uint32_t)place * (uint32_t)(a.cache.num_heads * a.cache.head_dim));
 }
 
 // Bit k: query i of the request (its mask row at `mask`, or null: the causal chain) sees token

@@ -12,7 +12,7 @@
 namespace kvmi {
 namespace {
 
-constexpr int kRows = 128, kKeys = 64;
+constexpr int kKeys = 64;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ u32x2v read_transposed(const uint8_t* p) {
@@ -60,22 +60,25 @@ struct Turn {
 };
 
 // NT: 32-channel tiles of a head, D <= 32 * NT.
-template <int DT, int NT>
+// WHOLE: D == 32 * NT, no channels to leave out.
+template <int DT, int NT, bool WHOLE>
 __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi_attention_args a, AttendPlan plan) {
   constexpr int PC = 4 * NT, RS = 16 * PC, kPart = kKeys * RS;  // chunks and bytes of a row, bytes of a tile
   using T = Turn<PC>;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kPart];  // K and V of two tiles
-  // of tile t in place t % 3 each key's offset in the cache (looked up two tiles ahead), in
-  // place t % 2 the keys with a value that is not finite
-  __shared__ int64_t offs[3][kKeys];
+  // of tile t in place t % 8 each key's offset in the cache, in place t % 2 the keys with a value
+  // that is not finite
+  __shared__ int64_t offs[8][kKeys];
   __shared__ uint32_t odd[2][2];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int waves = 4, threads = 256;
   const int head = blockIdx.x, r = blockIdx.z;
   const int tile = plan.row_tiles - 1 - (int)blockIdx.y % plan.row_tiles, part = blockIdx.y / plan.row_tiles;
   const Request q = request_of(a, r, tid == 0);
   const int D = a.cache.head_dim, H = a.cache.num_heads, G = a.query_heads / H;
-  const int M = min(q.queries, a.max_query) * G, m0 = tile * kRows;
+  const int M = min(q.queries, a.max_query) * G, m0 = tile * 32 * waves;
   if (m0 >= M) return;
   const int parts = parts_of(plan, q.length);
   if (part >= parts) return;
@@ -84,16 +87,18 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
   const uint16_t* const values = keys + a.cache.part_stride;
 
   // keys that any row of the workgroup sees end at `end`; those before `all` are seen by all
-  const int last_row = min(m0 + kRows, M) - 1;
+  const int last_row = min(m0 + 32 * waves, M) - 1;
   const int end = masks ? q.length : min(q.length, q.prefix + last_row / G + 1);
   const int all = masks ? q.prefix : q.prefix + m0 / G + 1;
   const int w0 = m0 + 32 * wave;
-  const bool idle = w0 >= M;
   const int w_all = masks ? q.prefix : q.prefix + w0 / G + 1;
-  const int w_end = masks ? end : min(end, q.prefix + min(w0 + 31, M - 1) / G + 1);
   const int tiles = (q.length + kKeys - 1) / kKeys;
   const int t0 = (int)((int64_t)tiles * part / parts);
   const int t1 = min((int)((int64_t)tiles * (part + 1) / parts), (end + kKeys - 1) / kKeys);
+  const int hiding = min(all, end) >> 6;  // the first tile with a key that some row does not see
+  // this wave's: its rows see nothing from tile w1 on
+  const int w_end = masks ? end : min(end, q.prefix + min(w0 + 31, M - 1) / G + 1);
+  const int w1 = w0 >= M ? t0 : min(t1, (w_end + kKeys - 1) / kKeys), w_hiding = min(w_all, q.length) >> 6;
 
   // this lane's row
   const int m = min(w0 + col, M - 1), qi = m / G, qh = head * G + m - qi * G;
@@ -118,62 +123,58 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
 #pragma unroll
     for (int x = 0; x < 16; ++x) o[n][x] = 0;
 
-  // the first wave's lanes look a key each up: the id is loaded ahead of a tile's loads, and
-  // waited for without waiting for those
+  // Every 4th tile each wave looks one of the next 4 tiles' keys up, a key a lane; the ids are
+  // loaded ahead of a tile's loads, and waited for without waiting for those.
   const int32_t* const table = a.tables + (int64_t)r * a.columns;
-  auto find = [&](int t) -> Place {
-    const int p = t * kKeys + lane;
-    return place_of(a, p < end ? p : 0);
+  int place = 0, id = 0;
+  auto look_up = [&](int t) {
+    const int p = (t + wave) * kKeys + lane, at = plan.block(p < end ? p : 0);
+    place = p < end ? p - at * a.cache.block_size : 0;
+    id = gld(table + at);
   };
-  // pieces of 16 bytes in the order of LDS, NT of K's and of V's a lane
-  auto load = [&](int t, int slot) {
-    uint8_t* const kb = lds + (t & 1) * 2 * kPart + wave * NT * 1024;
-    const bool whole = D == 32 * NT;
+  auto note = [&](int t) { offs[(t + wave) & 7][lane] = row_offset(a, id, place); };
+  // pieces of 16 bytes in the order of LDS, 64 an instruction; NT instructions of K's and of V's
+  // a wave where there are 4 waves
+  auto load = [&](int t) {
+    uint8_t* const kb = lds + (t & 1) * 2 * kPart + wave * 1024;
+    int64_t off[NT];
+#pragma unroll
+    for (int k = 0; k < NT; ++k) off[k] = offs[t & 7][((k * waves + wave) * 64 + lane) / PC];
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
-      const int idx = (wave * NT + k) * 64 + lane, key = idx / PC, place = idx - key * PC;
-      const int64_t off = offs[slot][key];
-      const int ck = T::chunk(place, T::key(key)), cv = T::chunk(place, T::value(key));
-      if (whole || ck * 8 < D) to_lds(keys + off + ck * 8, kb + k * 1024);
-      if (whole || cv * 8 < D) to_lds(values + off + cv * 8, kb + kPart + k * 1024);
+      const int idx = (k * waves + wave) * 64 + lane, key = idx / PC, at = idx - key * PC;
+      const int ck = T::chunk(at, T::key(key)), cv = T::chunk(at, T::value(key));
+      if (WHOLE || ck * 8 < D) to_lds(keys + ck * 8 + off[k], kb + k * waves * 1024);
+      if (WHOLE || cv * 8 < D) to_lds(values + cv * 8 + off[k], kb + kPart + k * waves * 1024);
     }
   };
 
-  int slot = 0;  // t % 3
   if (t0 < t1) {
-    if (D < 32 * NT) {  // channels behind the head's are zero once and for all
-      for (int x = tid; x < 4 * kKeys * PC; x += 256) {
+    if (!WHOLE) {  // channels behind the head's are zero once and for all
+      for (int x = tid; x < 4 * kKeys * PC; x += threads) {
         const int row = x / PC, place = x - row * PC, key = row & 63;
         if (T::chunk(place, row & 64 ? T::value(key) : T::key(key)) * 8 >= D)
           *(u32x4v*)(lds + x * 16) = u32x4v{0, 0, 0, 0};
       }
     }
     if (tid < 4) odd[tid >> 1][tid & 1] = 0;
-    if (wave == 0) {
-      for (int x = 0; x < 2; ++x) {
-        const Place at = find(t0 + x);
-        offs[x][lane] = row_offset(a, gld(table + at.column), at.place);
-      }
-    }
+    look_up(t0);
+    note(t0);
     __syncthreads();
-    load(t0, 0);
+    load(t0);
     __syncthreads();
   }
   for (int t = t0; t < t1; ++t) {
-    Place at{};
-    int id = 0;
-    if (wave == 0) {
-      at = find(t + 2);
-      id = gld(table + at.column);
-    }
-    if (t + 1 < t1) load(t + 1, slot == 2 ? 0 : slot + 1);
+    const bool look = ((t - t0) & 3) == 0;
+    if (look) look_up(t + 4);
+    if (t + 1 < t1) load(t + 1);
     uint32_t bad0 = 0, bad1 = 0;
-    if (t * kKeys + kKeys > min(all, end)) {
+    if (t >= hiding) {
       // some row does not see some key here: its weight is zero, and so must its product be.
       // Values that are not finite leave the tile, and go to the rows that see them below.
       uint8_t* const vb = lds + (t & 1) * 2 * kPart + kPart;
 #pragma unroll 1
-      for (int x = tid; x < kKeys * PC; x += 256) {
+      for (int x = tid; x < kKeys * PC; x += threads) {
         const int key = x / PC;
         const u32x4v v = *(const u32x4v*)(vb + x * 16);
         u32x4v f = {0, 0, 0, 0};
@@ -188,10 +189,10 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
       __syncthreads();
       bad0 = __builtin_amdgcn_readfirstlane(odd[t & 1][0]);
       bad1 = __builtin_amdgcn_readfirstlane(odd[t & 1][1]);
+      if (tid < 2) odd[(t + 1) & 1][tid] = 0;
     }
-    if (tid < 2) odd[(t + 1) & 1][tid] = 0;
     const int p0 = t * kKeys;
-    if (!idle && p0 < w_end) {
+    if (t < w1) {
       const uint8_t* const kb = lds + (t & 1) * 2 * kPart;
       const uint8_t* const vb = kb + kPart;
       f32x16 s[2];
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
       }
       interleave<4 * NT, 1, 4>();
       uint64_t seen = ~0ull;
-      if (p0 + kKeys > w_all || p0 + kKeys > q.length) {
+      if (t >= w_hiding) {
         seen = seen_bits(q, mask, a.mask_words, qi, p0);
         const uint64_t mine = seen >> (4 * half);
 #pragma unroll
@@ -259,7 +260,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
         for (int x = 0; x < 32; ++x) p = x == at ? s[x >> 4][x & 15] : p;
         p = __shfl(p, col + 32 * ((key >> 2) & 1), 64);
         const bool sees = (seen >> key) & 1;
-        const uint16_t* const vp = values + offs[slot][key];
+        const uint16_t* const vp = values + offs[t & 7][key];
         const int d0 = 4 * here(half);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -286,13 +287,12 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
         }
       interleave<4 * NT, 2, 2>();
     }
-    if (wave == 0) offs[slot == 0 ? 2 : slot - 1][lane] = row_offset(a, id, at.place);
-    slot = slot == 2 ? 0 : slot + 1;
+    if (look) note(t + 4);
     __syncthreads();
   }
 
   l = join32(l, Plus());
-  if (idle || w0 + col >= M) return;
+  if (w0 + col >= M) return;
   const int64_t out_row = row * a.query_heads + qh;
   if (parts == 1) {
     const float f = l == 0 ? 0.0f : 1.0f / l;
@@ -321,24 +321,26 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
   }
 }
 
-template <int DT>
+template <int DT, int NT>
 void launch(const kvmi_attention_args& a, const AttendPlan& p, hipStream_t st) {
   const dim3 grid((unsigned)a.cache.num_heads, (unsigned)(p.row_tiles * p.splits), (unsigned)a.requests);
-  const int tiles = (a.cache.head_dim + 31) / 32;
-#define KVMI_TILES(N) hipLaunchKernelGGL((attend_tiles_kernel<DT, N>), grid, dim3(256), 0, st, a, p)
-  if (tiles <= 2)
-    KVMI_TILES(2);
-  else if (tiles == 3)
-    KVMI_TILES(3);
-  else if (tiles == 4)
-    KVMI_TILES(4);
-  else if (tiles == 5)
-    KVMI_TILES(5);
-  else if (tiles == 6)
-    KVMI_TILES(6);
+  const dim3 threads((unsigned)(64 * p.waves));
+  if (a.cache.head_dim == 32 * NT)
+    hipLaunchKernelGGL((attend_tiles_kernel<DT, NT, true>), grid, threads, 0, st, a, p);
   else
-    KVMI_TILES(8);
-#undef KVMI_TILES
+    hipLaunchKernelGGL((attend_tiles_kernel<DT, NT, false>), grid, threads, 0, st, a, p);
+}
+template <int DT>
+void launch(const kvmi_attention_args& a, const AttendPlan& p, hipStream_t st) {
+  switch ((a.cache.head_dim + 31) / 32) {
+    case 1:
+    case 2: return launch<DT, 2>(a, p, st);
+    case 3: return launch<DT, 3>(a, p, st);
+    case 4: return launch<DT, 4>(a, p, st);
+    case 5: return launch<DT, 5>(a, p, st);
+    case 6: return launch<DT, 6>(a, p, st);
+    default: return launch<DT, 8>(a, p, st);
+  }
 }
 
 }  // namespace

@@ -17,6 +17,19 @@ __host__ __device__ constexpr int next_pow2(int x) {
   return p;
 }
 
+// x / S for 0 <= x < 2^31: with 2^(l-1) < S <= 2^l and m = ceil(2^(31+l) / S) < 2^32, x m / 2^(31+l)
+// is over the quotient by less than x S / (2^(31+l) S) < 1 / S, so its floor is the quotient's.
+struct BlockOf {
+  uint32_t m;
+  int shift;
+  __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> shift); }
+};
+inline BlockOf block_of(int block_size) {
+  int l = 0;
+  while ((1LL << l) < block_size) ++l;
+  return BlockOf{(uint32_t)(((1ULL << (31 + l)) + block_size - 1) / block_size), 31 + l};
+}
+
 // Quantization axis of a part (0 = K, 1 = V): the default is K per channel and V per
 // token; the KVMI_F_* axis flags select the others.
 enum Axis { kAxChannel = 0, kAxToken = 1, kAxTensor = 2 };

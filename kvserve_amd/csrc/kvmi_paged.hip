@@ -24,19 +24,6 @@ __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* lds) {
 }
 
 // ---------------------------------------------------------------- block tables
-// x / S for 0 <= x < 2^31: with 2^(l-1) < S <= 2^l and m = ceil(2^(31+l) / S) < 2^32, x m / 2^(31+l)
-// is over the quotient by less than x S / (2^(31+l) S) < 1 / S, so its floor is the quotient's.
-struct BlockOf {
-  uint32_t m;
-  int shift;
-  __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> shift); }
-};
-BlockOf block_of(int block_size) {
-  int l = 0;
-  while ((1LL << l) < block_size) ++l;
-  return BlockOf{(uint32_t)(((1ULL << (31 + l)) + block_size - 1) / block_size), 31 + l};
-}
-
 struct Need {  // what one request's change of length asks for
   int now, next, have, want;
   bool bad;
