@@ -16,13 +16,20 @@ constexpr int kStep = 32;  // keys a wave takes at a time
 //                   channels; pairs of keys are brought together by byte permutes, and the
 //                   output row of tile j is channel 8 * row + j
 // so that nothing goes through LDS before the waves' sums are joined at the end.
-// N8 / N4: panels of 128 / 64 channels.
+// N8 / N4: panels of 128 / 64 channels.  Past 128 channels, or 16 rows, the queries stay in LDS and
+// are read again for every 32 keys: with them in registers a wave would not fit its 256.  Past 192
+// it does not fit them either way, and has a SIMD's 512 to itself.
 template <int DT, int N8, int N4, int R>
-__global__ __launch_bounds__(512, 2) void attend_rows_kernel(kvmi_attention_args a, AttendPlan plan) {
+__global__ __launch_bounds__((N8 == 2 ? 256 : 512), (N8 == 2 ? 1 : 2)) void attend_rows_kernel(kvmi_attention_args a,
+                                                                                             AttendPlan plan) {
+  constexpr bool kShared = (N8 + N4 > 1 || R > 1) && N8 < 2;
   constexpr int KS = 4 * N8 + 2 * N4, OT = 8 * N8 + 4 * N4;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // [waves][rows][D] sums
   __shared__ int64_t offs[8][2][kStep];
   __shared__ float2 stat[8][16 * R];
+  // chunk c of row m at c ^ (m % 16): 16 rows' reads meet every bank once
+  constexpr int kRowChunks = KS > 4 ? 32 : 16;
+  __shared__ __attribute__((aligned(16))) uint8_t shared_q[kShared ? 16 * R * kRowChunks * 16 : 16];
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int col = lane & 15, g = lane >> 4;
@@ -36,13 +43,13 @@ __global__ __launch_bounds__(512, 2) void attend_rows_kernel(kvmi_attention_args
   const uint16_t* const keys = (const uint16_t*)a.cache.base + head * D;
   const uint16_t* const values = keys + a.cache.part_stride;
 
-  u32x4v qf[R][KS];
+  u32x4v qf[R][kShared ? 1 : KS];
   int qi[R];
   const uint64_t* mask[R];
 #pragma unroll
   for (int x = 0; x < R; ++x) {
     const int m = min(16 * x + col, M - 1);
-    qi[x] = m / G;
+    qi[x] = plan.group(m);
     const int64_t row = q.first + qi[x];
     mask[x] = a.mask ? a.mask + row * a.mask_words : nullptr;
     const uint16_t* qp = (const uint16_t*)a.query + row * a.query_token_stride +
@@ -50,9 +57,21 @@ __global__ __launch_bounds__(512, 2) void attend_rows_kernel(kvmi_attention_args
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       const int d = 32 * k + 8 * g;
-      qf[x][k] = d < D ? ld16(qp + d) : u32x4v{0, 0, 0, 0};
+      const u32x4v v = d < D ? ld16(qp + d) : u32x4v{0, 0, 0, 0};
+      if constexpr (kShared) {
+        if (wave == 0) *(u32x4v*)(shared_q + ((16 * x + col) * kRowChunks + ((4 * k + g) ^ col)) * 16) = v;
+      } else {
+        qf[x][k] = v;
+      }
     }
   }
+  if constexpr (kShared) __syncthreads();
+  auto query = [&](int x, int k, int at) -> u32x4v {  // `at`: the lane's column, taken anew
+    if constexpr (kShared)
+      return *(const u32x4v*)(shared_q + ((16 * x + at) * kRowChunks + ((4 * k + g) ^ at)) * 16);
+    else
+      return qf[x][k];
+  };
   const float c = a.scale * kLog2e;
   float mx[R], l[R];
   f32x4 o[R][OT];
@@ -66,7 +85,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows_kernel(kvmi_attention_args
 
   const int end = q.length, all = a.mask ? q.prefix : q.prefix + 1;  // seen by some row, by all
   const int steps = (q.length + kStep - 1) / kStep;
-  const int t0 = (int)((int64_t)steps * part / parts) + wave, t1 = (int)((int64_t)steps * (part + 1) / parts);
+  const int t0 = part_begin(steps, part, parts) + wave, t1 = part_begin(steps, part + 1, parts);
 
   auto lookup = [&](int t) -> int64_t {
     const int p = t * kStep + (lane & 31);
@@ -115,14 +134,17 @@ __global__ __launch_bounds__(512, 2) void attend_rows_kernel(kvmi_attention_args
     const int p0 = t * kStep;
     if (lane < kStep) mine[(buf ^ 1) * kStep + lane] = lookup(t + waves);
     f32x4 s[R][2];
+    const int at = kShared ? here(col) : col;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int x = 0; x < R; ++x) {
+      s[x][0] = s[x][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int x = 0; x < R; ++x) {
-        s[x][b] = f32x4{0, 0, 0, 0};
+      for (int k = 0; k < KS; ++k) {
+        const u32x4v v = query(x, k, at);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) s[x][b] = mma16<DT>(kf[b][k], qf[x][k], s[x][b]);
+        for (int b = 0; b < 2; ++b) s[x][b] = mma16<DT>(kf[b][k], v, s[x][b]);
       }
+    }
     __builtin_amdgcn_wave_barrier();
     const int64_t* const next = mine + (buf ^ 1) * kStep;
     load_keys(next);
@@ -279,8 +301,11 @@ __global__ __launch_bounds__(512, 2) void attend_rows_kernel(kvmi_attention_args
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < rows * (D / 4); e += blockDim.x) {
-    const int m = e / (D / 4), d = 4 * (e - m * (D / 4));
+  // D / 4 lanes, or the next power of two, a row
+  const int lanes_log2 = D > 128 ? 6 : D > 64 ? 5 : D > 32 ? 4 : D > 16 ? 3 : 2;
+  for (int e = threadIdx.x; e < rows << lanes_log2; e += blockDim.x) {
+    const int m = e >> lanes_log2, d = 4 * (e - (m << lanes_log2));
+    if (d >= D) continue;
     float top = -INFINITY, total = 0;
     for (int w = 0; w < waves; ++w) top = fmaxf(top, stat[w][m].x);
     f32x4 v = {0, 0, 0, 0};
@@ -289,7 +314,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows_kernel(kvmi_attention_args
       total += s.x == -INFINITY ? 0.0f : s.y * __builtin_amdgcn_exp2f(s.x - top);
       v += *(const f32x4*)(sums + (w * rows + m) * DP + d);
     }
-    const int i = m / G;
+    const int i = plan.group(m);
     const int64_t out_row = (int64_t)(q.first + i) * a.query_heads + head * G + m - i * G;
     if (parts == 1) {
       const float f = total == 0 ? 0.0f : 1.0f / total;
@@ -303,28 +328,48 @@ __global__ __launch_bounds__(512, 2) void attend_rows_kernel(kvmi_attention_args
   }
 }
 
-// The parts of each query head of a request that was split, joined in their order.  D / 4
-// lanes (a power of two at least) a row.
+// The parts of each query head of a request that was split, joined in their order.  D / 4 lanes,
+// or the next power of two, a row.
 template <int DT>
-__global__ __launch_bounds__(256) void join_kernel(kvmi_attention_args a, AttendPlan plan, int lanes) {
+__global__ __launch_bounds__(256) void join_kernel(kvmi_attention_args a, AttendPlan plan, int lanes_log2) {
   const int r = blockIdx.y, D = a.cache.head_dim;
   const Request q = request_of(a, r, false);
   const int parts = parts_of(plan, q.length);
   if (parts == 1) return;
-  const int e = blockIdx.x * (256 / lanes) + threadIdx.x / lanes, d = 4 * (threadIdx.x % lanes);
+  const int e = (int)(blockIdx.x << (8 - lanes_log2)) + (threadIdx.x >> lanes_log2);
+  const int d = 4 * (threadIdx.x & ((1 << lanes_log2) - 1));
   if (e >= min(q.queries, a.max_query) * a.query_heads || d >= D) return;
   const int64_t row = (int64_t)q.first * a.query_heads + e;
   const float2* const stats = plan.stats + row * plan.splits;
   const float* const sums = plan.sums + row * plan.splits * D + d;
+  // kAtOnce parts' loads together, then their sums with a running maximum
+  constexpr int kAtOnce = 8;
   float top = -INFINITY, total = 0;
-  for (int s = 0; s < parts; ++s) top = fmaxf(top, stats[s].x);
   f32x4 v = {0, 0, 0, 0};
-  for (int s = 0; s < parts; ++s) {
-    const float2 st = stats[s];
-    if (st.x == -INFINITY) continue;
-    const float f = __builtin_amdgcn_exp2f(st.x - top);
-    total += st.y * f;
-    v += *(const KVMI_GLOBAL f32x4*)(sums + (int64_t)s * D) * f;
+  for (int s0 = 0; s0 < parts; s0 += kAtOnce) {
+    float2 st[kAtOnce];
+    f32x4 x[kAtOnce];
+#pragma unroll
+    for (int s = 0; s < kAtOnce; ++s) {
+      const int at = min(s0 + s, parts - 1);
+      st[s] = stats[at];
+      x[s] = *(const KVMI_GLOBAL f32x4*)(sums + (int64_t)at * D);
+      if (s0 + s >= parts) st[s].x = -INFINITY;
+    }
+    float most = top;
+#pragma unroll
+    for (int s = 0; s < kAtOnce; ++s) most = fmaxf(most, st[s].x);
+    const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - most);
+    total *= f;
+    v *= f;
+    top = most;
+#pragma unroll
+    for (int s = 0; s < kAtOnce; ++s)
+      if (st[s].x != -INFINITY) {
+        const float g = __builtin_amdgcn_exp2f(st[s].x - top);
+        total += st[s].y * g;
+        v += x[s] * g;
+      }
   }
   const float f = total == 0 ? 0.0f : 1.0f / total;
   gst((uint2*)((uint16_t*)a.out + row * D + d),
@@ -368,15 +413,26 @@ Choice choose(const kvmi_attention_args& a) {
   c.rows = rows <= (D <= 128 ? 32 : 16);
   const int64_t length = a.max_length < 1 ? 1 : a.max_length;
   c.plan.block = block_of(a.cache.block_size);
+  c.plan.group = block_of(G);
   c.plan.waves = 4;
   c.plan.row_tiles = 1;
   if (!c.rows) c.plan.row_tiles = (int)((rows + 127) / 128);
-  const int64_t groups = (int64_t)a.requests * a.cache.num_heads * c.plan.row_tiles;
-  c.plan.chunk = c.rows ? 1024 : 512;
-  int64_t splits = (length + c.plan.chunk - 1) / c.plan.chunk;
-  if (!c.rows) splits = std::min<int64_t>(splits, (1024 + groups - 1) / groups);
-  splits = std::min<int64_t>(splits, 64);
-  if (!c.rows && splits > 1) c.plan.chunk = (int)((length + splits - 1) / splits);
+  // Row tiles that have rows: requests may differ in queries, but not add up to more than all.
+  const int64_t tiles = std::min<int64_t>((int64_t)a.requests * c.plan.row_tiles,
+                                          (int64_t)a.total_queries * G / 128 + a.requests);
+  const int64_t groups = tiles * a.cache.num_heads;
+  // Keys are split until there are workgroups for the chip, one a CU for few rows (a workgroup
+  // then keeps 4 waves' loads in flight) and two for tiles, but not below the part at which the
+  // join costs more than it saves: 64 keys of few rows (512 keys of one token: 7.5 us in 8 parts,
+  // 8.3 in 4, 8.8 in 16, 9.6 whole), 256 of tiles.  Few rows are split at 1024 keys in any case,
+  // against requests of unequal lengths (64 of 1 to 12 Ki: 320 us; 330 at 512, 328 at 4096).
+  const int64_t want = std::max<int64_t>(1, ((c.rows ? 256 : 512) + groups - 1) / groups);
+  c.plan.chunk = (int)std::max<int64_t>((length + want - 1) / want, c.rows ? 64 : 256);
+  if (c.rows) {
+    c.plan.chunk = std::min(c.plan.chunk, 1024);
+    c.plan.waves = std::min(4, (c.plan.chunk + kStep - 1) / kStep);
+  }
+  int64_t splits = std::min<int64_t>((length + c.plan.chunk - 1) / c.plan.chunk, 64);
   while (splits > 1 && ((int64_t)c.plan.row_tiles * splits > 65535 || parts_bytes(a, (int)splits) > (1LL << 31))) splits /= 2;
   c.plan.splits = (int)splits;
   return c;
@@ -443,14 +499,15 @@ extern "C" int kvmi_tree_attention(const kvmi_attention_args* args, kvmi_stream_
     launch_rows<KVMI_DTYPE_FP16>(a, c, st);
   }
   if (c.plan.splits > 1) {
-    int lanes = 2;
-    while (4 * lanes < a.cache.head_dim) lanes *= 2;
+    int lanes_log2 = 1;
+    while ((4 << lanes_log2) < a.cache.head_dim) ++lanes_log2;
+    const int per = 256 >> lanes_log2;
     const int64_t rows = (int64_t)a.max_query * a.query_heads;
-    const dim3 grid((unsigned)((rows + 256 / lanes - 1) / (256 / lanes)), (unsigned)a.requests);
+    const dim3 grid((unsigned)((rows + per - 1) / per), (unsigned)a.requests);
     if (bf16)
-      hipLaunchKernelGGL((join_kernel<KVMI_DTYPE_BF16>), grid, dim3(256), 0, st, a, c.plan, lanes);
+      hipLaunchKernelGGL((join_kernel<KVMI_DTYPE_BF16>), grid, dim3(256), 0, st, a, c.plan, lanes_log2);
     else
-      hipLaunchKernelGGL((join_kernel<KVMI_DTYPE_FP16>), grid, dim3(256), 0, st, a, c.plan, lanes);
+      hipLaunchKernelGGL((join_kernel<KVMI_DTYPE_FP16>), grid, dim3(256), 0, st, a, c.plan, lanes_log2);
   }
   return hipGetLastError() == hipSuccess ? KVMI_OK : KVMI_ELAUNCH;
 }

@@ -21,7 +21,7 @@ constexpr float kRaise = 8.0f;
 
 // How the keys of a request are split over workgroups and where the parts go.
 struct AttendPlan {
-  BlockOf block;
+  BlockOf block, group;  // by the block size, by the query heads of a KV head
   int waves;      // of a workgroup
   int row_tiles;  // tiles kernel: row tiles of a KV head, 32 rows a wave
   int splits;     // the most parts of a request
@@ -49,6 +49,11 @@ __device__ __forceinline__ Request request_of(const kvmi_attention_args& a, int 
 // Parts that a request of so many tokens has.
 __device__ __forceinline__ int parts_of(const AttendPlan& p, int length) {
   return min(p.splits, max(1, (length + p.chunk - 1) / p.chunk));
+}
+
+// Where part `part` of `parts` of n tiles begins (n < 2^26, 64 parts at most).
+__device__ __forceinline__ int part_begin(int n, int part, int parts) {
+  return parts == 1 ? n * part : (int)((uint32_t)n * (uint32_t)part / (uint32_t)parts);
 }
 
 // Element offset of a token's row from the part's base, from its block's id and its place in the

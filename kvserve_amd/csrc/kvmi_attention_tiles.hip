@@ -88,20 +88,20 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
 
   // keys that any row of the workgroup sees end at `end`; those before `all` are seen by all
   const int last_row = min(m0 + 32 * waves, M) - 1;
-  const int end = masks ? q.length : min(q.length, q.prefix + last_row / G + 1);
-  const int all = masks ? q.prefix : q.prefix + m0 / G + 1;
+  const int end = masks ? q.length : min(q.length, q.prefix + plan.group(last_row) + 1);
+  const int all = masks ? q.prefix : q.prefix + plan.group(m0) + 1;
   const int w0 = m0 + 32 * wave;
-  const int w_all = masks ? q.prefix : q.prefix + w0 / G + 1;
+  const int w_all = masks ? q.prefix : q.prefix + plan.group(w0) + 1;
   const int tiles = (q.length + kKeys - 1) / kKeys;
-  const int t0 = (int)((int64_t)tiles * part / parts);
-  const int t1 = min((int)((int64_t)tiles * (part + 1) / parts), (end + kKeys - 1) / kKeys);
+  const int t0 = part_begin(tiles, part, parts);
+  const int t1 = min(part_begin(tiles, part + 1, parts), (end + kKeys - 1) / kKeys);
   const int hiding = min(all, end) >> 6;  // the first tile with a key that some row does not see
   // this wave's: its rows see nothing from tile w1 on
-  const int w_end = masks ? end : min(end, q.prefix + min(w0 + 31, M - 1) / G + 1);
+  const int w_end = masks ? end : min(end, q.prefix + plan.group(min(w0 + 31, M - 1)) + 1);
   const int w1 = w0 >= M ? t0 : min(t1, (w_end + kKeys - 1) / kKeys), w_hiding = min(w_all, q.length) >> 6;
 
   // this lane's row
-  const int m = min(w0 + col, M - 1), qi = m / G, qh = head * G + m - qi * G;
+  const int m = min(w0 + col, M - 1), qi = plan.group(m), qh = head * G + m - qi * G;
   const int64_t row = q.first + qi;
   const uint64_t* const mask = masks ? masks + row * a.mask_words : nullptr;
   u32x4v qf[2 * NT];

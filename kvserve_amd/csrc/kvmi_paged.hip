@@ -13,14 +13,20 @@ __device__ __forceinline__ void flag_error(int32_t* err, int32_t bits) {
   if (err && bits) atomicOr(err, bits);
 }
 
-// Sum over the workgroup, given to every thread.
-__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* lds) {
+// Sums of N values over the workgroup, given to every thread.
+template <int N>
+__device__ __forceinline__ void block_sum(int64_t (&v)[N], int64_t (&lds)[N][4]) {
 #pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v[n] += __shfl_xor(v[n], d, 64);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 0)
+#pragma unroll
+    for (int n = 0; n < N; ++n) lds[n][threadIdx.x >> 6] = v[n];
   __syncthreads();
-  return lds[0] + lds[1] + lds[2] + lds[3];
+#pragma unroll
+  for (int n = 0; n < N; ++n) v[n] = lds[n][0] + lds[n][1] + lds[n][2] + lds[n][3];
 }
 
 // ---------------------------------------------------------------- block tables
@@ -57,19 +63,18 @@ __device__ __forceinline__ uint32_t ring_at(uint32_t base, uint32_t i, uint32_t 
 // another workgroup writes.  A ring holds every block of the pool, so the places behind the
 // last free block never reach the head's: blocks returned here are not read here.
 __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a, BlockOf div) {
-  __shared__ int64_t lds[4];
+  __shared__ int64_t lds[3][4];
   __shared__ int last;
   const int r = blockIdx.x, tid = threadIdx.x;
-  int64_t take = 0, give = 0, tokens = 0;
+  int64_t before[3] = {0, 0, 0};  // what the requests before this one take, give back and grow by
   for (int i = tid; i < r; i += kThreads) {
     const Need n = need_of(a, div, i);
-    take += n.take();
-    give += n.give();
-    tokens += n.tokens();
+    before[0] += n.take();
+    before[1] += n.give();
+    before[2] += n.tokens();
   }
-  take = block_sum(take, lds);
-  give = block_sum(give, lds);
-  tokens = block_sum(tokens, lds);
+  block_sum(before, lds);
+  const int64_t take = before[0], give = before[1], tokens = before[2];
   const Need n = need_of(a, div, r);
   const int N = a.ring;
   const int head = (int)((uint32_t)a.state[0] % (uint32_t)N);
@@ -79,39 +84,58 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a, Bl
   const int keep = granted ? n.want : n.have;
   const bool in_place = a.out_tables == a.tables;
   const int64_t row = (int64_t)r * a.columns;
-  const int64_t step = (int64_t)kThreads * gridDim.y;
-  const int64_t lane = (int64_t)blockIdx.y * kThreads + tid;
   // where this request takes blocks (looked at only where it fits: take <= N) and gives them back
   const uint32_t from = ring_at(head, fits ? (uint32_t)take : 0, N);
   const uint32_t to = (uint32_t)((uint64_t)(head + (int64_t)count + give) % (uint32_t)N);
+  // A thread takes kUnroll entries at a time: all their loads, then their stores.  (One by one,
+  // each waiting for its load, a request that brought 8192 tokens took 11 us by itself.)
+  constexpr int kUnroll = 8;
+  const int64_t step = (int64_t)kThreads * gridDim.y;
+  const int64_t lane = (int64_t)blockIdx.y * kThreads + tid;
 
   // the table row: blocks kept, blocks taken, and -1 behind them; the blocks given back go
   // behind the last free one
   const int lo = in_place ? (n.have < keep ? n.have : keep) : 0;
   const int hi = in_place ? (n.have > keep ? n.have : keep) : a.columns;
-  for (int64_t k = lo + lane; k < hi; k += step) {
-    const int32_t old = k < n.have ? a.tables[row + k] : -1;
-    int32_t id = old;
-    if (k >= keep) {
-      if (k < n.have) a.free_blocks[ring_at(to, (uint32_t)(k - keep), N)] = old;
-      id = -1;
-    } else if (k >= n.have) {
-      id = a.free_blocks[ring_at(from, (uint32_t)(k - n.have), N)];
+  for (int64_t k0 = lo + lane; k0 < hi; k0 += step * kUnroll) {
+    int32_t id[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t k = k0 + u * step;
+      id[u] = -1;
+      if (k < hi && k < n.have)
+        id[u] = gld(a.tables + row + k);
+      else if (k < hi && k < keep)
+        id[u] = gld(a.free_blocks + ring_at(from, (uint32_t)(k - n.have), N));
     }
-    a.out_tables[row + k] = id;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t k = k0 + u * step;
+      if (k >= hi) break;
+      if (k >= keep && k < n.have) gst(a.free_blocks + ring_at(to, (uint32_t)(k - keep), N), id[u]);
+      gst(a.out_tables + row + k, k < keep ? id[u] : -1);
+    }
   }
 
   // the new tokens' slots
-  for (int64_t i = lane; i < n.tokens(); i += step) {
-    const int64_t at = tokens + i;
-    if (at >= a.max_tokens) break;
-    int64_t slot = -1;
-    if (granted) {
-      const int p = n.now + (int)i, k = div(p);
-      const int32_t id = k < n.have ? a.tables[row + k] : a.free_blocks[ring_at(from, k - n.have, N)];
-      slot = (int64_t)id * a.block_size + (p - k * a.block_size);
+  const int64_t fit = a.max_tokens - tokens, grown = n.tokens() < fit ? n.tokens() : fit;
+  for (int64_t i0 = lane; i0 < grown; i0 += step * kUnroll) {
+    int64_t slot[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = i0 + u * step;
+      slot[u] = -1;
+      if (granted && i < grown) {
+        const int p = n.now + (int)i, k = div(p);
+        const int32_t id = k < n.have ? gld(a.tables + row + k) : gld(a.free_blocks + ring_at(from, k - n.have, N));
+        slot[u] = (int64_t)id * a.block_size + (p - k * a.block_size);
+      }
     }
-    a.slots[at] = slot;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = i0 + u * step;
+      if (i < grown) gst(a.slots + tokens + i, slot[u]);
+    }
   }
   const int64_t upto = tokens + n.tokens();
   if (r == a.requests - 1)
@@ -141,8 +165,7 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a, Bl
   const int64_t all_give = give + (granted ? n.give() : 0);
   int64_t taken = take + n.take(), returned = all_give;
   if (over || !fits) {
-    int64_t before = 0, fit = 0;
-    returned = 0;
+    int64_t asked = 0, sum[2] = {0, 0};  // taken by those that fit, given back
     for (int base = 0; base < a.requests; base += kThreads) {
       const int i = base + tid;
       Need m{};
@@ -155,20 +178,22 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a, Bl
         if ((tid & 63) >= d) s += t;
       }
       __syncthreads();
-      if ((tid & 63) == 63) lds[tid >> 6] = s;
+      if ((tid & 63) == 63) lds[0][tid >> 6] = s;
       __syncthreads();
-      int64_t carry = before;
-      for (int w = 0; w < (tid >> 6); ++w) carry += lds[w];
-      const int64_t piece = lds[0] + lds[1] + lds[2] + lds[3];
+      int64_t carry = asked;
+      for (int w = 0; w < (tid >> 6); ++w) carry += lds[0][w];
+      const int64_t piece = lds[0][0] + lds[0][1] + lds[0][2] + lds[0][3];
       s += carry;
       const bool ok = s <= count;
       if (over && i < a.requests && !m.bad) a.out_lengths[i] = ok || m.take() == 0 ? m.next : m.now;
-      fit += i < a.requests && ok ? m.take() : 0;
-      returned += m.give();
-      before += piece;
+      sum[0] += i < a.requests && ok ? m.take() : 0;
+      sum[1] += m.give();
+      asked += piece;
     }
-    taken = block_sum(fit, lds);
-    returned = block_sum(returned, lds);
+    int64_t (&two)[2][4] = *reinterpret_cast<int64_t (*)[2][4]>(lds);
+    block_sum(sum, two);
+    taken = sum[0];
+    returned = sum[1];
   }
   if (tid == 0) {
     a.out_state[0] = (int)((head + taken) % N);
