@@ -336,45 +336,47 @@ __global__ __launch_bounds__(256) void join_kernel(kvmi_attention_args a, Attend
   const Request q = request_of(a, r, false);
   const int parts = parts_of(plan, q.length);
   if (parts == 1) return;
-  const int e = (int)(blockIdx.x << (8 - lanes_log2)) + (threadIdx.x >> lanes_log2);
-  const int d = 4 * (threadIdx.x & ((1 << lanes_log2) - 1));
-  if (e >= min(q.queries, a.max_query) * a.query_heads || d >= D) return;
-  const int64_t row = (int64_t)q.first * a.query_heads + e;
-  const float2* const stats = plan.stats + row * plan.splits;
-  const float* const sums = plan.sums + row * plan.splits * D + d;
-  // kAtOnce parts' loads together, then their sums with a running maximum
-  constexpr int kAtOnce = 8;
-  float top = -INFINITY, total = 0;
-  f32x4 v = {0, 0, 0, 0};
-  for (int s0 = 0; s0 < parts; s0 += kAtOnce) {
-    float2 st[kAtOnce];
-    f32x4 x[kAtOnce];
+  const int d = 4 * (threadIdx.x & ((1 << lanes_log2) - 1)), per = 256 >> lanes_log2;
+  const int rows = min(q.queries, a.max_query) * a.query_heads;
+  if (d >= D) return;
+  for (int e = (int)blockIdx.x * per + (threadIdx.x >> lanes_log2); e < rows; e += (int)gridDim.x * per) {
+    const int64_t row = (int64_t)q.first * a.query_heads + e;
+    const float2* const stats = plan.stats + row * plan.splits;
+    const float* const sums = plan.sums + row * plan.splits * D + d;
+    // kAtOnce parts' loads together, then their sums with a running maximum
+    constexpr int kAtOnce = 8;
+    float top = -INFINITY, total = 0;
+    f32x4 v = {0, 0, 0, 0};
+    for (int s0 = 0; s0 < parts; s0 += kAtOnce) {
+      float2 st[kAtOnce];
+      f32x4 x[kAtOnce];
 #pragma unroll
-    for (int s = 0; s < kAtOnce; ++s) {
-      const int at = min(s0 + s, parts - 1);
-      st[s] = stats[at];
-      x[s] = *(const KVMI_GLOBAL f32x4*)(sums + (int64_t)at * D);
-      if (s0 + s >= parts) st[s].x = -INFINITY;
-    }
-    float most = top;
-#pragma unroll
-    for (int s = 0; s < kAtOnce; ++s) most = fmaxf(most, st[s].x);
-    const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - most);
-    total *= f;
-    v *= f;
-    top = most;
-#pragma unroll
-    for (int s = 0; s < kAtOnce; ++s)
-      if (st[s].x != -INFINITY) {
-        const float g = __builtin_amdgcn_exp2f(st[s].x - top);
-        total += st[s].y * g;
-        v += x[s] * g;
+      for (int s = 0; s < kAtOnce; ++s) {
+        const int at = min(s0 + s, parts - 1);
+        st[s] = stats[at];
+        x[s] = *(const KVMI_GLOBAL f32x4*)(sums + (int64_t)at * D);
+        if (s0 + s >= parts) st[s].x = -INFINITY;
       }
+      float most = top;
+#pragma unroll
+      for (int s = 0; s < kAtOnce; ++s) most = fmaxf(most, st[s].x);
+      const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - most);
+      total *= f;
+      v *= f;
+      top = most;
+#pragma unroll
+      for (int s = 0; s < kAtOnce; ++s)
+        if (st[s].x != -INFINITY) {
+          const float g = __builtin_amdgcn_exp2f(st[s].x - top);
+          total += st[s].y * g;
+          v += x[s] * g;
+        }
+    }
+    const float f = total == 0 ? 0.0f : 1.0f / total;
+    gst((uint2*)((uint16_t*)a.out + row * D + d),
+        make_uint2(pack2<DT>(v[0] * f, v[1] * f), pack2<DT>(v[2] * f, v[3] * f)));
+    if (a.lse && d == 0) a.lse[row] = total == 0 ? -INFINITY : (top + __builtin_amdgcn_logf(total)) / kLog2e;
   }
-  const float f = total == 0 ? 0.0f : 1.0f / total;
-  gst((uint2*)((uint16_t*)a.out + row * D + d),
-      make_uint2(pack2<DT>(v[0] * f, v[1] * f), pack2<DT>(v[2] * f, v[3] * f)));
-  if (a.lse && d == 0) a.lse[row] = total == 0 ? -INFINITY : (top + __builtin_amdgcn_logf(total)) / kLog2e;
 }
 
 bool attention_ok(const kvmi_attention_args* a) {
@@ -426,7 +428,8 @@ Choice choose(const kvmi_attention_args& a) {
   // join costs more than it saves: 64 keys of few rows (512 keys of one token: 7.5 us in 8 parts,
   // 8.3 in 4, 8.8 in 16, 9.6 whole), 256 of tiles.  Few rows are split at 1024 keys in any case,
   // against requests of unequal lengths (64 of 1 to 12 Ki: 320 us; 330 at 512, 328 at 4096).
-  const int64_t want = std::max<int64_t>(1, ((c.rows ? 256 : 512) + groups - 1) / groups);
+  const bool even = (int64_t)a.requests * c.plan.row_tiles <= tiles;  // not more than there is room for
+  const int64_t room = c.rows ? 256 : 512, want = std::max<int64_t>(1, (room + (even ? 0 : groups - 1)) / groups);
   c.plan.chunk = (int)std::max<int64_t>((length + want - 1) / want, c.rows ? 64 : 256);
   if (c.rows) {
     c.plan.chunk = std::min(c.plan.chunk, 1024);
@@ -503,7 +506,9 @@ extern "C" int kvmi_tree_attention(const kvmi_attention_args* args, kvmi_stream_
     while ((4 << lanes_log2) < a.cache.head_dim) ++lanes_log2;
     const int per = 256 >> lanes_log2;
     const int64_t rows = (int64_t)a.max_query * a.query_heads;
-    const dim3 grid((unsigned)((rows + per - 1) / per), (unsigned)a.requests);
+    // (requests of fewer queries than the most leave workgroups without rows)
+    const int64_t most = std::max<int64_t>(1, 4096 / a.requests);
+    const dim3 grid((unsigned)std::min((rows + per - 1) / per, most), (unsigned)a.requests);
     if (bf16)
       hipLaunchKernelGGL((join_kernel<KVMI_DTYPE_BF16>), grid, dim3(256), 0, st, a, c.plan, lanes_log2);
     else

@@ -35,11 +35,10 @@ struct Request {
   int length, prefix;  // cached tokens, and those before the queries (negative: fewer than queries)
 };
 __device__ __forceinline__ Request request_of(const kvmi_attention_args& a, int r, bool report) {
-  int s0 = a.starts[r], s1 = a.starts[r + 1], err = 0;
+  int s0 = cld(a.starts + r), s1 = cld(a.starts + r + 1), len = cld(a.lengths + r), err = 0;
   if (s0 < 0 || s1 < s0 || s1 > a.total_queries || s1 - s0 > a.max_query) err |= KVMI_ERR_LENGTH;
   s0 = min(max(s0, 0), a.total_queries);
   s1 = min(max(s1, s0), a.total_queries);
-  int len = a.lengths[r];
   const int top = a.columns * a.cache.block_size;
   if (len < 0 || len > top) err |= KVMI_ERR_LENGTH;
   len = min(max(len, 0), top);

@@ -100,21 +100,6 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
   const int w_end = masks ? end : min(end, q.prefix + plan.group(min(w0 + 31, M - 1)) + 1);
   const int w1 = w0 >= M ? t0 : min(t1, (w_end + kKeys - 1) / kKeys), w_hiding = min(w_all, q.length) >> 6;
 
-  // this lane's row
-  const int m = min(w0 + col, M - 1), qi = plan.group(m), qh = head * G + m - qi * G;
-  const int64_t row = q.first + qi;
-  const uint64_t* const mask = masks ? masks + row * a.mask_words : nullptr;
-  u32x4v qf[2 * NT];
-  {
-    const uint16_t* qp = (const uint16_t*)a.query + row * a.query_token_stride + qh * a.query_head_stride;
-#pragma unroll
-    for (int k = 0; k < 2 * NT; ++k) {
-      const int d = 16 * k + 8 * half;
-      qf[k] = d < D ? ld16(qp + d) : u32x4v{0, 0, 0, 0};
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < 2 * NT; ++k) arrive(qf[k]);
   const float c = a.scale * kLog2e;
   float mx = -INFINITY, l = 0;
   f32x16 o[NT];
@@ -133,6 +118,22 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
     id = gld(table + at);
   };
   auto note = [&](int t) { offs[(t + wave) & 7][lane] = row_offset(a, id, place); };
+  if (t0 < t1) look_up(t0);
+
+  // this lane's row
+  const int m = min(w0 + col, M - 1), qi = plan.group(m), qh = head * G + m - qi * G;
+  const int64_t row = q.first + qi;
+  const uint64_t* const mask = masks ? masks + row * a.mask_words : nullptr;
+  u32x4v qf[2 * NT];
+  {
+    const uint16_t* qp = (const uint16_t*)a.query + row * a.query_token_stride + qh * a.query_head_stride;
+#pragma unroll
+    for (int k = 0; k < 2 * NT; ++k) {
+      const int d = 16 * k + 8 * half;
+      qf[k] = d < D ? ld16(qp + d) : u32x4v{0, 0, 0, 0};
+    }
+  }
+
   // pieces of 16 bytes in the order of LDS, 64 an instruction; NT instructions of K's and of V's
   // a wave where there are 4 waves
   auto load = [&](int t) {
@@ -158,12 +159,13 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
       }
     }
     if (tid < 4) odd[tid >> 1][tid & 1] = 0;
-    look_up(t0);
     note(t0);
     __syncthreads();
     load(t0);
     __syncthreads();
   }
+#pragma unroll
+  for (int k = 0; k < 2 * NT; ++k) arrive(qf[k]);
   for (int t = t0; t < t1; ++t) {
     const bool look = ((t - t0) & 3) == 0;
     if (look) look_up(t + 4);
