@@ -436,8 +436,10 @@ Choice choose(const kvmi_attention_args& a) {
     c.plan.waves = std::min(4, (c.plan.chunk + kStep - 1) / kStep);
   }
   int64_t splits = std::min<int64_t>((length + c.plan.chunk - 1) / c.plan.chunk, 64);
-  while (splits > 1 && ((int64_t)c.plan.row_tiles * splits > 65535 || parts_bytes(a, (int)splits) > (1LL << 31))) splits /= 2;
+  while (splits > 1 && parts_bytes(a, (int)splits) > (1LL << 31)) splits /= 2;
   c.plan.splits = (int)splits;
+  c.plan.tiles = block_of(c.plan.row_tiles * (int)splits);
+  c.plan.heads = block_of(a.cache.num_heads);
   return c;
 }
 
@@ -485,7 +487,8 @@ extern "C" int kvmi_tree_attention(const kvmi_attention_args* args, kvmi_stream_
     return KVMI_EINVAL;
   Choice c = choose(a);
   const int64_t space = parts_bytes(a, c.plan.splits);
-  if (c.plan.row_tiles * (int64_t)c.plan.splits > 65535 ||
+  // the tiles kernel's workgroups are numbered in 31 bits
+  if ((!c.rows && ((int64_t)a.requests * a.cache.num_heads + 7) / 8 * 8 * c.plan.row_tiles * c.plan.splits > 0x7fffffffLL) ||
       (space && (!a.workspace || a.workspace_bytes < space || (uintptr_t)a.workspace % 16)))
     return KVMI_EINVAL;
   c.plan.sums = (float*)a.workspace;

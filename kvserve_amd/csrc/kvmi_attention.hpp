@@ -22,6 +22,7 @@ constexpr float kRaise = 8.0f;
 // How the keys of a request are split over workgroups and where the parts go.
 struct AttendPlan {
   BlockOf block, group;  // by the block size, by the query heads of a KV head
+  BlockOf tiles, heads;  // tiles kernel: by row_tiles * splits, by the KV heads
   int waves;      // of a workgroup
   int row_tiles;  // tiles kernel: row tiles of a KV head, 32 rows a wave
   int splits;     // the most parts of a request
