@@ -22,7 +22,9 @@ __host__ __device__ constexpr int next_pow2(int x) {
 struct BlockOf {
   uint32_t m;
   int shift;
-  __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> shift); }
+  __device__ __forceinline__ int operator()(int x) const {
+    return shift == 31 ? x : (int)(__umulhi((uint32_t)x, m) >> (shift - 32));  // (31: S == 1)
+  }
 };
 inline BlockOf block_of(int block_size) {
   int l = 0;

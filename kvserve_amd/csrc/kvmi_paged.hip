@@ -13,21 +13,16 @@ __device__ __forceinline__ void flag_error(int32_t* err, int32_t bits) {
   if (err && bits) atomicOr(err, bits);
 }
 
-// Sums of N values over the workgroup, given to every thread.
-template <int N>
-__device__ __forceinline__ void block_sum(int64_t (&v)[N], int64_t (&lds)[N][4]) {
+// Sum over the workgroup, given to every thread.
+__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* lds) {
 #pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v[n] += __shfl_xor(v[n], d, 64);
+  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0)
-#pragma unroll
-    for (int n = 0; n < N; ++n) lds[n][threadIdx.x >> 6] = v[n];
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-#pragma unroll
-  for (int n = 0; n < N; ++n) v[n] = lds[n][0] + lds[n][1] + lds[n][2] + lds[n][3];
+  return lds[0] + lds[1] + lds[2] + lds[3];
 }
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
 
 // ---------------------------------------------------------------- block tables
 struct Need {  // what one request's change of length asks for
@@ -37,16 +32,19 @@ struct Need {  // what one request's change of length asks for
   __device__ int give() const { return have > want ? have - want : 0; }
   __device__ int tokens() const { return next > now ? next - now : 0; }
 };
-__device__ __forceinline__ Need need_of(const kvmi_tables_args& a, const BlockOf& div, int r) {
+__device__ __forceinline__ Need need_of(const kvmi_tables_args& a, const BlockOf& div, int now, int next) {
   Need n;
   const int top = a.columns * a.block_size;
-  n.now = a.lengths[r];
-  n.next = a.new_lengths[r];
-  n.bad = n.now < 0 || n.now > top || n.next < 0 || n.next > top;
-  if (n.bad) n.next = n.now = n.now < 0 ? 0 : n.now > top ? top : n.now;
-  n.have = n.now ? div(n.now - 1) + 1 : 0;
-  n.want = n.next ? div(n.next - 1) + 1 : 0;
+  n.bad = (uint32_t)now > (uint32_t)top || (uint32_t)next > (uint32_t)top;
+  if (n.bad) next = now = now < 0 ? 0 : now > top ? top : now;
+  n.now = now;
+  n.next = next;
+  n.have = now ? div(now - 1) + 1 : 0;
+  n.want = next ? div(next - 1) + 1 : 0;
   return n;
+}
+__device__ __forceinline__ Need need_of(const kvmi_tables_args& a, const BlockOf& div, int r) {
+  return need_of(a, div, a.lengths[r], a.new_lengths[r]);
 }
 // Place of the i-th entry behind `base` (< N) in a ring of N; past 2 N only where the free count
 // and the blocks given back exceed the ring.
@@ -63,83 +61,118 @@ __device__ __forceinline__ uint32_t ring_at(uint32_t base, uint32_t i, uint32_t 
 // another workgroup writes.  A ring holds every block of the pool, so the places behind the
 // last free block never reach the head's: blocks returned here are not read here.
 __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a, BlockOf div) {
-  __shared__ int64_t lds[3][4];
+  __shared__ uint32_t sums[3][4];
+  __shared__ int64_t lds[4];
   __shared__ int last;
   const int r = blockIdx.x, tid = threadIdx.x;
-  int64_t before[3] = {0, 0, 0};  // what the requests before this one take, give back and grow by
-  for (int i = tid; i < r; i += kThreads) {
-    const Need n = need_of(a, div, i);
-    before[0] += n.take();
-    before[1] += n.give();
-    before[2] += n.tokens();
-  }
-  block_sum(before, lds);
-  const int64_t take = before[0], give = before[1], tokens = before[2];
   const Need n = need_of(a, div, r);
   const int N = a.ring;
   const int head = (int)((uint32_t)a.state[0] % (uint32_t)N);
   const int count = a.state[1] < 0 ? 0 : a.state[1] > N ? N : a.state[1];
+
+  // What the requests before this one take, give back and grow by.  Blocks add up to less than
+  // the table's entries, 2^31; tokens stay at 2^32 - 1, past any slot map.
+  uint32_t before[3] = {0, 0, 0};
+  for (int i0 = 0; i0 < r; i0 += 4 * kThreads) {  // four loads at a time
+    int now[4], next[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = min(i0 + u * kThreads + tid, r - 1);
+      if (i0 + u * kThreads < r) {
+        now[u] = gld(a.lengths + i);
+        next[u] = gld(a.new_lengths + i);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i0 + u * kThreads < r) {
+        const Need m = need_of(a, div, now[u], next[u]);
+        if (i0 + u * kThreads + tid < r) {
+          before[0] += m.take();
+          before[1] += m.give();
+          before[2] = add_sat(before[2], m.tokens());
+        }
+      }
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    before[0] += __shfl_xor(before[0], d, 64);
+    before[1] += __shfl_xor(before[1], d, 64);
+    before[2] = add_sat(before[2], __shfl_xor(before[2], d, 64));
+  }
+  if ((tid & 63) == 0)
+#pragma unroll
+    for (int x = 0; x < 3; ++x) sums[x][tid >> 6] = before[x];
+  __syncthreads();
+  const int64_t take = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+  const int64_t give = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
+  const int64_t tokens = add_sat(add_sat(sums[2][0], sums[2][1]), add_sat(sums[2][2], sums[2][3]));
+
   const bool fits = take + n.take() <= count;
   const bool granted = fits || n.take() == 0;
   const int keep = granted ? n.want : n.have;
   const bool in_place = a.out_tables == a.tables;
-  const int64_t row = (int64_t)r * a.columns;
+  const int32_t* const old = a.tables + (int64_t)r * a.columns;
+  int32_t* const out = a.out_tables + (int64_t)r * a.columns;
+  const int step = kThreads * gridDim.y, lane = blockIdx.y * kThreads + tid;
   // where this request takes blocks (looked at only where it fits: take <= N) and gives them back
   const uint32_t from = ring_at(head, fits ? (uint32_t)take : 0, N);
   const uint32_t to = (uint32_t)((uint64_t)(head + (int64_t)count + give) % (uint32_t)N);
-  // A thread takes kUnroll entries at a time: all their loads, then their stores.  (One by one,
-  // each waiting for its load, a request that brought 8192 tokens took 11 us by itself.)
-  constexpr int kUnroll = 8;
-  const int64_t step = (int64_t)kThreads * gridDim.y;
-  const int64_t lane = (int64_t)blockIdx.y * kThreads + tid;
 
   // the table row: blocks kept, blocks taken, and -1 behind them; the blocks given back go
   // behind the last free one
-  const int lo = in_place ? (n.have < keep ? n.have : keep) : 0;
-  const int hi = in_place ? (n.have > keep ? n.have : keep) : a.columns;
-  for (int64_t k0 = lo + lane; k0 < hi; k0 += step * kUnroll) {
-    int32_t id[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t k = k0 + u * step;
-      id[u] = -1;
-      if (k < hi && k < n.have)
-        id[u] = gld(a.tables + row + k);
-      else if (k < hi && k < keep)
-        id[u] = gld(a.free_blocks + ring_at(from, (uint32_t)(k - n.have), N));
+  const int lo = in_place ? min(n.have, keep) : 0;
+  const int hi = in_place ? max(n.have, keep) : a.columns;
+  auto entry = [&](int k) -> int32_t {  // the row's entry k
+    if (k < min(n.have, keep)) return gld(old + k);
+    if (k < keep) return gld(a.free_blocks + ring_at(from, k - n.have, N));
+    return -1;
+  };
+  if (!in_place && (a.columns & 3) == 0 && (((uintptr_t)a.tables | (uintptr_t)a.out_tables) & 15) == 0) {
+    // four entries a thread: most of a row is kept, or -1
+    for (int k = 4 * lane; k < a.columns; k += 4 * step) {
+      uint4 v = make_uint4(~0u, ~0u, ~0u, ~0u);
+      if (k + 4 <= min(n.have, keep)) {
+        v = gld((const uint4*)(old + k));
+      } else if (k < keep) {
+        v.x = entry(k);
+        v.y = entry(k + 1);
+        v.z = entry(k + 2);
+        v.w = entry(k + 3);
+      }
+      gst((uint4*)(out + k), v);
     }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t k = k0 + u * step;
-      if (k >= hi) break;
-      if (k >= keep && k < n.have) gst(a.free_blocks + ring_at(to, (uint32_t)(k - keep), N), id[u]);
-      gst(a.out_tables + row + k, k < keep ? id[u] : -1);
+    for (int k = keep + lane; k < n.have; k += step) gst(a.free_blocks + ring_at(to, k - keep, N), gld(old + k));
+  } else {
+    for (int k = lo + lane; k < hi; k += step) {
+      const int32_t had = k >= keep && k < n.have ? gld(old + k) : -1;
+      if (k >= keep && k < n.have) gst(a.free_blocks + ring_at(to, k - keep, N), had);
+      gst(out + k, entry(k));
     }
   }
 
   // the new tokens' slots
-  const int64_t fit = a.max_tokens - tokens, grown = n.tokens() < fit ? n.tokens() : fit;
-  for (int64_t i0 = lane; i0 < grown; i0 += step * kUnroll) {
-    int64_t slot[kUnroll];
+  const int64_t room = a.max_tokens - tokens;
+  const int grown = room <= 0 ? 0 : (int)min((int64_t)n.tokens(), room);
+  auto slot_of = [&](int i) -> int64_t {
+    const int p = n.now + i, k = div(p);
+    const int32_t id = gld(k < n.have ? old + k : a.free_blocks + ring_at(from, k - n.have, N));
+    return (int64_t)id * a.block_size + (p - k * a.block_size);
+  };
+  int64_t* const slots = a.slots + tokens;
+  int i = lane;
+  if (granted)  // all of a thread's loads before its stores, where it has several
+    for (; i + 3 * (int64_t)step < grown; i += 4 * step) {
+      int64_t v[4];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t i = i0 + u * step;
-      slot[u] = -1;
-      if (granted && i < grown) {
-        const int p = n.now + (int)i, k = div(p);
-        const int32_t id = k < n.have ? gld(a.tables + row + k) : gld(a.free_blocks + ring_at(from, k - n.have, N));
-        slot[u] = (int64_t)id * a.block_size + (p - k * a.block_size);
-      }
-    }
+      for (int u = 0; u < 4; ++u) v[u] = slot_of(i + u * step);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t i = i0 + u * step;
-      if (i < grown) gst(a.slots + tokens + i, slot[u]);
+      for (int u = 0; u < 4; ++u) gst(slots + i + u * step, v[u]);
     }
-  }
+  for (; i < grown; i += step) gst(slots + i, granted ? slot_of(i) : (int64_t)-1);
   const int64_t upto = tokens + n.tokens();
   if (r == a.requests - 1)
-    for (int64_t i = upto + lane; i < a.max_tokens; i += step) a.slots[i] = -1;
+    for (int64_t k = upto + lane; k < a.max_tokens; k += step) gst(a.slots + k, (int64_t)-1);
   if (blockIdx.y == 0 && tid == 0) {
     if (r == 0) a.starts[0] = 0;
     a.starts[r + 1] = upto > 0x7fffffff ? 0x7fffffff : (int)upto;
@@ -165,7 +198,8 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a, Bl
   const int64_t all_give = give + (granted ? n.give() : 0);
   int64_t taken = take + n.take(), returned = all_give;
   if (over || !fits) {
-    int64_t asked = 0, sum[2] = {0, 0};  // taken by those that fit, given back
+    int64_t asked = 0, fit = 0;
+    returned = 0;
     for (int base = 0; base < a.requests; base += kThreads) {
       const int i = base + tid;
       Need m{};
@@ -178,22 +212,20 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a, Bl
         if ((tid & 63) >= d) s += t;
       }
       __syncthreads();
-      if ((tid & 63) == 63) lds[0][tid >> 6] = s;
+      if ((tid & 63) == 63) lds[tid >> 6] = s;
       __syncthreads();
       int64_t carry = asked;
-      for (int w = 0; w < (tid >> 6); ++w) carry += lds[0][w];
-      const int64_t piece = lds[0][0] + lds[0][1] + lds[0][2] + lds[0][3];
+      for (int w = 0; w < (tid >> 6); ++w) carry += lds[w];
+      const int64_t piece = lds[0] + lds[1] + lds[2] + lds[3];
       s += carry;
       const bool ok = s <= count;
       if (over && i < a.requests && !m.bad) a.out_lengths[i] = ok || m.take() == 0 ? m.next : m.now;
-      sum[0] += i < a.requests && ok ? m.take() : 0;
-      sum[1] += m.give();
+      fit += i < a.requests && ok ? m.take() : 0;
+      returned += m.give();
       asked += piece;
     }
-    int64_t (&two)[2][4] = *reinterpret_cast<int64_t (*)[2][4]>(lds);
-    block_sum(sum, two);
-    taken = sum[0];
-    returned = sum[1];
+    taken = block_sum(fit, lds);
+    returned = block_sum(returned, lds);
   }
   if (tid == 0) {
     a.out_state[0] = (int)((head + taken) % N);
@@ -249,58 +281,83 @@ struct KeepArgs {
   int32_t* out_lengths;
   int32_t* err;
   int columns, width, layers;
+  BlockOf block;
 };
 constexpr int kMaxPath = 1024;
 
 // Workgroup (request, layer).  The path is checked as a whole before anything moves.  A thread
 // owns one 16-byte (or 2-byte) column of the row and walks the path in order, so no thread waits
 // for another: path[i] >= i and the path increases, hence a row is read before, or in the same
-// step as, it is overwritten.
-template <class V>
+// step as, it is overwritten.  Bound by its chain of loads (path, tables, rows): a path of up to
+// 64 is checked by every wave for itself, a draft a lane, without a barrier.
+template <class V, bool SHORT>
 __global__ __launch_bounds__(kThreads) void keep_kernel(KeepArgs a) {
   constexpr int U = sizeof(V) / 2, kStep = 8;
-  __shared__ int64_t src[kMaxPath], dst[kMaxPath];
+  __shared__ int64_t src[SHORT ? 1 : kMaxPath], dst[SHORT ? 1 : kMaxPath];
   __shared__ int count;
-  const int r = blockIdx.x, layer = blockIdx.y, tid = threadIdx.x;
+  const int r = blockIdx.x, layer = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const int32_t* path = a.accepted + (int64_t)r * a.width;
+  const int32_t* const table = a.tables + (int64_t)r * a.columns;
   const int S = a.cache.block_size;
   const int64_t base = a.lengths[r], top = (int64_t)a.columns * S;
-  if (tid == 0) count = a.width;
-  __syncthreads();
-  for (int i = tid; i < a.width; i += kThreads)
-    if (path[i] < 0) atomicMin(&count, i);
-  __syncthreads();
-  const int n = count;
-  int bad = base < 0 || base > top ? KVMI_ERR_LENGTH : 0;
-  if (!bad)
-    for (int i = tid; i < n; i += kThreads) {
-      const int64_t from = base + path[i], to = base + i;
-      if ((i && path[i] <= path[i - 1]) || from >= top) {
-        bad |= KVMI_ERR_LENGTH;
-        continue;
-      }
-      const int32_t fb = a.tables[(int64_t)r * a.columns + from / S], tb = a.tables[(int64_t)r * a.columns + to / S];
-      if (fb < 0 || fb >= a.cache.num_blocks || tb < 0 || tb >= a.cache.num_blocks) bad |= KVMI_ERR_BLOCK_ID;
-      const int64_t row = (int64_t)a.cache.num_heads * a.cache.head_dim;
-      src[i] = (int64_t)fb * a.cache.block_stride + (from % S) * row;
-      dst[i] = (int64_t)tb * a.cache.block_stride + (to % S) * row;
+  const int64_t row = (int64_t)a.cache.num_heads * a.cache.head_dim;
+  int bad = base < 0 || base > top ? KVMI_ERR_LENGTH : 0, n;
+  int64_t lane_src = 0, lane_dst = 0;
+  // draft i of the path, `before` the one ahead of it: where it lies and where it goes
+  auto place = [&](int i, int draft, int before, int64_t* from_row, int64_t* to_row) {
+    const int64_t from = base + draft, to = base + i;
+    if ((i && draft <= before) || from >= top) {
+      bad |= KVMI_ERR_LENGTH;
+      return;
     }
-  if (bad && layer == 0) flag_error(a.err, bad);
-  const int any = __syncthreads_or(bad);
-  if (layer == 0 && tid == 0) a.out_lengths[r] = (int)base + (any ? 0 : n);
-  if (any) return;
-  const int per_part = a.cache.num_heads * a.cache.head_dim / U;
-  for (int p = tid; p < 2 * per_part; p += kThreads) {
-    const int part = p >= per_part;
-    uint16_t* col = (uint16_t*)a.bases[layer] + part * a.cache.part_stride + (int64_t)(p - part * per_part) * U;
+    const int fc = a.block((int)from), tc = a.block((int)to);
+    const int32_t fb = gld(table + fc), tb = gld(table + tc);
+    if (fb < 0 || fb >= a.cache.num_blocks || tb < 0 || tb >= a.cache.num_blocks) bad |= KVMI_ERR_BLOCK_ID;
+    *from_row = (int64_t)fb * a.cache.block_stride + (from - (int64_t)fc * S) * row;
+    *to_row = (int64_t)tb * a.cache.block_stride + (to - (int64_t)tc * S) * row;
+  };
+  if constexpr (SHORT) {
+    const int draft = lane < a.width ? gld(path + lane) : -1, before = __shfl_up(draft, 1, 64);
+    const uint64_t ends = __ballot(draft < 0);
+    n = ends ? __builtin_ctzll(ends) : 64;
+    if (!bad && lane < n) place(lane, draft, before, &lane_src, &lane_dst);
+    if (bad && layer == 0 && tid < 64) flag_error(a.err, bad);
+    bad = __ballot(bad) != 0;
+  } else {
+    if (tid == 0) count = a.width;
+    __syncthreads();
+    for (int i = tid; i < a.width; i += kThreads)
+      if (path[i] < 0) atomicMin(&count, i);
+    __syncthreads();
+    n = count;
+    if (!bad)
+      for (int i = tid; i < n; i += kThreads) place(i, path[i], i ? path[i - 1] : -1, &src[i], &dst[i]);
+    if (bad && layer == 0) flag_error(a.err, bad);
+    bad = __syncthreads_or(bad);
+  }
+  if (layer == 0 && tid == 0) a.out_lengths[r] = (int)base + (bad ? 0 : n);
+  if (bad) return;
+  auto from_row = [&](int i) -> int64_t { return SHORT ? __shfl(lane_src, i, 64) : src[i]; };
+  auto to_row = [&](int i) -> int64_t { return SHORT ? __shfl(lane_dst, i, 64) : dst[i]; };
+  const int per_part = a.cache.num_heads * a.cache.head_dim / U, all = 2 * per_part;
+  const int64_t layer_base = (int64_t)(uintptr_t)gld((const int64_t*)a.bases + layer);
+  for (int p0 = 0; p0 < all; p0 += kThreads) {
+    const int p = p0 + tid, part = p >= per_part;
+    uint16_t* col = (uint16_t*)layer_base + part * a.cache.part_stride + (int64_t)(p - part * per_part) * U;
     for (int i0 = 0; i0 < n; i0 += kStep) {
       V held[kStep];
 #pragma unroll
-      for (int i = 0; i < kStep; ++i)
-        if (i0 + i < n && src[i0 + i] != dst[i0 + i]) held[i] = gld((const V*)(col + src[i0 + i]));
+      for (int i = 0; i < kStep; ++i) {
+        if (i0 + i >= n) break;
+        const int64_t from = from_row(i0 + i);
+        if (p < all && from != to_row(i0 + i)) held[i] = gld((const V*)(col + from));
+      }
 #pragma unroll
-      for (int i = 0; i < kStep; ++i)
-        if (i0 + i < n && src[i0 + i] != dst[i0 + i]) gst((V*)(col + dst[i0 + i]), held[i]);
+      for (int i = 0; i < kStep; ++i) {
+        if (i0 + i >= n) break;
+        const int64_t to = to_row(i0 + i);
+        if (p < all && from_row(i0 + i) != to) gst((V*)(col + to), held[i]);
+      }
     }
   }
 }
@@ -324,7 +381,8 @@ extern "C" int kvmi_build_tables(const kvmi_tables_args* args, kvmi_stream_t str
   if (!args) return KVMI_EINVAL;
   const kvmi_tables_args& a = *args;
   if (a.requests < 0 || a.columns < 1 || a.ring < 1 || a.block_size < 1 || a.max_tokens < 0) return KVMI_EINVAL;
-  if ((int64_t)a.columns * a.block_size > 0x7fffffffLL || (int64_t)a.ring * a.block_size > 0x7fffffffLL)
+  if ((int64_t)a.columns * a.block_size > 0x7fffffffLL || (int64_t)a.ring * a.block_size > 0x7fffffffLL ||
+      (int64_t)a.columns * a.requests > 0x7fffffffLL)
     return KVMI_EINVAL;
   if (a.requests == 0) return KVMI_OK;
   if (!a.lengths || !a.new_lengths || !a.tables || !a.free_blocks || !a.state || !a.out_tables || !a.out_lengths ||
@@ -336,7 +394,7 @@ extern "C" int kvmi_build_tables(const kvmi_tables_args* args, kvmi_stream_t str
   // several workgroups share one, 4096 slots each.  Every part adds up the requests before its
   // own again, so there are no more than that needs (64 parts of 1024 requests took 153 us).
   const int64_t parts = std::max<int64_t>(
-      1, std::min<int64_t>(((int64_t)a.max_tokens + 4095) / 4096, std::min(64, 1024 / a.requests)));
+      1, std::min<int64_t>(((int64_t)a.max_tokens + 4095) / 4096, std::min(64, 2048 / a.requests)));
   hipLaunchKernelGGL(tables_kernel, dim3((unsigned)a.requests, (unsigned)parts), dim3(kThreads), 0,
                      reinterpret_cast<hipStream_t>(stream), a, block_of(a.block_size));
   return launched();
@@ -382,13 +440,19 @@ extern "C" int kvmi_keep_drafts(const kvmi_cache* cache, void* const* bases, int
   if (requests == 0) return KVMI_OK;
   if (!bases || !tables || !lengths || !out_lengths || (width && !accepted) || lengths == out_lengths)
     return KVMI_EINVAL;
-  KeepArgs a{*cache, bases, tables, lengths, accepted, out_lengths, err, columns, width, layers};
+  KeepArgs a{*cache, bases, tables, lengths, accepted, out_lengths, err, columns, width, layers,
+             block_of(cache->block_size)};
   const dim3 grid((unsigned)requests, (unsigned)layers);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   // `cache->base` tells how the bases are aligned: the caller passes the OR of all of them
-  if (strides16(cache) && aligned16(cache->base))
-    hipLaunchKernelGGL((keep_kernel<uint4>), grid, dim3(kThreads), 0, st, a);
+  const bool wide = strides16(cache) && aligned16(cache->base);
+  if (width <= 64 && wide)
+    hipLaunchKernelGGL((keep_kernel<uint4, true>), grid, dim3(kThreads), 0, st, a);
+  else if (width <= 64)
+    hipLaunchKernelGGL((keep_kernel<uint16_t, true>), grid, dim3(kThreads), 0, st, a);
+  else if (wide)
+    hipLaunchKernelGGL((keep_kernel<uint4, false>), grid, dim3(kThreads), 0, st, a);
   else
-    hipLaunchKernelGGL((keep_kernel<uint16_t>), grid, dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((keep_kernel<uint16_t, false>), grid, dim3(kThreads), 0, st, a);
   return launched();
 }
