@@ -285,6 +285,12 @@ struct KeepArgs {
 };
 constexpr int kMaxPath = 1024;
 
+// Lane i's value, i the same for all; lanes that have left count too, unlike in a shuffle.
+__device__ __forceinline__ int64_t lane_value(int64_t v, int i) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, i) |
+                   (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32);
+}
+
 // Workgroup (request, layer).  The path is checked as a whole before anything moves.  A thread
 // owns one 16-byte (or 2-byte) column of the row and walks the path in order, so no thread waits
 // for another: path[i] >= i and the path increases, hence a row is read before, or in the same
@@ -337,8 +343,8 @@ __global__ __launch_bounds__(kThreads) void keep_kernel(KeepArgs a) {
   }
   if (layer == 0 && tid == 0) a.out_lengths[r] = (int)base + (bad ? 0 : n);
   if (bad) return;
-  auto from_row = [&](int i) -> int64_t { return SHORT ? __shfl(lane_src, i, 64) : src[i]; };
-  auto to_row = [&](int i) -> int64_t { return SHORT ? __shfl(lane_dst, i, 64) : dst[i]; };
+  auto from_row = [&](int i) -> int64_t { return SHORT ? lane_value(lane_src, i) : src[i]; };
+  auto to_row = [&](int i) -> int64_t { return SHORT ? lane_value(lane_dst, i) : dst[i]; };
   const int per_part = a.cache.num_heads * a.cache.head_dim / U, all = 2 * per_part;
   const int64_t layer_base = (int64_t)(uintptr_t)gld((const int64_t*)a.bases + layer);
   for (int p0 = 0; p0 < all; p0 += kThreads) {
