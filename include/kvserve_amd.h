@@ -553,12 +553,12 @@ int kvmi_write_kv(const kvmi_cache* cache, const void* key, const void* value, i
  * (and lse -inf).  What a query does not see does not touch its result, NaN and infinities
  * included.
  *   query, out  [total_queries][query_heads][D], query with strides in elements (channels
- *               adjacent, 16-byte aligned rows), out contiguous; query head h reads KV head
+ *               adjacent, 16-byte aligned rows), out contiguous and 16-byte aligned; query head h reads KV head
  *               h / (query_heads / num_heads)
  *   lse         fp32 [total_queries][query_heads] natural log of the sums, or null
  *   max_query   no request may have more queries (KVMI_ERR_LENGTH, the rows past it unwritten)
- *   max_length  the longest length, for the launch shape only: any value gives the same sums up
- *               to the order of their parts
+ *   max_length  the longest length, for the launch shape only (keys are split over workgroups by
+ *               it): any value gives the same sums up to the order of their parts
  *   workspace   kvmi_attention_workspace_bytes of the same arguments, 16-byte aligned
  * D is a multiple of 8 up to 256.  A block id outside the cache sets KVMI_ERR_BLOCK_ID (the
  * nearest block is read in its place), a length outside [0, columns * S] or a range outside the

@@ -333,6 +333,13 @@ def tree_attention(query: torch.Tensor, cache: torch.Tensor, tables: torch.Tenso
             query, cache, tables, lengths, starts, max_query, max_length, tree_mask, scale, out, err):
         return out
     lse = torch.full(query.shape[:2], -math.inf, dtype=torch.float32, device=query.device) if return_lse else None
+    if isinstance(out, torch.Tensor) and out.data_ptr() % 16 and out.is_contiguous():
+        # the kernels write 8 and 16 bytes at a time
+        whole = tree_attention(query, cache, tables, lengths, starts, max_query=max_query, max_length=max_length,
+                               tree_mask=tree_mask, scale=scale, out=out.clone(), return_lse=return_lse, check=check,
+                               err=err)
+        out.copy_(whole[0] if return_lse else whole)
+        return (out, whole[1]) if return_lse else out
     args, query = _attention_args(query, cache, tables, lengths, starts, max_query, max_length, tree_mask, scale, out,
                                   lse)
     call = _Call(cache.device, check, err)

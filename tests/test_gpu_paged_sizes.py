@@ -130,3 +130,17 @@ def test_pages_that_end_inside_a_tile_hold_what_they_will(cuda):
         lens = [(n + t, t) for n in (0, 1, 62, 63, 64, 65, 99, 100, 101, 163, 164, 165, 499)]
         d = make(cuda, lens, 2, G, 128, 100, seed=t)
         hold(d, *call(d, return_lse=True))
+
+
+def test_outputs_off_their_alignment(cuda):
+    """Any contiguous output will do; rows of no request stay as they are."""
+    d = make(cuda, [(90, 3), (20, 20)], 2, 4, 64, 16, seed=21)
+    want = call(d)
+    for check in (True, False):
+        for skip in (1, 2, 4):
+            out = torch.full((want.numel() + skip,), 7.0, dtype=want.dtype, device=cuda)[skip:].view_as(want)
+            assert call(d, out=out, check=check) is out and torch.equal(out, want)
+            short = dict(d, starts=torch.tensor([0, 3, 10], dtype=torch.int32, device=cuda))
+            out.fill_(7.0)
+            call(short, out=out, check=check)
+            assert (out[10:] == 7.0).all() and not (out[:10] == 7.0).all(-1).any()
