@@ -418,17 +418,28 @@ Choice choose(const kvmi_attention_args& a) {
   c.plan.group = block_of(G);
   c.plan.waves = 4;
   c.plan.row_tiles = 1;
-  if (!c.rows) c.plan.row_tiles = (int)((rows + 127) / 128);
   // Row tiles that have rows: requests may differ in queries, but not add up to more than all.
-  const int64_t tiles = std::min<int64_t>((int64_t)a.requests * c.plan.row_tiles,
-                                          (int64_t)a.total_queries * G / 128 + a.requests);
+  auto tiles_of = [&](int tile) -> int64_t {
+    return std::min<int64_t>(a.requests * ((rows + tile - 1) / tile), (int64_t)a.total_queries * G / tile + a.requests);
+  };
+  int64_t tiles = a.requests;
+  if (!c.rows) {
+    // Tiles of 256 rows where those alone fill every CU twice over, for 97 to 128 channels, whose
+    // 4 waves have half a CU's registers: a tile of keys is loaded once for both halves (a prompt
+    // of 8192: 577 -> 555 us; 64 channels, three workgroups of 4 waves a CU: 332 -> 368), and are
+    // mostly full.
+    const bool full = rows >= 1024 || (rows + 127) / 128 % 2 == 0;
+    if (D > 96 && D <= 128 && full && tiles_of(256) * a.cache.num_heads >= 512) c.plan.waves = 8;
+    c.plan.row_tiles = (int)((rows + 32 * c.plan.waves - 1) / (32 * c.plan.waves));
+    tiles = tiles_of(32 * c.plan.waves);
+  }
   const int64_t groups = tiles * a.cache.num_heads;
   // Keys are split until there are workgroups for the chip, one a CU for few rows (a workgroup
   // then keeps 4 waves' loads in flight) and two for tiles, but not below the part at which the
   // join costs more than it saves: 64 keys of few rows (512 keys of one token: 7.5 us in 8 parts,
   // 8.3 in 4, 8.8 in 16, 9.6 whole), 256 of tiles.  Few rows are split at 1024 keys in any case,
   // against requests of unequal lengths (64 of 1 to 12 Ki: 320 us; 330 at 512, 328 at 4096).
-  const bool even = (int64_t)a.requests * c.plan.row_tiles <= tiles;  // not more than there is room for
+  const bool even = (int64_t)a.requests * c.plan.row_tiles <= tiles;  // all have the most queries
   const int64_t room = c.rows ? 256 : 512, want = std::max<int64_t>(1, (room + (even ? 0 : groups - 1)) / groups);
   c.plan.chunk = (int)std::max<int64_t>((length + want - 1) / want, c.rows ? 64 : 256);
   if (c.rows) {

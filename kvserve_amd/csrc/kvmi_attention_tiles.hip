@@ -1,4 +1,4 @@
-// Attention over the paged cache for many rows: tiles of 128 query rows against 64 keys.
+// Attention over the paged cache for many rows: tiles of 128 or 256 query rows against 64 keys.
 //
 // The rows of a KV head are its queries' heads, row m = query m / G, head m % G.  A wave holds
 // 32 rows as the columns of its matrix products:
@@ -61,8 +61,9 @@ struct Turn {
 
 // NT: 32-channel tiles of a head, D <= 32 * NT.
 // WHOLE: D == 32 * NT, no channels to leave out.
-template <int DT, int NT, bool WHOLE>
-__global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi_attention_args a, AttendPlan plan) {
+// W: waves, of 32 rows each.
+template <int DT, int NT, bool WHOLE, int W>
+__global__ __launch_bounds__(64 * W, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi_attention_args a, AttendPlan plan) {
   constexpr int PC = 4 * NT, RS = 16 * PC, kPart = kKeys * RS;  // chunks and bytes of a row, bytes of a tile
   using T = Turn<PC>;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kPart];  // K and V of two tiles
@@ -73,7 +74,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
 
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  constexpr int waves = 4, threads = 256;
+  constexpr int threads = 64 * W, kRows = 32 * W, NP = PC / W;  // NP: a wave's instructions to load a K or V tile
   // Workgroups go to the XCDs in turn: all of a request's KV head go to one, one after the other,
   // so that its L2 has their keys (trees of 7 x 26 rows 56.7 -> 54.2 us); the last rows, which see
   // the most, first.
@@ -84,7 +85,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
   const int tile = plan.row_tiles - 1 - (y - part * plan.row_tiles);
   const Request q = request_of(a, r, tid == 0);
   const int D = a.cache.head_dim, H = a.cache.num_heads, G = a.query_heads / H;
-  const int M = min(q.queries, a.max_query) * G, m0 = tile * 32 * waves;
+  const int M = min(q.queries, a.max_query) * G, m0 = tile * kRows;
   if (m0 >= M) return;
   const int parts = parts_of(plan, q.length);
   if (part >= parts) return;
@@ -93,7 +94,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
   const uint16_t* const values = keys + a.cache.part_stride;
 
   // keys that any row of the workgroup sees end at `end`; those before `all` are seen by all
-  const int last_row = min(m0 + 32 * waves, M) - 1;
+  const int last_row = min(m0 + kRows, M) - 1;
   const int end = masks ? q.length : min(q.length, q.prefix + plan.group(last_row) + 1);
   const int all = masks ? q.prefix : q.prefix + plan.group(m0) + 1;
   const int w0 = m0 + 32 * wave;
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
 #pragma unroll
     for (int x = 0; x < 16; ++x) o[n][x] = 0;
 
-  // Every 4th tile each wave looks one of the next 4 tiles' keys up, a key a lane; the ids are
+  // Every 4th tile each of the first 4 waves looks one of the next 4 tiles' keys up, a key a lane; the ids are
   // loaded ahead of a tile's loads, and waited for without waiting for those.
   const int32_t* const table = a.tables + (int64_t)r * a.columns;
   int place = 0, id = 0;
@@ -124,7 +125,8 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
     id = gld(table + at);
   };
   auto note = [&](int t) { offs[(t + wave) & 7][lane] = row_offset(a, id, place); };
-  if (t0 < t1) look_up(t0);
+  const bool looks = W == 4 || wave < 4;
+  if (t0 < t1 && looks) look_up(t0);
 
   // this lane's row
   const int m = min(w0 + col, M - 1), qi = plan.group(m), qh = head * G + m - qi * G;
@@ -144,15 +146,15 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
   // a wave where there are 4 waves
   auto load = [&](int t) {
     uint8_t* const kb = lds + (t & 1) * 2 * kPart + wave * 1024;
-    int64_t off[NT];
+    int64_t off[NP];
 #pragma unroll
-    for (int k = 0; k < NT; ++k) off[k] = offs[t & 7][((k * waves + wave) * 64 + lane) / PC];
+    for (int k = 0; k < NP; ++k) off[k] = offs[t & 7][((k * W + wave) * 64 + lane) / PC];
 #pragma unroll
-    for (int k = 0; k < NT; ++k) {
-      const int idx = (k * waves + wave) * 64 + lane, key = idx / PC, at = idx - key * PC;
+    for (int k = 0; k < NP; ++k) {
+      const int idx = (k * W + wave) * 64 + lane, key = idx / PC, at = idx - key * PC;
       const int ck = T::chunk(at, T::key(key)), cv = T::chunk(at, T::value(key));
-      if (WHOLE || ck * 8 < D) to_lds(keys + ck * 8 + off[k], kb + k * waves * 1024);
-      if (WHOLE || cv * 8 < D) to_lds(values + cv * 8 + off[k], kb + kPart + k * waves * 1024);
+      if (WHOLE || ck * 8 < D) to_lds(keys + ck * 8 + off[k], kb + k * W * 1024);
+      if (WHOLE || cv * 8 < D) to_lds(values + cv * 8 + off[k], kb + kPart + k * W * 1024);
     }
   };
 
@@ -165,7 +167,7 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
       }
     }
     if (tid < 4) odd[tid >> 1][tid & 1] = 0;
-    note(t0);
+    if (looks) note(t0);
     __syncthreads();
     load(t0);
     __syncthreads();
@@ -173,9 +175,11 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
 #pragma unroll
   for (int k = 0; k < 2 * NT; ++k) arrive(qf[k]);
   for (int t = t0; t < t1; ++t) {
-    const bool look = ((t - t0) & 3) == 0;
+    const bool look = looks && ((t - t0) & 3) == 0;
     if (look) look_up(t + 4);
-    if (t + 1 < t1) load(t + 1);
+    // (two pairs of waves a SIMD, W = 8, all wait at one barrier: their loads go behind the first
+    // product's reads, 5 % faster; two workgroups of 4 waves, which run apart, are 5 % slower so)
+    if (t + 1 < t1 && (W == 4 || t >= w1)) load(t + 1);
     uint32_t bad0 = 0, bad1 = 0;
     if (t >= hiding) {
       // some row does not see some key here: its weight is zero, and so must its product be.
@@ -215,6 +219,10 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
         for (int b = 0; b < 2; ++b) s[b] = mma32<DT>(*(const u32x4v*)(kp + 32 * b * RS), qf[k], s[b]);
       }
       interleave<4 * NT, 1, 4>();
+      if constexpr (W == 8) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (t + 1 < t1) load(t + 1);
+      }
       uint64_t seen = ~0ull;
       if (t >= w_hiding) {
         seen = seen_bits(q, mask, a.mask_words, qi, p0);
@@ -329,26 +337,25 @@ __global__ __launch_bounds__(256, NT <= 4 ? 2 : 1) void attend_tiles_kernel(kvmi
   }
 }
 
-template <int DT, int NT>
+template <int DT, int NT, int W>
 void launch(const kvmi_attention_args& a, const AttendPlan& p, hipStream_t st) {
   const int64_t pairs = ((int64_t)a.requests * a.cache.num_heads + 7) / 8 * 8;
-  const dim3 grid((unsigned)(pairs * p.row_tiles * p.splits));
-  const dim3 threads((unsigned)(64 * p.waves));
+  const dim3 grid((unsigned)(pairs * p.row_tiles * p.splits)), threads(64 * W);
   if (a.cache.head_dim == 32 * NT)
-    hipLaunchKernelGGL((attend_tiles_kernel<DT, NT, true>), grid, threads, 0, st, a, p);
+    hipLaunchKernelGGL((attend_tiles_kernel<DT, NT, true, W>), grid, threads, 0, st, a, p);
   else
-    hipLaunchKernelGGL((attend_tiles_kernel<DT, NT, false>), grid, threads, 0, st, a, p);
+    hipLaunchKernelGGL((attend_tiles_kernel<DT, NT, false, W>), grid, threads, 0, st, a, p);
 }
 template <int DT>
 void launch(const kvmi_attention_args& a, const AttendPlan& p, hipStream_t st) {
   switch ((a.cache.head_dim + 31) / 32) {
     case 1:
-    case 2: return launch<DT, 2>(a, p, st);
-    case 3: return launch<DT, 3>(a, p, st);
-    case 4: return launch<DT, 4>(a, p, st);
-    case 5: return launch<DT, 5>(a, p, st);
-    case 6: return launch<DT, 6>(a, p, st);
-    default: return launch<DT, 8>(a, p, st);
+    case 2: return launch<DT, 2, 4>(a, p, st);
+    case 3: return launch<DT, 3, 4>(a, p, st);
+    case 4: return p.waves == 8 ? launch<DT, 4, 8>(a, p, st) : launch<DT, 4, 4>(a, p, st);
+    case 5: return launch<DT, 5, 4>(a, p, st);
+    case 6: return launch<DT, 6, 4>(a, p, st);
+    default: return launch<DT, 8, 4>(a, p, st);
   }
 }
 
