@@ -243,6 +243,7 @@ struct WriteArgs {
   int64_t tokens;
   int32_t* err;
   int lanes_log2;  // lanes of a token, a power of two up to the workgroup
+  BlockOf block, head;  // by the block size, by a head's units
 };
 
 // A group of 2^lanes_log2 lanes copies one token's K and V rows in units of V (16 bytes, or 2
@@ -260,10 +261,12 @@ __global__ __launch_bounds__(kThreads) void write_kernel(WriteArgs a) {
     if (slot != -1 && lane == 0) flag_error(a.err, KVMI_ERR_BLOCK_ID);
     return;
   }
-  const int64_t place = (slot / S) * a.cache.block_stride + (slot % S) * a.cache.num_heads * a.cache.head_dim;
+  const int block = a.block((int)slot);
+  const int64_t place = block * a.cache.block_stride +
+                        (int64_t)((int)slot - block * S) * (a.cache.num_heads * a.cache.head_dim);
   for (int p = lane; p < 2 * per_part; p += lanes) {
     const int part = p >= per_part, q = p - part * per_part;
-    const int head = q / per_head;
+    const int head = a.head(q);
     const uint16_t* src = a.rows[part] + tok * a.token_stride[part] + head * a.head_stride[part] +
                           (int64_t)(q - head * per_head) * U;
     uint16_t* dst = (uint16_t*)a.cache.base + part * a.cache.part_stride + place + (int64_t)q * U;
@@ -420,11 +423,14 @@ extern "C" int kvmi_write_kv(const kvmi_cache* cache, const void* key, const voi
               slots,
               tokens,
               err,
-              8};
+              8,
+              block_of(cache->block_size),
+              {}};
   const bool wide = strides16(cache) && aligned16(cache->base) && aligned16(key) && aligned16(value) &&
                     key_token_stride % 8 == 0 && key_head_stride % 8 == 0 && value_token_stride % 8 == 0 &&
                     value_head_stride % 8 == 0;
   const int units = 2 * cache->num_heads * cache->head_dim / (wide ? 8 : 1);
+  a.head = block_of(wide ? cache->head_dim / 8 : cache->head_dim);
   while (a.lanes_log2 > 0 && (1 << (a.lanes_log2 - 1)) >= units) --a.lanes_log2;
   const int64_t per_wg = kThreads >> a.lanes_log2, grid = (tokens + per_wg - 1) / per_wg;
   if (grid > 0x7fffffffLL) return KVMI_EINVAL;
