@@ -15,7 +15,10 @@ constexpr int kStep = 32;  // keys a wave takes at a time
 //   O^T += V^T P^T  a lane loads 16 bytes of each of its 8 keys, 16 lanes a whole row of 128
 //                   channels; pairs of keys are brought together by byte permutes, and the
 //                   output row of tile j is channel 8 * row + j
-// so that nothing goes through LDS before the waves' sums are joined at the end.
+// so that nothing goes through LDS before the waves' sums are joined at the end.  64 requests of
+// 1 to 12 Ki tokens, 32 heads over 8, 128 channels: 322 us with the join, 5.1 TB/s, as fast as a
+// copy reads and writes; 32 rows 3.7 TB/s, 256 channels 4.2; one token over 512, a chain of loads,
+// 7.5 us.
 // N8 / N4: panels of 128 / 64 channels.  Past 128 channels, or 16 rows, the queries stay in LDS and
 // are read again for every 32 keys: with them in registers a wave would not fit its 256.  Past 192
 // it does not fit them either way, and has a SIMD's 512 to itself.
@@ -24,7 +27,7 @@ __global__ __launch_bounds__((N8 == 2 ? 256 : 512), (N8 == 2 ? 1 : 2)) void atte
                                                                                              AttendPlan plan) {
   constexpr bool kShared = (N8 + N4 > 1 || R > 1) && N8 < 2;
   constexpr int KS = 4 * N8 + 2 * N4, OT = 8 * N8 + 4 * N4;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // [waves][rows][D] sums
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // [waves][16 rows][D] sums
   __shared__ int64_t offs[8][2][kStep];
   __shared__ float2 stat[8][16 * R];
   // chunk c of row m at c ^ (m % 16): 16 rows' reads meet every bank once
@@ -268,8 +271,9 @@ __global__ __launch_bounds__((N8 == 2 ? 256 : 512), (N8 == 2 ? 1 : 2)) void atte
     buf ^= 1;
   }
 
-  // the waves' sums, brought to their common maximum and added up in the waves' order
-  const int rows = min(M, 16 * R), DP = D + 4;
+  // the waves' sums, brought to their common maximum and added up in the waves' order, 16 rows at
+  // a time (32 at once take the LDS of two workgroups)
+  const int DP = D + 4;
   float* const sums = (float*)lds;
 #pragma unroll
   for (int x = 0; x < R; ++x) {
@@ -279,12 +283,14 @@ __global__ __launch_bounds__((N8 == 2 ? 256 : 512), (N8 == 2 ? 1 : 2)) void atte
   __syncthreads();
 #pragma unroll
   for (int x = 0; x < R; ++x) {
-    const int m = 16 * x + col;
+    const int rows = min(M - 16 * x, 16);
+    if (rows <= 0) break;
+    if (x) __syncthreads();
     float top = -INFINITY;
-    for (int w = 0; w < waves; ++w) top = fmaxf(top, stat[w][m].x);
+    for (int w = 0; w < waves; ++w) top = fmaxf(top, stat[w][16 * x + col].x);
     const float f = mx[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx[x] - top);
-    if (m < rows) {
-      float* const dst = sums + (wave * rows + m) * DP;
+    if (col < rows) {
+      float* const dst = sums + (wave * 16 + col) * DP;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -299,36 +305,37 @@ __global__ __launch_bounds__((N8 == 2 ? 256 : 512), (N8 == 2 ? 1 : 2)) void atte
         }
       }
     }
-  }
-  __syncthreads();
-  // D / 4 lanes, or the next power of two, a row
-  const int lanes_log2 = D > 128 ? 6 : D > 64 ? 5 : D > 32 ? 4 : D > 16 ? 3 : 2;
-  for (int e = threadIdx.x; e < rows << lanes_log2; e += blockDim.x) {
-    const int m = e >> lanes_log2, d = 4 * (e - (m << lanes_log2));
-    if (d >= D) continue;
-    float top = -INFINITY, total = 0;
-    for (int w = 0; w < waves; ++w) top = fmaxf(top, stat[w][m].x);
-    f32x4 v = {0, 0, 0, 0};
-    for (int w = 0; w < waves; ++w) {
-      const float2 s = stat[w][m];
-      total += s.x == -INFINITY ? 0.0f : s.y * __builtin_amdgcn_exp2f(s.x - top);
-      v += *(const f32x4*)(sums + (w * rows + m) * DP + d);
-    }
-    const int i = plan.group(m);
-    const int64_t out_row = (int64_t)(q.first + i) * a.query_heads + head * G + m - i * G;
-    if (parts == 1) {
-      const float f = total == 0 ? 0.0f : 1.0f / total;
-      gst((uint2*)((uint16_t*)a.out + out_row * D + d),
-          make_uint2(pack2<DT>(v[0] * f, v[1] * f), pack2<DT>(v[2] * f, v[3] * f)));
-      if (a.lse && d == 0) a.lse[out_row] = total == 0 ? -INFINITY : (top + __builtin_amdgcn_logf(total)) / kLog2e;
-    } else {
-      *(KVMI_GLOBAL f32x4*)(plan.sums + (out_row * plan.splits + part) * D + d) = v;
-      if (d == 0) plan.stats[out_row * plan.splits + part] = make_float2(top, total);
+    __syncthreads();
+    // D / 4 lanes, or the next power of two, a row
+    const int lanes_log2 = D > 128 ? 6 : D > 64 ? 5 : D > 32 ? 4 : D > 16 ? 3 : 2;
+    for (int e = threadIdx.x; e < rows << lanes_log2; e += blockDim.x) {
+      const int at = e >> lanes_log2, d = 4 * (e - (at << lanes_log2)), m = 16 * x + at;
+      if (d >= D) continue;
+      float most = -INFINITY, total = 0;
+      for (int w = 0; w < waves; ++w) most = fmaxf(most, stat[w][m].x);
+      f32x4 v = {0, 0, 0, 0};
+      for (int w = 0; w < waves; ++w) {
+        const float2 s = stat[w][m];
+        total += s.x == -INFINITY ? 0.0f : s.y * __builtin_amdgcn_exp2f(s.x - most);
+        v += *(const f32x4*)(sums + (w * 16 + at) * DP + d);
+      }
+      const int i = plan.group(m);
+      const int64_t out_row = (int64_t)(q.first + i) * a.query_heads + head * G + m - i * G;
+      if (parts == 1) {
+        const float f = total == 0 ? 0.0f : 1.0f / total;
+        gst((uint2*)((uint16_t*)a.out + out_row * D + d),
+            make_uint2(pack2<DT>(v[0] * f, v[1] * f), pack2<DT>(v[2] * f, v[3] * f)));
+        if (a.lse && d == 0) a.lse[out_row] = total == 0 ? -INFINITY : (most + __builtin_amdgcn_logf(total)) / kLog2e;
+      } else {
+        *(KVMI_GLOBAL f32x4*)(plan.sums + (out_row * plan.splits + part) * D + d) = v;
+        if (d == 0) plan.stats[out_row * plan.splits + part] = make_float2(most, total);
+      }
     }
   }
 }
 
-// The parts of each query head of a request that was split, joined in their order.  D / 4 lanes,
+// The parts of each query head of a request that was split, joined in their order (3 us for 8
+// parts of 32 rows, 7 for the 19 MB of 1900 queries' parts).  D / 4 lanes,
 // or the next power of two, a row.
 template <int DT>
 __global__ __launch_bounds__(256) void join_kernel(kvmi_attention_args a, AttendPlan plan, int lanes_log2) {
@@ -437,13 +444,16 @@ Choice choose(const kvmi_attention_args& a) {
   // Keys are split until there are workgroups for the chip, one a CU for few rows (a workgroup
   // then keeps 4 waves' loads in flight) and two for tiles, but not below the part at which the
   // join costs more than it saves: 64 keys of few rows (512 keys of one token: 7.5 us in 8 parts,
-  // 8.3 in 4, 8.8 in 16, 9.6 whole), 256 of tiles.  Few rows are split at 1024 keys in any case,
-  // against requests of unequal lengths (64 of 1 to 12 Ki: 320 us; 330 at 512, 328 at 4096).
+  // 8.3 in 4, 8.8 in 16, 9.6 whole), 256 of tiles.  Few rows are split at 704 keys in any case,
+  // against requests of unequal lengths and a last round of workgroups that leaves the chip half
+  // empty (us at 512 / 704 / 1024 / 1536 keys: 64 requests of 1 to 12 Ki 333 / 325 / 325 / 329, 64 of
+  // 1 to 8 Ki and 64 channels 128 / 127 / 140 / 132, 32 of 256 channels 123 / 119 / 135 / 108, 256 of
+  // up to 3 Ki 357 / 340 / 333 / 350).
   const bool even = (int64_t)a.requests * c.plan.row_tiles <= tiles;  // all have the most queries
   const int64_t room = c.rows ? 256 : 512, want = std::max<int64_t>(1, (room + (even ? 0 : groups - 1)) / groups);
   c.plan.chunk = (int)std::max<int64_t>((length + want - 1) / want, c.rows ? 64 : 256);
   if (c.rows) {
-    c.plan.chunk = std::min(c.plan.chunk, 1024);
+    c.plan.chunk = std::min(c.plan.chunk, 704);
     c.plan.waves = std::min(4, (c.plan.chunk + kStep - 1) / kStep);
   }
   int64_t splits = std::min<int64_t>((length + c.plan.chunk - 1) / c.plan.chunk, 64);
@@ -456,11 +466,10 @@ Choice choose(const kvmi_attention_args& a) {
 
 template <int DT>
 void launch_rows(const kvmi_attention_args& a, const Choice& c, hipStream_t st) {
-  const int D = a.cache.head_dim, G = a.query_heads / a.cache.num_heads;
-  const int rows = std::min(16 * c.row_groups, a.max_query * G);
+  const int D = a.cache.head_dim;
   const dim3 grid((unsigned)a.cache.num_heads, (unsigned)c.plan.splits, (unsigned)a.requests);
   const dim3 threads((unsigned)(64 * c.plan.waves));
-  const size_t lds = (size_t)c.plan.waves * rows * (D + 4) * 4;
+  const size_t lds = (size_t)c.plan.waves * 16 * (D + 4) * 4;
 #define KVMI_ROWS(N8, N4, R) \
   hipLaunchKernelGGL((attend_rows_kernel<DT, N8, N4, R>), grid, threads, lds, st, a, c.plan)
   if (D > 192)
