@@ -316,7 +316,7 @@ __global__ __launch_bounds__((N8 == 2 ? 256 : 512), (N8 == 2 ? 1 : 2)) void atte
       f32x4 v = {0, 0, 0, 0};
       for (int w = 0; w < waves; ++w) {
         const float2 s = stat[w][m];
-        total += s.x == -INFINITY ? 0.0f : s.y * __builtin_amdgcn_exp2f(s.x - most);
+        total += s.y == 0 ? 0.0f : s.y * __builtin_amdgcn_exp2f(s.x - most);  // (0: saw nothing)
         v += *(const f32x4*)(sums + (w * 16 + at) * DP + d);
       }
       const int i = plan.group(m);
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(256) void join_kernel(kvmi_attention_args a, Attend
         const int at = min(s0 + s, parts - 1);
         st[s] = stats[at];
         x[s] = *(const KVMI_GLOBAL f32x4*)(sums + (int64_t)at * D);
-        if (s0 + s >= parts) st[s].x = -INFINITY;
+        if (s0 + s >= parts) st[s] = make_float2(-INFINITY, 0);
       }
       float most = top;
 #pragma unroll
@@ -373,7 +373,7 @@ __global__ __launch_bounds__(256) void join_kernel(kvmi_attention_args a, Attend
       top = most;
 #pragma unroll
       for (int s = 0; s < kAtOnce; ++s)
-        if (st[s].x != -INFINITY) {
+        if (st[s].y != 0) {  // 0: saw nothing; a part of NaN scores has a NaN sum and no maximum
           const float g = __builtin_amdgcn_exp2f(st[s].x - top);
           total += st[s].y * g;
           v += x[s] * g;
