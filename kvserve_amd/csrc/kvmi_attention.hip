@@ -69,6 +69,9 @@ __global__ __launch_bounds__((N8 == 2 ? 256 : 512), (N8 == 2 ? 1 : 2)) void atte
     }
   }
   if constexpr (kShared) __syncthreads();
+  // A panel's last two chunks may lie behind the head's channels: there the keys' loads repeat the
+  // first 8, and are left out of the product, since an infinity times the query's zero is NaN.
+  auto key = [&](int k, u32x4v v) -> u32x4v { return k < KS - 2 || 32 * k + 8 * g < D ? v : u32x4v{0, 0, 0, 0}; };
   auto query = [&](int x, int k, int at) -> u32x4v {  // `at`: the lane's column, taken anew
     if constexpr (kShared)
       return *(const u32x4v*)(shared_q + ((16 * x + at) * kRowChunks + ((4 * k + g) ^ at)) * 16);
@@ -145,7 +148,7 @@ __global__ __launch_bounds__((N8 == 2 ? 256 : 512), (N8 == 2 ? 1 : 2)) void atte
       for (int k = 0; k < KS; ++k) {
         const u32x4v v = query(x, k, at);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) s[x][b] = mma16<DT>(kf[b][k], v, s[x][b]);
+        for (int b = 0; b < 2; ++b) s[x][b] = mma16<DT>(key(k, kf[b][k]), v, s[x][b]);
       }
     }
     __builtin_amdgcn_wave_barrier();

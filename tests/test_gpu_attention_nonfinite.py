@@ -50,3 +50,22 @@ def test_keys_of_nan_give_nan_to_all_who_see_them(cuda, t, G, first):
             assert torch.isfinite(out[:t, G:]).all() and torch.isfinite(lse).sum() == lse.numel() - t * G
         assert torch.equal(call(d, max_length=3000)[t:], clean[t:])
         d["cache"].copy_(held)
+
+
+@pytest.mark.parametrize("D", [8, 24, 40, 56, 72, 80, 96, 104, 120, 128, 136, 160, 200, 224, 248, 256])
+@pytest.mark.parametrize("t,G", [(1, 4), (5, 3), (40, 4)])
+def test_a_score_of_minus_infinity_weighs_nothing(cuda, D, t, G):
+    """A key with an infinity whose scores are all -inf: as if it were not there, at every head size."""
+    for first in (0, D - 1):
+        d = make(cuda, [(700, t), (90, t)], 2, G, D, 16, seed=D + t)
+        d["query"][..., first] = -d["query"][..., first].abs() - 0.5
+        cache, tables = d["cache"], d["tables"].long()
+        for p in (0, 130, 699 - t):
+            cache[0, tables[0, p // 16], p % 16, :, first] = math.inf
+        out, lse = call(d, return_lse=True)
+        assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+        # the definition drops the keys; a key far on the other side of every query comes near it
+        cache[0, tables[0, 0], 0, :, first] = 1e30
+        for p in (130, 699 - t):
+            cache[0, tables[0, p // 16], p % 16, :, first] = 1e30
+        assert torch.equal(call(d), out)
