@@ -318,7 +318,8 @@ __global__ __launch_bounds__(kThreads) void keep_kernel(KeepArgs a) {
   // draft i of the path, `before` the one ahead of it: where it lies and where it goes
   auto place = [&](int i, int draft, int before, int64_t* from_row, int64_t* to_row) {
     const int64_t from = base + draft, to = base + i;
-    if ((i && draft <= before) || from >= top) {
+    // (draft < i: the path does not increase, and `to` may lie behind the table's row)
+    if ((i && draft <= before) || draft < i || from >= top) {
       bad |= KVMI_ERR_LENGTH;
       return;
     }
