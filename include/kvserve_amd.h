@@ -63,7 +63,7 @@ typedef struct ihipStream_t* kvmi_stream_t;
 #define KVMI_ERR_BLOCK_ID 16    /* a block id outside its pool (kvmi_check_block_ids) */
 #define KVMI_ERR_SCHEDULE 32    /* a job has more blocks than its one-pass schedule */
 #define KVMI_ERR_NO_BLOCKS 64   /* kvmi_build_tables: a request was refused, too few free blocks */
-#define KVMI_ERR_LENGTH 128     /* a length, slot range, query range or path outside its bounds */
+#define KVMI_ERR_LENGTH 128     /* a length, slot range, query range, path or free ring outside its bounds */
 
 /* Host-visible return codes. */
 #define KVMI_OK 0
@@ -487,7 +487,9 @@ int kvmi_rt_hadamard(const void* in, void* out, int64_t rows, int32_t head_dim, 
  *   lengths, new_lengths  int32 [R] tokens before / after
  *   tables                int32 [R][columns], a request's blocks in order
  *   free_blocks           int32 [ring] ring of free block ids: `state` = {head, count}; blocks are
- *                         taken at the head and returned behind the last
+ *                         taken at the head and returned behind the last, so the ring needs room
+ *                         for every block that is free or held.  Blocks returned past its room are
+ *                         dropped, and they, or a count outside [0, ring], set KVMI_ERR_LENGTH
  * Requests are served in order: one that grows is granted iff the blocks asked for by it and
  * all before it fit the count (else KVMI_ERR_NO_BLOCKS: it keeps its length and blocks, and its
  * new tokens get slot -1).  Blocks returned by this call are free for the next one.  A length

@@ -46,20 +46,20 @@ __device__ __forceinline__ Need need_of(const kvmi_tables_args& a, const BlockOf
 __device__ __forceinline__ Need need_of(const kvmi_tables_args& a, const BlockOf& div, int r) {
   return need_of(a, div, a.lengths[r], a.new_lengths[r]);
 }
-// Place of the i-th entry behind `base` (< N) in a ring of N; past 2 N only where the free count
-// and the blocks given back exceed the ring.
+// Place of the i-th entry behind `base` in a ring of N (base < N, i <= N).
 __device__ __forceinline__ uint32_t ring_at(uint32_t base, uint32_t i, uint32_t N) {
-  uint32_t x = base + i;
-  if (x >= N) x -= N;
-  return x < N ? x : x % N;
+  const uint32_t x = base + i;
+  return x < N ? x : x - N;
 }
 
 // Workgroup (r, y) makes part y of request r's table row and slots.  No workgroup waits for
 // another: each adds up what the requests before its own ask for and give back (R lengths out
 // of the L2, a few microseconds less than a scan kernel and a second launch would take), and
 // from those sums it knows its place in the ring, so that a slot needs no table entry that
-// another workgroup writes.  A ring holds every block of the pool, so the places behind the
-// last free block never reach the head's: blocks returned here are not read here.
+// another workgroup writes.  A ring has room for every block of the pool, so the places behind
+// the last free block never reach the head's: blocks returned here are not read here.  In a ring
+// that has no such room, blocks past its free places are dropped and reported, not written over
+// the free ones that other workgroups read.
 // 1024 requests of all sorts, rows of 1024, 420 Ki new tokens: 9.4 us (1.8 by its 8.8 MB: bound by
 // instructions and the chain lengths, ring, stores); 256 that grow by 8 tokens: 4.5.
 __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a, BlockOf div) {
@@ -70,7 +70,7 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a, Bl
   const Need n = need_of(a, div, r);
   const int N = a.ring;
   const int head = (int)((uint32_t)a.state[0] % (uint32_t)N);
-  const int count = a.state[1] < 0 ? 0 : a.state[1] > N ? N : a.state[1];
+  const int given = a.state[1], count = given < 0 ? 0 : given > N ? N : given;
 
   // What the requests before this one take, give back and grow by.  Blocks add up to less than
   // the table's entries, 2^31; tokens stay at 2^32 - 1, past any slot map.
@@ -120,6 +120,7 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a, Bl
   // where this request takes blocks (looked at only where it fits: take <= N) and gives them back
   const uint32_t from = ring_at(head, fits ? (uint32_t)take : 0, N);
   const uint32_t to = (uint32_t)((uint64_t)(head + (int64_t)count + give) % (uint32_t)N);
+  const int back = keep + (int)max((int64_t)0, min((int64_t)n.have - keep, N - count - give));  // keep .. back - 1
 
   // the table row: blocks kept, blocks taken, and -1 behind them; the blocks given back go
   // behind the last free one
@@ -144,11 +145,11 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a, Bl
       }
       gst((uint4*)(out + k), v);
     }
-    for (int k = keep + lane; k < n.have; k += step) gst(a.free_blocks + ring_at(to, k - keep, N), gld(old + k));
+    for (int k = keep + lane; k < back; k += step) gst(a.free_blocks + ring_at(to, k - keep, N), gld(old + k));
   } else {
     for (int k = lo + lane; k < hi; k += step) {
-      const int32_t had = k >= keep && k < n.have ? gld(old + k) : -1;
-      if (k >= keep && k < n.have) gst(a.free_blocks + ring_at(to, k - keep, N), had);
+      const int32_t had = k >= keep && k < back ? gld(old + k) : -1;
+      if (k >= keep && k < back) gst(a.free_blocks + ring_at(to, k - keep, N), had);
       gst(out + k, entry(k));
     }
   }
@@ -230,8 +231,10 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a, Bl
     returned = block_sum(returned, lds);
   }
   if (tid == 0) {
+    const int64_t spare = N - count;
+    if (given != count || returned > spare) flag_error(a.err, KVMI_ERR_LENGTH);
     a.out_state[0] = (int)((head + taken) % N);
-    a.out_state[1] = (int)(count - taken + returned);
+    a.out_state[1] = (int)(count - taken + min(returned, spare));
     if (over) *a.ticket = 0;
   }
 }

@@ -679,7 +679,7 @@ def raise_device_error(code: int) -> None:
     if code & _lib.ERR_NO_BLOCKS:
         raise RuntimeError("too few free blocks: a request was refused")
     if code & _lib.ERR_LENGTH:  # before the block ids: a length too long reads past its blocks
-        raise ValueError("a length, token range or path is out of range")
+        raise ValueError("a length, token range, path or ring of free blocks is out of range")
     if code & _lib.ERR_SYMBOL_RANGE:
         raise RuntimeError("symbol exceeds bitpack_bits")
     if code & _lib.ERR_BAD_HEADER:

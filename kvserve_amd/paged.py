@@ -118,7 +118,8 @@ def build_block_tables(lengths: torch.Tensor, new_lengths: torch.Tensor, tables:
     `tables` int32 [R, columns] holds the present blocks, `free` int32 [blocks] a ring of the
     free ones beginning at state[0], state[1] of them.  A growing request takes blocks at the
     ring's head, a shrinking one's go behind its last (`free` is changed in place; they can be
-    taken by the next call).  Requests are served in order; one whose blocks, with those asked
+    taken by the next call); the ring needs room for every block of the pool.  Blocks given back
+    past its room are dropped, and the call raises ValueError where it checks.  Requests are served in order; one whose blocks, with those asked
     for before it, exceed the free ones is refused: it keeps its length, its tokens get slot -1,
     and the call raises RuntimeError where it checks.
 

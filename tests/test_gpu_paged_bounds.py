@@ -23,3 +23,35 @@ def test_paths_that_fall_back_stay_in_their_row(cuda, S, C, base, path):
     err = i32([0], cuda)
     got = paged.keep_drafts([cache], whole[:1], i32([base], cuda), i32([path], cuda), check=False, err=err)
     assert got.tolist() == [base] and int(err) == 128 and torch.equal(cache, before)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_a_ring_without_room_keeps_its_free_blocks(cuda, in_place):
+    """Blocks given back past the ring's room are dropped and reported, in order, and those that
+    are free stay so; a count of more blocks than the ring has is reported."""
+    S = 4
+    # (lengths, new lengths, tables, ring, state) -> (tables, ring, state)
+    cases = [
+        ([8, 4], [0, 4], [[0, 1], [2, -1]], [8, 9], [0, 2], [[-1, -1], [2, -1]], [8, 9], [0, 2]),
+        ([8, 8], [4, 0], [[0, 1], [2, 3]], [-1, -1, 7], [2, 1], [[0, -1], [-1, -1]], [1, 2, 7], [2, 3]),
+        ([8, 0, 4], [0, 5, 0], [[0, 1], [-1, -1], [2, -1]], [6, 7, 8, -1], [0, 3], [[-1, -1], [6, 7], [-1, -1]],
+         [6, 7, 8, 0], [2, 2]),
+        ([4], [8], [[0, -1]], [5, 6], [1, 3], [[0, 6]], [5, 6], [0, 1]),
+    ]
+    for now, new, tables, ring, state, want_tables, want_ring, want_state in cases:
+        for check in (False, True):
+            t = [i32(v, cuda) for v in (now, new, tables, ring, state)]
+            kw = {}
+            if in_place:
+                slots, starts = torch.empty(9, dtype=torch.int64, device=cuda), i32([0] * (len(now) + 1), cuda)
+                kw = dict(out=(t[2], t[0], t[4], slots, starts), ticket=i32([0], cuda))
+            err = i32([0], cuda)
+            args = (t[0], t[1], t[2], t[3], t[4], S, 9)
+            if check:
+                with pytest.raises(ValueError, match="ring of free blocks"):
+                    paged.build_block_tables(*args, check=True, **kw)
+                continue
+            got = paged.build_block_tables(*args, check=False, err=err, **kw)
+            assert int(err) == 128
+            assert got.tables.tolist() == want_tables and got.lengths.tolist() == new
+            assert t[3].tolist() == want_ring and got.state.tolist() == want_state
