@@ -502,7 +502,8 @@ int kvmi_rt_hadamard(const void* in, void* out, int64_t rows, int32_t head_dim, 
  *                         requests in order; -1 behind the last.  More tokens than that set
  *                         KVMI_ERR_LENGTH
  *   starts                int32 [R + 1]: where each request's new tokens begin in `slots`
- * `err` may be null here and in the entry points below.
+ * `err` may be null here and in the entry points below; in all of them a row of a table holds at
+ * most 2^31 - 2^20 tokens (columns * block_size).
  */
 typedef struct kvmi_tables_args {
   const int32_t* lengths;

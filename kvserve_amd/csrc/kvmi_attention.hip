@@ -400,8 +400,8 @@ bool attention_ok(const kvmi_attention_args* a) {
       a->max_length < 0 || a->query_heads < 1 || a->query_heads % c.num_heads ||
       (a->dtype != KVMI_DTYPE_BF16 && a->dtype != KVMI_DTYPE_FP16) || !(a->scale > 0) || a->scale > 3.0e38f)
     return false;
-  if ((int64_t)a->columns * c.block_size > 0x7fffffffLL || (int64_t)c.num_blocks * c.block_size > 0x7fffffffLL ||
-      (int64_t)a->max_query * a->query_heads > 0x7fffffffLL ||
+  if ((int64_t)a->columns * c.block_size > kMostPlaces || (int64_t)c.num_blocks * c.block_size > 0x7fffffffLL ||
+      (int64_t)a->max_query * a->query_heads > kMostPlaces ||
       (int64_t)c.block_size * c.num_heads * c.head_dim > 0x7fffffffLL)
     return false;
   if (a->mask && a->mask_words < 1) return false;

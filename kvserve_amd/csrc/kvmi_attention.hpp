@@ -48,7 +48,7 @@ __device__ __forceinline__ Request request_of(const kvmi_attention_args& a, int 
 }
 // Parts that a request of so many tokens has.
 __device__ __forceinline__ int parts_of(const AttendPlan& p, int length) {
-  return min(p.splits, max(1, (length + p.chunk - 1) / p.chunk));
+  return min(p.splits, max(1, (int)(((uint32_t)length + (uint32_t)p.chunk - 1) / (uint32_t)p.chunk)));
 }
 
 // Where part `part` of `parts` of n tiles begins (n < 2^26, 64 parts at most).

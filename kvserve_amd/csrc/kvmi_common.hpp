@@ -32,6 +32,10 @@ inline BlockOf block_of(int block_size) {
   return BlockOf{(uint32_t)(((1ULL << (31 + l)) + block_size - 1) / block_size), 31 + l};
 }
 
+// The most tokens of a request's blocks, and rows of a request's queries: counters in 31 bits go up
+// to a workgroup's or a grid's step past the last one.
+constexpr int64_t kMostPlaces = 0x7fffffffLL - (1 << 20);
+
 // Quantization axis of a part (0 = K, 1 = V): the default is K per channel and V per
 // token; the KVMI_F_* axis flags select the others.
 enum Axis { kAxChannel = 0, kAxToken = 1, kAxTensor = 2 };

@@ -397,7 +397,7 @@ extern "C" int kvmi_build_tables(const kvmi_tables_args* args, kvmi_stream_t str
   if (!args) return KVMI_EINVAL;
   const kvmi_tables_args& a = *args;
   if (a.requests < 0 || a.columns < 1 || a.ring < 1 || a.block_size < 1 || a.max_tokens < 0) return KVMI_EINVAL;
-  if ((int64_t)a.columns * a.block_size > 0x7fffffffLL || (int64_t)a.ring * a.block_size > 0x7fffffffLL ||
+  if ((int64_t)a.columns * a.block_size > kMostPlaces || (int64_t)a.ring * a.block_size > 0x7fffffffLL ||
       (int64_t)a.columns * a.requests > 0x7fffffffLL)
     return KVMI_EINVAL;
   if (a.requests == 0) return KVMI_OK;
@@ -454,7 +454,7 @@ extern "C" int kvmi_keep_drafts(const kvmi_cache* cache, void* const* bases, int
                                 int32_t width, int32_t* out_lengths, int32_t* err, kvmi_stream_t stream) {
   using namespace kvmi;
   if (!cache_ok(cache, false) || layers < 1 || layers > 65535 || columns < 1 || requests < 0 || width < 0 ||
-      width > kMaxPath || (int64_t)columns * cache->block_size > 0x7fffffffLL)
+      width > kMaxPath || (int64_t)columns * cache->block_size > kMostPlaces)
     return KVMI_EINVAL;
   if (requests == 0) return KVMI_OK;
   if (!bases || !tables || !lengths || !out_lengths || (width && !accepted) || lengths == out_lengths)

@@ -1,0 +1,42 @@
+"""Sizes at the end of 31 bits, refused on the host (nothing is launched)."""
+
+import pytest
+
+from kvserve_amd import _lib
+
+from test_paged_host import SOME, attention_args, cache_struct
+
+MOST = 2**31 - 2**20 - 1  # tokens of a table's row, rows of a request's queries
+
+
+def one_token_blocks():
+    return cache_struct(block_size=1, block_stride=2 * 64, part_stride=4 * 2 * 64)
+
+
+def test_attention_refuses_places_that_its_counters_would_pass():
+    lib = _lib.load()
+    size = lambda **kw: lib.kvmi_attention_workspace_bytes(attention_args(one_token_blocks(), **kw))
+    assert size(columns=MOST) >= 0
+    assert size(columns=MOST + 1) == size(columns=2**31 - 1) == _lib.EINVAL
+    assert lib.kvmi_tree_attention(attention_args(one_token_blocks(), columns=2**31 - 1), None) == _lib.EINVAL
+    rows = lambda n: size(max_query=n, query_heads=2, total_queries=n)
+    assert rows(MOST // 2) >= 0
+    assert rows(MOST // 2 + 1) == rows(2**30 - 1) == _lib.EINVAL
+
+
+def test_any_longest_length_is_taken():
+    lib = _lib.load()
+    for n in (0, 1, 64, 10**6, 2**31 - 1):
+        assert lib.kvmi_attention_workspace_bytes(attention_args(max_length=n)) >= 0
+
+
+@pytest.mark.parametrize("columns,fine", [(MOST, True), (MOST + 1, False), (2**31 - 1, False)])
+def test_tables_and_kept_drafts_refuse_longer_rows(columns, fine):
+    lib = _lib.load()
+    want = _lib.OK if fine else _lib.EINVAL
+    names = [f for f, _ in _lib.TablesArgs._fields_]
+    a = {n: 4096 * (i + 1) for i, n in enumerate(names[:12])}
+    a.update(err=None, requests=0, columns=columns, ring=8, block_size=1, max_tokens=10, reserved=0)
+    assert lib.kvmi_build_tables(_lib.TablesArgs(*(a[n] for n in names)), None) == want
+    c = one_token_blocks()
+    assert lib.kvmi_keep_drafts(c, SOME, 1, SOME, columns, SOME, SOME, 0, 3, SOME, None, None) == want
