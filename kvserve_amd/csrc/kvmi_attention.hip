@@ -22,7 +22,8 @@ constexpr int kStep = 32;  // keys a wave takes at a time
 // N8 / N4: panels of 128 / 64 channels.  Past 128 channels, or 16 rows, the queries stay in LDS and
 // are read again for every 32 keys: with them in registers a wave would not fit its 256.  Past 192
 // it does not fit them either way, and has a SIMD's 512 to itself.
-template <int DT, int N8, int N4, int R>
+// WHOLE: D is all of the panels' channels.
+template <int DT, int N8, int N4, int R, bool WHOLE>
 __global__ __launch_bounds__((N8 == 2 ? 256 : 512), (N8 == 2 ? 1 : 2)) void attend_rows_kernel(kvmi_attention_args a,
                                                                                              AttendPlan plan) {
   constexpr bool kShared = (N8 + N4 > 1 || R > 1) && N8 < 2;
@@ -71,7 +72,10 @@ __global__ __launch_bounds__((N8 == 2 ? 256 : 512), (N8 == 2 ? 1 : 2)) void atte
   if constexpr (kShared) __syncthreads();
   // A panel's last two chunks may lie behind the head's channels: there the keys' loads repeat the
   // first 8, and are left out of the product, since an infinity times the query's zero is NaN.
-  auto key = [&](int k, u32x4v v) -> u32x4v { return k < KS - 2 || 32 * k + 8 * g < D ? v : u32x4v{0, 0, 0, 0}; };
+  // (4 us of 121 at 256 channels, one wave a SIMD, so that whole heads have kernels of their own)
+  auto key = [&](int k, u32x4v v) -> u32x4v {
+    return WHOLE || k < KS - 2 || 32 * k + 8 * g < D ? v : u32x4v{0, 0, 0, 0};
+  };
   auto query = [&](int x, int k, int at) -> u32x4v {  // `at`: the lane's column, taken anew
     if constexpr (kShared)
       return *(const u32x4v*)(shared_q + ((16 * x + at) * kRowChunks + ((4 * k + g) ^ at)) * 16);
@@ -473,8 +477,13 @@ void launch_rows(const kvmi_attention_args& a, const Choice& c, hipStream_t st) 
   const dim3 grid((unsigned)a.cache.num_heads, (unsigned)c.plan.splits, (unsigned)a.requests);
   const dim3 threads((unsigned)(64 * c.plan.waves));
   const size_t lds = (size_t)c.plan.waves * 16 * (D + 4) * 4;
-#define KVMI_ROWS(N8, N4, R) \
-  hipLaunchKernelGGL((attend_rows_kernel<DT, N8, N4, R>), grid, threads, lds, st, a, c.plan)
+#define KVMI_ROWS(N8, N4, R)                                                                       \
+  do {                                                                                             \
+    if (D == 128 * N8 + 64 * N4)                                                                   \
+      hipLaunchKernelGGL((attend_rows_kernel<DT, N8, N4, R, true>), grid, threads, lds, st, a, c.plan);  \
+    else                                                                                           \
+      hipLaunchKernelGGL((attend_rows_kernel<DT, N8, N4, R, false>), grid, threads, lds, st, a, c.plan); \
+  } while (0)
   if (D > 192)
     KVMI_ROWS(2, 0, 1);
   else if (D > 128)
