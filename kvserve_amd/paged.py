@@ -36,6 +36,7 @@ from .ops import _check_default
 # not take comes back, to the checks and errors here.
 _calls = _lib.calls()
 
+_INT32_MAX = 2**31 - 1  # sizes are 32-bit words in the library's structs
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 
 
@@ -64,6 +65,8 @@ def _cache_struct(cache: torch.Tensor) -> _lib.Cache:
         raise TypeError("the KV cache must be a 16-bit tensor")
     if cache.dim() != 5 or 2 not in cache.shape[:2]:
         raise ValueError(f"Unsupported KV layout shape: {tuple(cache.shape)}")
+    if max(cache.shape) > _INT32_MAX:
+        raise ValueError(f"the KV cache's sizes must be in 31 bits, not {tuple(cache.shape)}")
     if not cache.is_cuda or not cache.is_contiguous() or not cache.numel():
         raise ValueError("the KV cache must be a contiguous, non-empty CUDA tensor")
     S, H, D = cache.shape[2:]
@@ -131,8 +134,9 @@ def build_block_tables(lengths: torch.Tensor, new_lengths: torch.Tensor, tables:
     if type(out) is TablesUpdate and _unchecked(check) and _calls.build_block_tables(
             lengths, new_lengths, tables, free, state, block_size, max_tokens, out, ticket, err):
         return out
-    if type(block_size) is not int or block_size < 1 or type(max_tokens) is not int or max_tokens < 0:
-        raise ValueError("block_size must be a positive integer and max_tokens a nonnegative one")
+    if type(block_size) is not int or not 1 <= block_size <= _INT32_MAX or type(max_tokens) is not int \
+            or not 0 <= max_tokens <= _INT32_MAX:
+        raise ValueError("block_size must be a positive integer and max_tokens a nonnegative one, in 31 bits")
     now = _tensor(lengths, "lengths", torch.int32, (None,))
     dev, R = lengths.device, lengths.numel()
     new = _tensor(new_lengths, "new_lengths", torch.int32, (R,), dev)
@@ -186,8 +190,8 @@ class BlockTables:
                  free_blocks: Optional[Iterable[int]] = None):
         for name, v in (("num_blocks", num_blocks), ("block_size", block_size), ("requests", requests),
                         ("columns", columns)):
-            if type(v) is not int or v < 1:
-                raise ValueError(f"{name} must be a positive integer")
+            if type(v) is not int or not 1 <= v <= _INT32_MAX:
+                raise ValueError(f"{name} must be a positive integer in 31 bits")
         ids = list(range(num_blocks)) if free_blocks is None else [int(b) for b in free_blocks]
         if len(set(ids)) != len(ids) or (ids and (min(ids) < 0 or max(ids) >= num_blocks)):
             raise ValueError("free_blocks must be distinct block ids of the cache")
@@ -283,6 +287,8 @@ def _attention_args(query, cache, tables, lengths, starts, max_query, max_length
             _tensor(starts, "starts", torch.int32, (R + 1,), dev))
     if max_length is None:
         max_length = tables.shape[1] * c.block_size
+    if type(max_length) is int:
+        max_length = min(max_length, _INT32_MAX)
     for name, v in (("max_query", max_query), ("max_length", max_length)):
         if type(v) is not int or v < 0:
             raise ValueError(f"{name} must be a nonnegative integer")

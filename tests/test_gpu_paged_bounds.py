@@ -1,12 +1,15 @@
 """The paged operators on arguments that are wrong in the middle: nothing outside the arrays they
 were given is read or written."""
 
+import sys
+
 import pytest
 import torch
 
 from kvserve_amd import paged
 
 from test_gpu_paged import i32
+from test_gpu_tree_attention import call, hold, make
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +58,13 @@ def test_a_ring_without_room_keeps_its_free_blocks(cuda, in_place):
             assert int(err) == 128
             assert got.tables.tolist() == want_tables and got.lengths.tolist() == new
             assert t[3].tolist() == want_ring and got.state.tolist() == want_state
+
+
+@pytest.mark.parametrize("check", [True, False])
+def test_any_longest_length_is_taken(cuda, check):
+    """`max_length` shapes the launch alone, whatever its size."""
+    d = make(cuda, [(900, 2), (70, 1)], 2, 4, 64, 16, seed=1)
+    want = call(d, max_length=2**31 - 1, check=check)
+    hold(d, want)
+    for n in (2**31, 2**32, 2**32 + 7, sys.maxsize):
+        assert torch.equal(call(d, max_length=n, check=check), want)

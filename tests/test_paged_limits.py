@@ -1,8 +1,9 @@
-"""Sizes at the end of 31 bits, refused on the host (nothing is launched)."""
+"""Sizes at the end of 31 bits and past it, refused on the host (nothing is launched)."""
 
 import pytest
+import torch
 
-from kvserve_amd import _lib
+from kvserve_amd import _lib, paged
 
 from test_paged_host import SOME, attention_args, cache_struct
 
@@ -40,3 +41,17 @@ def test_tables_and_kept_drafts_refuse_longer_rows(columns, fine):
     assert lib.kvmi_build_tables(_lib.TablesArgs(*(a[n] for n in names)), None) == want
     c = one_token_blocks()
     assert lib.kvmi_keep_drafts(c, SOME, 1, SOME, columns, SOME, SOME, 0, 3, SOME, None, None) == want
+
+
+def test_sizes_past_31_bits_are_not_cut():
+    """Python's integers are refused where the structs' words would keep their low bits only."""
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)
+    build = lambda S, n: paged.build_block_tables(i32(1), i32(1), i32(1, 2), i32(4), i32(2), S, n)
+    for S, n in ((2**32 + 16, 5), (2**31, 5), (16, 2**32 + 5), (16, 2**31)):
+        with pytest.raises(ValueError, match="block_size .* max_tokens"):
+            build(S, n)
+    with pytest.raises(ValueError, match="block_size"):
+        paged.BlockTables(4, 2**32 + 16, 2, 3, device="cpu")
+    cache = torch.empty((2, 1, 2**31, 1, 1), dtype=torch.bfloat16, device="meta")
+    with pytest.raises(ValueError, match="31 bits"):
+        paged._cache_struct(cache)
