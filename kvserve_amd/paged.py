@@ -363,8 +363,8 @@ def tree_attention(query: torch.Tensor, cache: torch.Tensor, tables: torch.Tenso
 
 # ------------------------------------------------------------------ kept drafts
 class LayerCaches:
-    """The caches of a model's layers (same type, shape and device), with their addresses on the
-    GPU: made once, for `keep_drafts`."""
+    """The caches of a model's layers (same type, shape and device, each a memory of its own: layers
+    that share one are given once), with their addresses on the GPU: made once, for `keep_drafts`."""
 
     def __init__(self, caches: Sequence[torch.Tensor]):
         self.caches = list(caches)
@@ -377,6 +377,10 @@ class LayerCaches:
             if c.shape != first.shape or c.dtype != first.dtype or c.device != first.device:
                 raise ValueError("the layers' caches must have one type, shape and device")
         bases = [c.data_ptr() for c in self.caches]
+        # two layers in one memory would move the same rows twice, each in the other's way
+        ordered, size = sorted(bases), first.numel() * first.element_size()
+        if any(b - a < size for a, b in zip(ordered, ordered[1:])):
+            raise ValueError("the layers' caches must not share memory")
         either = 0
         for b in bases:
             either |= b

@@ -68,3 +68,16 @@ def test_any_longest_length_is_taken(cuda, check):
     hold(d, want)
     for n in (2**31, 2**32, 2**32 + 7, sys.maxsize):
         assert torch.equal(call(d, max_length=n, check=check), want)
+
+
+def test_layers_in_one_memory_are_refused(cuda):
+    """Rows that two layers' workgroups would both move."""
+    one = torch.zeros((2, 6, 4, 1, 8), dtype=torch.bfloat16, device=cuda)
+    both = torch.zeros((3, 2, 6, 4, 1, 8), dtype=torch.bfloat16, device=cuda)
+    overlapping = both.flatten()[both[0].numel() // 2:][:both[0].numel()].view_as(both[0])
+    for caches in ([one, one], [both[0], one, both[0]], [both[0], overlapping], [both[1], both[2], overlapping]):
+        with pytest.raises(ValueError, match="share"):
+            paged.LayerCaches(caches)
+        with pytest.raises(ValueError, match="share"):
+            paged.keep_drafts(caches, i32([[0, 1]], cuda), i32([0], cuda), i32([[0]], cuda))
+    assert paged.LayerCaches([both[2], both[0], both[1]]).bases.tolist() == [c.data_ptr() for c in (both[2], both[0], both[1])]
