@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+import warnings
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libkvserve_amd.so"
@@ -243,10 +244,20 @@ class _NoCalls:
 
     def __init__(self, why: Exception):
         self._why = why
+        self._told = False
+
+    def _what(self) -> str:
+        return (f"kvserve_amd/_calls.so cannot be loaded ({self._why}): build it with "
+                "`python -m kvserve_amd.build`")
+
+    def tell(self) -> None:
+        """Warn, once, that calls go the slower way."""
+        if not self._told:
+            self._told = True
+            warnings.warn(self._what() + "; unchecked calls take longer on the host until then", stacklevel=4)
 
     def __getattr__(self, name):
-        raise KvmiError(f"kvserve_amd/_calls.so cannot be loaded ({self._why}): build it with "
-                        "`python -m kvserve_amd.build`")
+        raise KvmiError(self._what())
 
 
 def calls():

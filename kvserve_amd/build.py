@@ -15,6 +15,8 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
+import warnings
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -57,17 +59,33 @@ def _compile(src: Path, defines=()) -> Path:
 
 
 def _build_calls() -> None:
-    """The Python module over the library: the paged operators' unchecked calls."""
-    import sysconfig
-
-    import torch
-
-    root = Path(torch.__file__).resolve().parent
+    """The Python module over the library: the paged operators' unchecked calls.  Where g++ or
+    Python's or torch's headers are missing it is left out, with a warning, and an old one is
+    removed: the library is whole without it, and the calls go the slower way through Python."""
+    missing = None
+    include = Path(sysconfig.get_paths()["include"])
+    try:
+        import torch
+        root = Path(torch.__file__).resolve().parent
+    except ImportError:
+        missing = "torch"
+    else:
+        if not (root / "include" / "torch" / "csrc" / "autograd" / "python_variable.h").exists():
+            missing = "torch's headers"
+    if not (include / "Python.h").exists():
+        missing = "Python's headers"
+    if shutil.which("g++") is None:
+        missing = "g++"
+    if missing:
+        CALLS.unlink(missing_ok=True)
+        warnings.warn(f"{CALLS.name} is not built, {missing} not found: the paged operators' unchecked calls "
+                      "take longer on the host", stacklevel=2)
+        return
     rocm = Path(hipcc()).resolve().parents[1]
     tmp = CALLS.with_suffix(".so.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{root}/include",
-           f"-I{root}/include/torch/csrc/api/include", f"-I{rocm}/include", f"-I{sysconfig.get_paths()['include']}",
+           f"-I{root}/include/torch/csrc/api/include", f"-I{rocm}/include", f"-I{include}",
            f"-I{INCLUDE}", str(CSRC / "kvmi_calls.cpp"), "-o", str(tmp), f"-L{PKG}", f"-l:{LIB.name}",
            "-Wl,-rpath,$ORIGIN", f"-L{root}/lib", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
            f"-L{rocm}/lib", "-lamdhip64"]
@@ -97,7 +115,7 @@ def build(verbose: bool = False, defines=()) -> Path:
     os.replace(tmp, LIB)
     _build_calls()
     if verbose:
-        print(f"built {LIB} and {CALLS.name}")
+        print(f"built {LIB}" + (f" and {CALLS.name}" if CALLS.exists() else ""))
     return LIB
 
 

@@ -33,7 +33,8 @@ from .engine import raise_device_error
 from .ops import _check_default
 
 # A call that is not checked goes through this module at once (4 us instead of 13); what it does
-# not take comes back, to the checks and errors here.
+# not take comes back, to the checks and errors here, and so does everything where the module is
+# not built.
 _calls = _lib.calls()
 
 _INT32_MAX = 2**31 - 1  # sizes are 32-bit words in the library's structs
@@ -42,7 +43,13 @@ _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 
 # ------------------------------------------------------------------ shared checks
 def _unchecked(check: Optional[bool]) -> bool:
-    return check is False or (check is None and not _check_default())
+    """Whether the call may go through `_calls`."""
+    if check or (check is None and _check_default()):
+        return False
+    if isinstance(_calls, _lib._NoCalls):
+        _calls.tell()
+        return False
+    return True
 
 
 def _tensor(t, name: str, dtype: torch.dtype, shape, device=None) -> int:
