@@ -588,6 +588,15 @@ typedef struct kvmi_attention_args {
 #define KVMI_DTYPE_BF16 0
 #define KVMI_DTYPE_FP16 1
 int64_t kvmi_attention_workspace_bytes(const kvmi_attention_args* args);
+/*
+ * Which kernels an attention call runs (host only): KVMI_ATTENTION_ROWS, few rows a KV head, or
+ * KVMI_ATTENTION_TILES, or KVMI_EINVAL, also where there is nothing to do.  `shape` (may be NULL)
+ * receives int32[4]: waves of a workgroup, rows it holds, the most parts that a request's keys are
+ * split into, keys of a part.
+ */
+#define KVMI_ATTENTION_ROWS 0
+#define KVMI_ATTENTION_TILES 1
+int kvmi_attention_kernels(const kvmi_attention_args* args, int32_t* shape);
 int kvmi_tree_attention(const kvmi_attention_args* args, kvmi_stream_t stream);
 
 /*

@@ -80,6 +80,7 @@ EXPORTS = (
     "kvmi_build_tables",
     "kvmi_write_kv",
     "kvmi_attention_workspace_bytes",
+    "kvmi_attention_kernels",
     "kvmi_tree_attention",
     "kvmi_keep_drafts",
 )
@@ -132,6 +133,7 @@ class RtLayer(ctypes.Structure):
 
 
 DTYPE_BF16, DTYPE_FP16 = 0, 1
+ATTENTION_ROWS, ATTENTION_TILES = 0, 1
 
 
 class TablesArgs(ctypes.Structure):
@@ -207,6 +209,7 @@ _SIGNATURES = {
     "kvmi_build_tables": ([ctypes.POINTER(TablesArgs), _vp], ctypes.c_int),
     "kvmi_write_kv": ([ctypes.POINTER(Cache), _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp], ctypes.c_int),
     "kvmi_attention_workspace_bytes": ([ctypes.POINTER(AttentionArgs)], _i64),
+    "kvmi_attention_kernels": ([ctypes.POINTER(AttentionArgs), ctypes.POINTER(_i32)], ctypes.c_int),
     "kvmi_tree_attention": ([ctypes.POINTER(AttentionArgs), _vp], ctypes.c_int),
     "kvmi_keep_drafts": ([ctypes.POINTER(Cache), _vp, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp],
                          ctypes.c_int),

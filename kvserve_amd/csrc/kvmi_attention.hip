@@ -509,6 +509,20 @@ extern "C" int64_t kvmi_attention_workspace_bytes(const kvmi_attention_args* arg
   return parts_bytes(*args, choose(*args).plan.splits);
 }
 
+extern "C" int kvmi_attention_kernels(const kvmi_attention_args* args, int32_t* shape) {
+  using namespace kvmi;
+  if (!attention_ok(args) || args->requests == 0 || args->total_queries == 0 || args->max_query == 0)
+    return KVMI_EINVAL;
+  const Choice c = choose(*args);
+  if (shape) {
+    shape[0] = c.plan.waves;
+    shape[1] = c.rows ? 16 * c.row_groups : 32 * c.plan.waves;
+    shape[2] = c.plan.splits;
+    shape[3] = c.plan.chunk;
+  }
+  return c.rows ? KVMI_ATTENTION_ROWS : KVMI_ATTENTION_TILES;
+}
+
 extern "C" int kvmi_tree_attention(const kvmi_attention_args* args, kvmi_stream_t stream) {
   using namespace kvmi;
   if (!attention_ok(args)) return KVMI_EINVAL;

@@ -1,4 +1,7 @@
-"""Sizes at the end of 31 bits and past it, refused on the host (nothing is launched)."""
+"""What the library decides on the host, where nothing is launched: sizes at the end of 31 bits and
+past it are refused, and an attention call names its kernels."""
+
+import ctypes
 
 import pytest
 import torch
@@ -55,3 +58,31 @@ def test_sizes_past_31_bits_are_not_cut():
     cache = torch.empty((2, 1, 2**31, 1, 1), dtype=torch.bfloat16, device="meta")
     with pytest.raises(ValueError, match="31 bits"):
         paged._cache_struct(cache)
+
+
+def test_attention_names_its_kernels():
+    """Few rows or tiles, waves, rows of a workgroup, parts and keys of a part, for batches that
+    are not the GPU's to decide."""
+    lib, shape = _lib.load(), (ctypes.c_int32 * 4)()
+
+    def kernels(D=128, H=8, **kw):
+        c = cache_struct(head_dim=D, num_heads=H, block_stride=16 * H * D, part_stride=4 * 16 * H * D)
+        return lib.kvmi_attention_kernels(attention_args(c, columns=4096, **kw), shape), *shape
+
+    few, tiles = _lib.ATTENTION_ROWS, _lib.ATTENTION_TILES
+    one = dict(requests=1, total_queries=1, query_heads=32, max_query=1)
+    assert kernels(**one, max_length=512) == (few, 2, 16, 8, 64)
+    batch = dict(requests=64, total_queries=64, query_heads=32, max_query=1)
+    assert kernels(**batch, max_length=12289) == (few, 4, 16, 18, 704)
+    prompt = dict(requests=1, total_queries=8192, query_heads=32, max_query=8192)
+    assert kernels(**prompt, max_length=8192) == (tiles, 8, 256, 1, 8192)
+    assert kernels(D=64, **prompt, max_length=8192) == (tiles, 4, 128, 1, 8192)
+    # 16 rows, 32, and 33; above 128 channels 16 and 17
+    for D, rows, want in ((128, 16, (few, 16)), (128, 17, (few, 32)), (128, 32, (few, 32)), (128, 33, (tiles, 128)),
+                          (136, 16, (few, 16)), (136, 17, (tiles, 128))):
+        got = kernels(D=D, requests=1, total_queries=rows, query_heads=8, max_query=rows, max_length=100)
+        assert (got[0], got[2]) == want
+    assert lib.kvmi_attention_kernels(attention_args(), None) == few
+    for kw in (dict(requests=0), dict(total_queries=0), dict(max_query=0), dict(scale=0.0)):
+        assert lib.kvmi_attention_kernels(attention_args(**kw), shape) == _lib.EINVAL
+    assert lib.kvmi_attention_kernels(None, shape) == _lib.EINVAL
