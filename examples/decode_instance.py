@@ -100,6 +100,8 @@ def main(argv=None) -> None:
     for name, value in (("requests", 8), ("layers", 4), ("steps", 6), ("prompt", 2000)):
         parser.add_argument(f"--{name}", type=int, default=value)
     args = parser.parse_args(argv)
+    if min(args.requests, args.layers, args.steps) < 1 or args.prompt < 2:
+        parser.error("at least one request, layer and step, and prompts of two tokens")
     dev, heads, dim, block, rng = torch.device("cuda", 0), 8, 128, 16, random.Random(0)
     lengths = [rng.randint(args.prompt // 2, args.prompt) for _ in range(args.requests)]
     counts = [-(-n // block) for n in lengths]
