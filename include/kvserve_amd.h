@@ -500,7 +500,8 @@ int kvmi_rt_hadamard(const void* in, void* out, int64_t rows, int32_t head_dim, 
  *                         int32 word that is zero before the first call, is used and left zero
  *   slots                 int64 [max_tokens]: block * block_size + place of every new token,
  *                         requests in order; -1 behind the last.  More tokens than that set
- *                         KVMI_ERR_LENGTH
+ *                         KVMI_ERR_LENGTH: tables, lengths and state move on all the same, and the
+ *                         slots past max_tokens are written nowhere
  *   starts                int32 [R + 1]: where each request's new tokens begin in `slots`
  * `err` may be null here and in the entry points below; in all of them a row of a table holds at
  * most 2^31 - 2^20 tokens (columns * block_size).
@@ -559,11 +560,12 @@ int kvmi_write_kv(const kvmi_cache* cache, const void* key, const void* value, i
  *               adjacent, 16-byte aligned rows), out contiguous and 16-byte aligned; query head h reads KV head
  *               h / (query_heads / num_heads)
  *   lse         fp32 [total_queries][query_heads] natural log of the sums, or null
- *   max_query   no request may have more queries (KVMI_ERR_LENGTH, the rows past it unwritten)
+ *   max_query   no request may have more queries (KVMI_ERR_LENGTH, the rows past it unwritten; a
+ *               call with 0 does nothing)
  *   max_length  the longest length, for the launch shape only (keys are split over workgroups by
  *               it): any value gives the same sums up to the order of their parts
  *   workspace   kvmi_attention_workspace_bytes of the same arguments, 16-byte aligned
- * D is a multiple of 8 up to 256.  A block id outside the cache sets KVMI_ERR_BLOCK_ID (the
+ * D is a multiple of 8 up to 256, and there are at most 65535 requests.  A block id outside the cache sets KVMI_ERR_BLOCK_ID (the
  * nearest block is read in its place), a length outside [0, columns * S] or a range outside the
  * queries KVMI_ERR_LENGTH (and is clamped).
  */

@@ -131,7 +131,9 @@ def build_block_tables(lengths: torch.Tensor, new_lengths: torch.Tensor, tables:
     taken by the next call); the ring needs room for every block of the pool.  Blocks given back
     past its room are dropped, and the call raises ValueError where it checks.  Requests are served in order; one whose blocks, with those asked
     for before it, exceed the free ones is refused: it keeps its length, its tokens get slot -1,
-    and the call raises RuntimeError where it checks.
+    and the call raises RuntimeError where it checks.  More than `max_tokens` new tokens raise
+    ValueError there; tables and lengths have then moved on, and the slots past `max_tokens` are
+    lost, so the bound has to hold.
 
     `out`: the tensors of a `TablesUpdate` to write into.  Tables may be `tables` itself;
     lengths and state may both be `lengths` and `state` themselves, with `ticket`, an int32 word
@@ -326,8 +328,8 @@ def tree_attention(query: torch.Tensor, cache: torch.Tensor, tables: torch.Tenso
     query      [tokens, query heads, D], bfloat16 or float16 as the cache; query head h reads KV
                head h // (query heads / KV heads)
     cache      [2, P, S, H, D] or [P, 2, S, H, D]; the queries' own keys and values are in it
-    tables     int32 [R, columns] block tables; lengths int32 [R] tokens in the cache, queries
-               included
+    tables     int32 [R, columns] block tables of at most 65535 requests; lengths int32 [R] tokens in
+               the cache, queries included
     starts     int32 [R + 1]: request r's queries are rows starts[r] .. starts[r + 1] - 1
     max_query  the most queries of a request; max_length the longest length (default: what the
                tables hold; a tighter bound gives better launches)
@@ -335,7 +337,10 @@ def tree_attention(query: torch.Tensor, cache: torch.Tensor, tables: torch.Tenso
                its request (`tree_mask()` makes them).  Without it the queries are a causal chain:
                one token, a chunk or a whole prompt.
     Every query sees all tokens before its request's first query.  A query that sees nothing
-    gives zeros.  Rows of no request are left as they are in `out`.
+    gives zeros.  Rows of no request are left as they are in `out`.  No gradient flows back.
+
+    The requests with the most queries choose the kernel for all: a prompt's chunk beside single
+    tokens over long contexts is much faster as a call for the chunk and one for the tokens.
 
     Returns `out`, or (out, lse) with the fp32 natural log of each row's sum [tokens, query heads].
     """

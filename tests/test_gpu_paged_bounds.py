@@ -81,3 +81,13 @@ def test_layers_in_one_memory_are_refused(cuda):
         with pytest.raises(ValueError, match="share"):
             paged.keep_drafts(caches, i32([[0, 1]], cuda), i32([0], cuda), i32([[0]], cuda))
     assert paged.LayerCaches([both[2], both[0], both[1]]).bases.tolist() == [c.data_ptr() for c in (both[2], both[0], both[1])]
+
+
+def test_more_tokens_than_slots_move_the_tables_on(cuda):
+    """A `max_tokens` that does not hold is an error, found after lengths and tables have changed."""
+    own = paged.BlockTables(6, 4, 2, 3, cuda)
+    slots = torch.full((7,), -9, dtype=torch.int64, device=cuda)
+    with pytest.raises(ValueError):
+        own.update(i32([6, 5], cuda), 7, slots=slots, check=True)
+    assert own.lengths.tolist() == [6, 5] and own.state.tolist() == [4, 2]
+    assert own.tables.tolist() == [[0, 1, -1], [2, 3, -1]] and slots.tolist() == [0, 1, 2, 3, 4, 5, 8]
