@@ -33,7 +33,7 @@ HIPCC_FLAGS = [
     "-std=c++17",
     "-fPIC",
     "-ffp-contract=off",
-    # packed-fp32 VALU ops stay disabled on this pool
+    # packed-fp32 VALU ops stay disabled: some of their forms have given wrong results now and then
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     # MFMA results in VGPRs: the accumulators feed VALU code directly, without
     # v_accvgpr_read copies out of AGPRs

@@ -15,13 +15,15 @@ constexpr int kStep = 32;  // keys a wave takes at a time
 //   O^T += V^T P^T  a lane loads 16 bytes of each of its 8 keys, 16 lanes a whole row of 128
 //                   channels; pairs of keys are brought together by byte permutes, and the
 //                   output row of tile j is channel 8 * row + j
-// so that nothing goes through LDS before the waves' sums are joined at the end.  64 requests of
-// 1 to 12 Ki tokens, 32 heads over 8, 128 channels: 322 us with the join, 5.1 TB/s, as fast as a
-// copy reads and writes; 32 rows 3.7 TB/s, 256 channels 4.2; one token over 512, a chain of loads,
-// 7.5 us.
-// N8 / N4: panels of 128 / 64 channels.  Past 128 channels, or 16 rows, the queries stay in LDS and
-// are read again for every 32 keys: with them in registers a wave would not fit its 256.  Past 192
-// it does not fit them either way, and has a SIMD's 512 to itself.
+// so that keys and values do not go through LDS and, but for the queries below, no wave waits for
+// another before their sums are joined at the end; a wave's own row offsets go through LDS.  64
+// requests of 1 to 12 Ki tokens, 32 heads over 8, 128 channels: 323 us with the join, 5.1 TB/s, as
+// fast as a copy reads and writes; 32 rows 3.7 TB/s, 256 channels 4.2; one token over 512, a chain
+// of loads, 7.6 us with the join in a graph.
+// N8 / N4: panels of 128 / 64 channels.  Past 16 rows, and from 129 to 192 channels, the queries
+// stay in LDS (one barrier) and are read again for every 32 keys: with them in registers a wave
+// would not fit its 256.  Past 192 channels it does not fit them either way, and has a SIMD's 512 to
+// itself.
 // WHOLE: D is all of the panels' channels.
 template <int DT, int N8, int N4, int R, bool WHOLE>
 __global__ __launch_bounds__((N8 == 2 ? 256 : 512), (N8 == 2 ? 1 : 2)) void attend_rows_kernel(kvmi_attention_args a,
@@ -450,12 +452,15 @@ Choice choose(const kvmi_attention_args& a) {
   const int64_t groups = tiles * a.cache.num_heads;
   // Keys are split until there are workgroups for the chip, one a CU for few rows (a workgroup
   // then keeps 4 waves' loads in flight) and two for tiles, but not below the part at which the
-  // join costs more than it saves: 64 keys of few rows (512 keys of one token: 7.5 us in 8 parts,
-  // 8.3 in 4, 8.8 in 16, 9.6 whole), 256 of tiles.  Few rows are split at 704 keys in any case,
-  // against requests of unequal lengths and a last round of workgroups that leaves the chip half
-  // empty (us at 512 / 704 / 1024 / 1536 keys: 64 requests of 1 to 12 Ki 333 / 325 / 325 / 329, 64 of
-  // 1 to 8 Ki and 64 channels 128 / 127 / 140 / 132, 32 of 256 channels 123 / 119 / 135 / 108, 256 of
-  // up to 3 Ki 357 / 340 / 333 / 350).
+  // join costs more than it saves: 64 keys of few rows (512 keys of one token in a graph: 7.5 us in
+  // 8 parts, 8.3 in 4, 8.8 in 16, 9.6 whole), 256 of tiles.  Few rows are split at 704 keys in any
+  // case, against requests of unequal lengths and a last round of workgroups that leaves the chip
+  // half empty.  That is a compromise of four batches, two of which would have more (us at 512 / 704
+  // / 1024 / 1536 keys: 64 requests of 1 to 12 Ki 333 / 325 / 325 / 329, 64 of 1 to 8 Ki and 64
+  // channels 128 / 127 / 140 / 132, 32 of 256 channels 123 / 119 / 135 / 108, 256 of up to 3 Ki
+  // 357 / 340 / 333 / 350).  Tiles of a ragged batch are not split below the longest request: every
+  // finer part costs more than the chains it cuts (96 trees over 200 to 2000 tokens whole 54.7, at
+  // 1024 / 768 / 512 keys 64.2 / 58.7 / 65.2).
   const bool even = (int64_t)a.requests * c.plan.row_tiles <= tiles;  // all have the most queries
   const int64_t room = c.rows ? 256 : 512, want = std::max<int64_t>(1, (room + (even ? 0 : groups - 1)) / groups);
   c.plan.chunk = (int)std::max<int64_t>((length + want - 1) / want, c.rows ? 64 : 256);

@@ -10,10 +10,10 @@
 //
 // Work: 64 products of 32x32x16 a wave and tile at 128 channels, 2048 cycles of the matrix unit
 // for the two waves of a SIMD, against about 135 vector instructions and 32 exponentials each.  A
-// prompt of 8192 tokens, 32 heads over 8, 128 channels runs in 547 us (1.0 PFLOP/s, the matrix
-// unit busy 44 % of the time; 64 channels: 0.83, 256: 0.58), 8 trees of 64 drafts with 8 heads a
-// KV head over 28 Ki tokens in 551 us (885 TFLOP/s), 96 trees of 26 drafts with 7 heads over 200
-// to 2000 tokens of 64 channels in 53 us.  Bound by issue and latency of two waves a SIMD (three
+// prompt of 8192 tokens, 32 heads over 8, 128 channels runs in 564 us (0.98 PFLOP/s, the matrix
+// unit busy 45 % of the time; 64 channels: 0.80, 192: 0.74, 256: 0.59), 8 trees of 64 drafts with 8
+// heads a KV head over 28 Ki tokens in 569 us (856 TFLOP/s), 96 trees of 26 drafts with 7 heads over
+// 200 to 2000 tokens of 64 channels in 55 us.  Bound by issue and latency of two waves a SIMD (three
 // at 64 channels); where few workgroups are left, by one's chain of tiles, 1.0 (64 channels) to
 // 1.35 us (128) each.
 #include "kvmi_attention.hpp"

@@ -60,8 +60,10 @@ __device__ __forceinline__ uint32_t ring_at(uint32_t base, uint32_t i, uint32_t 
 // the last free block never reach the head's: blocks returned here are not read here.  In a ring
 // that has no such room, blocks past its free places are dropped and reported, not written over
 // the free ones that other workgroups read.
-// 1024 requests of all sorts, rows of 1024, 420 Ki new tokens: 9.4 us (1.8 by its 8.8 MB: bound by
-// instructions and the chain lengths, ring, stores); 256 that grow by 8 tokens: 4.5.
+// 1024 requests of all sorts, rows of 1024, 420 Ki new tokens: 8.8 us (1.8 by its 8.8 MB: bound by
+// instructions and the chain lengths, ring, stores); 256 that grow by 8 tokens: 4.2.  With lengths
+// and state written over, where every workgroup adds to the ticket and the last one walks all
+// requests again, 8.0 for those 256 and 32 for 1024 that grow by 33 (7.4 into other tensors).
 __global__ __launch_bounds__(kThreads) void tables_kernel(kvmi_tables_args a, BlockOf div) {
   __shared__ uint32_t sums[3][4];
   __shared__ int64_t lds[4];
@@ -253,7 +255,7 @@ struct WriteArgs {
 
 // A group of 2^lanes_log2 lanes copies one token's K and V rows in units of V (16 bytes, or 2
 // where a stride or an address is not aligned): copies, bound by memory.  16384 tokens of 8 x 128:
-// 28.6 us out of memory (4.7 TB/s read and written), 19.6 out of the caches; 96 tokens: 2.4.
+// 28.6 us out of memory (4.7 TB/s read and written), 21.4 out of the caches; 96 tokens: 2.5.
 template <class V>
 __global__ __launch_bounds__(kThreads) void write_kernel(WriteArgs a) {
   constexpr int U = sizeof(V) / 2;
@@ -304,7 +306,8 @@ __device__ __forceinline__ int64_t lane_value(int64_t v, int i) {
 // owns one 16-byte (or 2-byte) column of the row and walks the path in order, so no thread waits
 // for another: path[i] >= i and the path increases, hence a row is read before, or in the same
 // step as, it is overwritten.  Bound by its chain of loads (path, tables, rows; 28 layers of one
-// request 3.3 us, 32 layers of 32 requests 7.7): a path of up to 64 is checked by every wave for itself, a draft a lane, without a barrier.
+// request 2.9 us, 32 layers of 32 requests 8.7): a path of up to 64 is checked by every wave for
+// itself, a draft a lane, without a barrier.
 template <class V, bool SHORT>
 __global__ __launch_bounds__(kThreads) void keep_kernel(KeepArgs a) {
   constexpr int U = sizeof(V) / 2, kStep = 8;
