@@ -608,7 +608,8 @@ int kvmi_tree_attention(const kvmi_attention_args* args, kvmi_stream_t stream);
  * lengths[r] + the path's length (not `lengths` itself).  A path that does not increase or leaves
  * the table sets KVMI_ERR_LENGTH, a bad block id KVMI_ERR_BLOCK_ID; that request is left as it is
  * and keeps its length.  `bases` is a device array of the layers' cache bases; `cache` gives their
- * common layout, and `cache->base` the bitwise OR of all bases (their alignment).  width <= 1024.
+ * common layout, and `cache->base` the bitwise OR of all bases (their alignment).  No two layers may
+ * share memory.  width <= 1024.
  */
 int kvmi_keep_drafts(const kvmi_cache* cache, void* const* bases, int32_t layers, const int32_t* tables,
                      int32_t columns, const int32_t* lengths, const int32_t* accepted, int32_t requests,
