@@ -64,6 +64,7 @@ typedef struct ihipStream_t* kvmi_stream_t;
 #define KVMI_ERR_SCHEDULE 32    /* a job has more blocks than its one-pass schedule */
 #define KVMI_ERR_NO_BLOCKS 64   /* kvmi_build_tables: a request was refused, too few free blocks */
 #define KVMI_ERR_LENGTH 128     /* a length, slot range, query range, path or free ring outside its bounds */
+#define KVMI_ERR_NOT_FINITE 256 /* kvmi_select_beams: NaN or +inf among the scores or logits */
 
 /* Host-visible return codes. */
 #define KVMI_OK 0
@@ -614,6 +615,135 @@ int kvmi_tree_attention(const kvmi_attention_args* args, kvmi_stream_t stream);
 int kvmi_keep_drafts(const kvmi_cache* cache, void* const* bases, int32_t layers, const int32_t* tables,
                      int32_t columns, const int32_t* lengths, const int32_t* accepted, int32_t requests,
                      int32_t width, int32_t* out_lengths, int32_t* err, kvmi_stream_t stream);
+
+/*
+ * ---- Sequences that share blocks: block tables forked with counted blocks, blocks copied,
+ * the pool compacted, and beam search's selection.
+ */
+
+/*
+ * Block tables whose rows may share blocks, brought from one set of rows to another.  Row r
+ * becomes the first kept = min(lengths[p], new) tokens of row p = parents[r] and grows from there
+ * to `new` tokens with blocks out of the ring.
+ *   parents        int32 [R]: the row that each goes on from, or -1 (it starts empty); null: itself
+ *   new_lengths    int32 [R], or null: lengths[p] + grow, and 0 where there is no parent
+ *   shares         int32 [blocks]: how many rows hold a block besides the first (0: one or none)
+ *   free_blocks    int32 [blocks], the ring of kvmi_build_tables; `state` = {head, count}
+ * Whole blocks of kept tokens are shared.  The block with the last kept % S ones, if any, goes on
+ * with one row: the first child of p that keeps p's most blocks so, where no other row holds it
+ * before.  Every other row takes a block for these tokens and lists a copy.  Blocks that no row
+ * holds any more go behind the ring's last free block, in the order of their ids.
+ *   out_tables, out_lengths, out_shares, out_state   all of them the inputs themselves, or none
+ *   slots, starts  as in kvmi_build_tables, rows in the place of requests
+ *   copies         int32 [R][3]: (from, to, tokens) for kvmi_copy_blocks, which has to run before
+ *                  the new tokens are written; -1 behind the last
+ *   workspace      kvmi_fork_workspace_bytes, 8-byte aligned: zero before the first call, and left
+ *                  so that the next call of the same sizes can use it
+ * All or nothing: where the blocks asked for exceed the free ones (KVMI_ERR_NO_BLOCKS), the new
+ * tokens exceed max_tokens, or a parent, a length or the ring's count is out of range
+ * (KVMI_ERR_LENGTH), rows and ring stay as they are, all slots and copies are -1 and starts 0.
+ * A row's id outside the pool is handed on, and sets KVMI_ERR_BLOCK_ID where its holders change.
+ * Two launches; R <= 4096.
+ */
+typedef struct kvmi_fork_args {
+  const int32_t* lengths;
+  const int32_t* parents;
+  const int32_t* new_lengths;
+  const int32_t* tables;
+  const int32_t* shares;
+  int32_t* free_blocks;
+  const int32_t* state;
+  int32_t* out_tables;
+  int32_t* out_lengths;
+  int32_t* out_shares;
+  int32_t* out_state;
+  int64_t* slots;
+  int32_t* starts;
+  int32_t* copies;
+  int32_t* workspace;
+  int64_t workspace_bytes;
+  int32_t* err;
+  int32_t rows, columns, blocks, block_size, max_tokens, grow;
+} kvmi_fork_args;
+int64_t kvmi_fork_workspace_bytes(int32_t blocks, int32_t rows, int32_t columns);
+int kvmi_fork_tables(const kvmi_fork_args* args, kvmi_stream_t stream);
+
+/*
+ * In every layer (`cache`, `bases` as in kvmi_keep_drafts), for every row (from, to, tokens) of
+ * `copies` int32 [n][3]: the first `tokens` tokens of block `from`, keys and values, are written
+ * to block `to`.  Rows with a negative `from` are skipped.  No block may be written by two rows, nor
+ * read by one and written by another.  A block outside the cache sets KVMI_ERR_BLOCK_ID, more tokens
+ * than a block has (or a negative number) KVMI_ERR_LENGTH; such a row copies nothing.
+ */
+int kvmi_copy_blocks(const kvmi_cache* cache, void* const* bases, int32_t layers, const int32_t* copies, int32_t n,
+                     int32_t* err, kvmi_stream_t stream);
+
+/*
+ * The blocks that rows hold moved to the front of the pool.  The pool is what the rows hold and
+ * what the ring has free; with n blocks held, those among the pool's n lowest ids stay, and the others'
+ * names become, in order, the free ids among these n.
+ *   out_tables, out_shares, out_free, out_state   the arrays under the new names, every entry
+ *                  written (-1 behind a row, 0 for free blocks); the ring begins at 0 and holds the
+ *                  pool's other ids in order.  All of them the inputs themselves, or none
+ *   copies         int32 [blocks / 2][3]: the moves (from, to, block_size) for kvmi_copy_blocks,
+ *                  -1 behind the last
+ *   workspace      kvmi_compact_workspace_bytes, 8-byte aligned, as in kvmi_fork_tables
+ * Ids outside the pool set KVMI_ERR_BLOCK_ID and keep their names; so do blocks that are both held and
+ * free (held counts).  A length or count out of range sets KVMI_ERR_LENGTH and is cut.
+ */
+typedef struct kvmi_compact_args {
+  const int32_t* lengths;
+  const int32_t* tables;
+  const int32_t* shares;
+  const int32_t* free_blocks;
+  const int32_t* state;
+  int32_t* out_tables;
+  int32_t* out_shares;
+  int32_t* out_free;
+  int32_t* out_state;
+  int32_t* copies;
+  int32_t* workspace;
+  int64_t workspace_bytes;
+  int32_t* err;
+  int32_t rows, columns, blocks, block_size;
+} kvmi_compact_args;
+int64_t kvmi_compact_workspace_bytes(int32_t blocks);
+int kvmi_compact_tables(const kvmi_compact_args* args, kvmi_stream_t stream);
+
+/*
+ * The best continuations of every request's beams.  Row r * beams + b of `logits` [rows][vocab]
+ * (rows row_stride elements apart) belongs to request r's beam b, whose sum of log-probabilities so
+ * far is scores[row].  Candidate (row, token) has the value
+ *   scores[row] + (logits[row][token] - log(sum over t of exp(logits[row][t])))
+ * and the `count` largest of a request are found; among equal ones the lower row comes first, then the
+ * larger logit, then the lower token.  Sums and values are in 64 bits.  A value of -inf (after its
+ * rounding to fp32) is no candidate, nor is anything in a row whose score or sum is not finite; NaN
+ * or +inf there sets KVMI_ERR_NOT_FINITE, but for rows whose score is -inf, which are not read.
+ *   all_parents, all_tokens (int32), all_scores (fp32)  [requests][count] the candidates, best first:
+ *                  row, token, value; behind the last -1, -1, -inf
+ *   parents, tokens (int32), scores (fp32)  [requests * beams] those that go on: of each request the
+ *                  first `beams` candidates with a token other than end_token, filled up alike
+ * 1 <= beams <= count <= 64, at most 65535 rows; end_token -1: there is none.
+ */
+typedef struct kvmi_select_args {
+  const void* logits;
+  const float* scores;
+  int32_t* parents;
+  int32_t* tokens;
+  float* next_scores;
+  int32_t* all_parents;
+  int32_t* all_tokens;
+  float* all_scores;
+  void* workspace; /* kvmi_select_workspace_bytes of the same arguments, 16-byte aligned */
+  int64_t workspace_bytes;
+  int32_t* err;
+  int64_t row_stride;
+  int32_t dtype; /* KVMI_DTYPE_* */
+  int32_t requests, beams, vocab, count, end_token;
+} kvmi_select_args;
+#define KVMI_DTYPE_FP32 2 /* of logits */
+int64_t kvmi_select_workspace_bytes(const kvmi_select_args* args);
+int kvmi_select_beams(const kvmi_select_args* args, kvmi_stream_t stream);
 
 #ifdef __cplusplus
 }

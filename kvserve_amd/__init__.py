@@ -2,7 +2,8 @@
 
   engine    FusedKVCodec: paged gather + FWHT + min-max quant + bitpack (and inverse)
   ops       unit operators: bitpack codec, paged gather / scatter, Hadamard
-  paged     decode instance: block tables, slot writes, attention of drafts, kept drafts
+  paged     decode instance: block tables, slot writes, attention of drafts, kept drafts; rows that
+            share blocks, copied blocks, compaction, beam selection
   profiles  signs recipe, head / layer masks, per-layer quantization profiles
   compression  drop-in mirror of kvserve_v1.compression (adapter, manager, operators)
 

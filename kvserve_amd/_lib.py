@@ -25,6 +25,7 @@ ERR_BLOCK_ID = 16
 ERR_SCHEDULE = 32
 ERR_NO_BLOCKS = 64
 ERR_LENGTH = 128
+ERR_NOT_FINITE = 256
 OK, EINVAL, ELAUNCH, ENOSPC = 0, -22, -5, -28
 # Bytes of the fixed device array behind kvmi_v3_compress_noalloc (per GPU).
 V3_NOALLOC_SCRATCH_BYTES = 4 * 1024 * 1024
@@ -83,6 +84,13 @@ EXPORTS = (
     "kvmi_attention_kernels",
     "kvmi_tree_attention",
     "kvmi_keep_drafts",
+    "kvmi_fork_workspace_bytes",
+    "kvmi_fork_tables",
+    "kvmi_copy_blocks",
+    "kvmi_compact_workspace_bytes",
+    "kvmi_compact_tables",
+    "kvmi_select_workspace_bytes",
+    "kvmi_select_beams",
 )
 
 
@@ -132,7 +140,7 @@ class RtLayer(ctypes.Structure):
                 ("num_sections", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
-DTYPE_BF16, DTYPE_FP16 = 0, 1
+DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2
 ATTENTION_ROWS, ATTENTION_TILES = 0, 1
 
 
@@ -156,6 +164,29 @@ class AttentionArgs(ctypes.Structure):
             ("query_head_stride", ctypes.c_int64), ("scale", ctypes.c_float)] + [(name, ctypes.c_int32) for name in (
                 "dtype", "requests", "columns", "total_queries", "query_heads", "max_query", "max_length",
                 "mask_words", "reserved")]
+
+
+class ForkArgs(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "lengths", "parents", "new_lengths", "tables", "shares", "free_blocks", "state", "out_tables", "out_lengths",
+        "out_shares", "out_state", "slots", "starts", "copies", "workspace")] + [
+            ("workspace_bytes", ctypes.c_int64), ("err", ctypes.c_void_p)] + [(name, ctypes.c_int32) for name in (
+                "rows", "columns", "blocks", "block_size", "max_tokens", "grow")]
+
+
+class CompactArgs(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "lengths", "tables", "shares", "free_blocks", "state", "out_tables", "out_shares", "out_free", "out_state",
+        "copies", "workspace")] + [("workspace_bytes", ctypes.c_int64), ("err", ctypes.c_void_p)] + [
+            (name, ctypes.c_int32) for name in ("rows", "columns", "blocks", "block_size")]
+
+
+class SelectArgs(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "logits", "scores", "parents", "tokens", "next_scores", "all_parents", "all_tokens", "all_scores",
+        "workspace")] + [("workspace_bytes", ctypes.c_int64), ("err", ctypes.c_void_p),
+                         ("row_stride", ctypes.c_int64)] + [(name, ctypes.c_int32) for name in (
+                             "dtype", "requests", "beams", "vocab", "count", "end_token")]
 
 
 # kvmi_layer_job: 8 pointers, 4 int64, 2 int32 -> 104 bytes, 8-byte aligned.  It is
@@ -213,6 +244,13 @@ _SIGNATURES = {
     "kvmi_tree_attention": ([ctypes.POINTER(AttentionArgs), _vp], ctypes.c_int),
     "kvmi_keep_drafts": ([ctypes.POINTER(Cache), _vp, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp],
                          ctypes.c_int),
+    "kvmi_fork_workspace_bytes": ([_i32, _i32, _i32], _i64),
+    "kvmi_fork_tables": ([ctypes.POINTER(ForkArgs), _vp], ctypes.c_int),
+    "kvmi_copy_blocks": ([ctypes.POINTER(Cache), _vp, _i32, _vp, _i32, _vp, _vp], ctypes.c_int),
+    "kvmi_compact_workspace_bytes": ([_i32], _i64),
+    "kvmi_compact_tables": ([ctypes.POINTER(CompactArgs), _vp], ctypes.c_int),
+    "kvmi_select_workspace_bytes": ([ctypes.POINTER(SelectArgs)], _i64),
+    "kvmi_select_beams": ([ctypes.POINTER(SelectArgs), _vp], ctypes.c_int),
 }
 
 

@@ -255,11 +255,165 @@ PyObject* keep_drafts(PyObject*, PyObject* const* in, Py_ssize_t n) try {
   return answer(false);
 }
 
+// fork_block_tables(lengths, parents, new_lengths, tables, shares, free, state, block_size, max_tokens, out,
+// workspace, err), `out` a tuple of tables, lengths, shares, state, slots, starts, copies
+PyObject* fork_block_tables(PyObject*, PyObject* const* in, Py_ssize_t n) try {
+  if (n != 12 || !PyTuple_Check(in[9]) || PyTuple_GET_SIZE(in[9]) != 7) return answer(false);
+  Args a;
+  kvmi_fork_args t;
+  std::memset(&t, 0, sizeof(t));
+  a.integer(in[7], &t.block_size);
+  a.integer(in[8], &t.max_tokens);
+  const at::Tensor *now = a.any(in[0]), *tables = a.any(in[3]), *shares = a.any(in[4]), *space = a.any(in[10]);
+  if (!a.ok || tables->dim() != 2) return answer(false);
+  const int64_t R = now->numel(), C = tables->size(1), N = shares->numel();
+  if (R < 1 || R > 0x7fffffff || C > 0x7fffffff || N > 0x7fffffff) return answer(false);
+  t.rows = (int32_t)R;
+  t.columns = (int32_t)C;
+  t.blocks = (int32_t)N;
+  t.lengths = a.flat<int32_t>(in[0], at::kInt, R);
+  if (in[1] != Py_None) t.parents = a.flat<int32_t>(in[1], at::kInt, R);
+  if (PyLong_CheckExact(in[2]))
+    a.integer(in[2], &t.grow);
+  else
+    t.new_lengths = a.flat<int32_t>(in[2], at::kInt, R);
+  t.tables = a.flat<int32_t>(in[3], at::kInt, R, C);
+  t.shares = a.flat<int32_t>(in[4], at::kInt, N);
+  t.free_blocks = a.flat<int32_t>(in[5], at::kInt, N);
+  t.state = a.flat<int32_t>(in[6], at::kInt, 2);
+  PyObject* const out = in[9];
+  t.out_tables = a.flat<int32_t>(PyTuple_GET_ITEM(out, 0), at::kInt, R, C);
+  t.out_lengths = a.flat<int32_t>(PyTuple_GET_ITEM(out, 1), at::kInt, R);
+  t.out_shares = a.flat<int32_t>(PyTuple_GET_ITEM(out, 2), at::kInt, N);
+  t.out_state = a.flat<int32_t>(PyTuple_GET_ITEM(out, 3), at::kInt, 2);
+  t.slots = a.flat<int64_t>(PyTuple_GET_ITEM(out, 4), at::kLong, t.max_tokens);
+  t.starts = a.flat<int32_t>(PyTuple_GET_ITEM(out, 5), at::kInt, R + 1);
+  t.copies = a.flat<int32_t>(PyTuple_GET_ITEM(out, 6), at::kInt, R, 3);
+  t.workspace = a.flat<int32_t>(in[10], at::kInt, -1);
+  t.workspace_bytes = space->numel() * 4;
+  t.err = a.err(in[11]);
+  kvmi_stream_t st;
+  if (!a.stream(&st)) return answer(false);
+  return enqueue([&] { return kvmi_fork_tables(&t, st); });
+} catch (...) {
+  return answer(false);
+}
+
+// copy_blocks(cache struct's address, bases, copies, err)
+PyObject* copy_blocks(PyObject*, PyObject* const* in, Py_ssize_t n) try {
+  if (n != 4 || !PyLong_CheckExact(in[0])) return answer(false);
+  const kvmi_cache* c = static_cast<const kvmi_cache*>(PyLong_AsVoidPtr(in[0]));
+  if (!c) {
+    PyErr_Clear();
+    return answer(false);
+  }
+  Args a;
+  const at::Tensor *bases = a.any(in[1]), *copies = a.any(in[2]);
+  if (!a.ok || copies->dim() != 2) return answer(false);
+  const int64_t L = bases->numel(), rows = copies->size(0);
+  if (L > 32767 || rows < 1 || rows > 0x7fffffff) return answer(false);
+  const int64_t* at_bases = a.flat<int64_t>(in[1], at::kLong, L);
+  const int32_t* list = a.flat<int32_t>(in[2], at::kInt, rows, 3);
+  int32_t* err = a.err(in[3]);
+  kvmi_stream_t st;
+  if (!a.stream(&st)) return answer(false);
+  return enqueue([&] { return kvmi_copy_blocks(c, (void* const*)at_bases, (int32_t)L, list, (int32_t)rows, err, st); });
+} catch (...) {
+  return answer(false);
+}
+
+// compact_block_tables(lengths, tables, shares, free, state, block_size, out, workspace, err), `out` a
+// tuple of tables, shares, free, state, copies
+PyObject* compact_block_tables(PyObject*, PyObject* const* in, Py_ssize_t n) try {
+  if (n != 9 || !PyTuple_Check(in[6]) || PyTuple_GET_SIZE(in[6]) != 5) return answer(false);
+  Args a;
+  kvmi_compact_args t;
+  std::memset(&t, 0, sizeof(t));
+  a.integer(in[5], &t.block_size);
+  const at::Tensor *now = a.any(in[0]), *tables = a.any(in[1]), *shares = a.any(in[2]), *space = a.any(in[7]);
+  if (!a.ok || tables->dim() != 2) return answer(false);
+  const int64_t R = now->numel(), C = tables->size(1), N = shares->numel();
+  if (R < 1 || R > 0x7fffffff || C > 0x7fffffff || N < 1 || N > 0x7fffffff) return answer(false);
+  t.rows = (int32_t)R;
+  t.columns = (int32_t)C;
+  t.blocks = (int32_t)N;
+  t.lengths = a.flat<int32_t>(in[0], at::kInt, R);
+  t.tables = a.flat<int32_t>(in[1], at::kInt, R, C);
+  t.shares = a.flat<int32_t>(in[2], at::kInt, N);
+  t.free_blocks = a.flat<int32_t>(in[3], at::kInt, N);
+  t.state = a.flat<int32_t>(in[4], at::kInt, 2);
+  PyObject* const out = in[6];
+  t.out_tables = a.flat<int32_t>(PyTuple_GET_ITEM(out, 0), at::kInt, R, C);
+  t.out_shares = a.flat<int32_t>(PyTuple_GET_ITEM(out, 1), at::kInt, N);
+  t.out_free = a.flat<int32_t>(PyTuple_GET_ITEM(out, 2), at::kInt, N);
+  t.out_state = a.flat<int32_t>(PyTuple_GET_ITEM(out, 3), at::kInt, 2);
+  t.copies = a.flat<int32_t>(PyTuple_GET_ITEM(out, 4), at::kInt, N / 2, 3);
+  t.workspace = a.flat<int32_t>(in[7], at::kInt, -1);
+  t.workspace_bytes = space->numel() * 4;
+  t.err = a.err(in[8]);
+  kvmi_stream_t st;
+  if (!a.stream(&st)) return answer(false);
+  return enqueue([&] { return kvmi_compact_tables(&t, st); });
+} catch (...) {
+  return answer(false);
+}
+
+// select_beams(logits, scores, beams, count, end_token, out, err), `out` a tuple of parents, tokens,
+// scores, all_parents, all_tokens, all_scores
+PyObject* select_beams(PyObject*, PyObject* const* in, Py_ssize_t n) try {
+  if (n != 7 || !PyTuple_Check(in[5]) || PyTuple_GET_SIZE(in[5]) != 6) return answer(false);
+  Args a;
+  kvmi_select_args t;
+  std::memset(&t, 0, sizeof(t));
+  a.integer(in[2], &t.beams);
+  a.integer(in[3], &t.count);
+  t.end_token = -1;
+  if (in[4] != Py_None) a.integer(in[4], &t.end_token);
+  const at::Tensor* logits = a.any(in[0]);
+  if (!a.ok || t.beams < 1 || logits->dim() != 2) return answer(false);
+  const int64_t rows = logits->size(0), V = logits->size(1), R = rows / t.beams;
+  if (rows < 1 || rows > 65535 || rows % t.beams || V < 1 || V > 0x7fffffff || (logits->stride(1) != 1 && V > 1))
+    return answer(false);
+  switch (logits->scalar_type()) {
+    case at::kBFloat16: t.dtype = KVMI_DTYPE_BF16; break;
+    case at::kHalf: t.dtype = KVMI_DTYPE_FP16; break;
+    case at::kFloat: t.dtype = KVMI_DTYPE_FP32; break;
+    default: return answer(false);
+  }
+  t.requests = (int32_t)R;
+  t.vocab = (int32_t)V;
+  t.logits = logits->data_ptr();
+  t.row_stride = logits->stride(0);
+  t.scores = a.flat<float>(in[1], at::kFloat, rows);
+  PyObject* const out = in[5];
+  t.parents = a.flat<int32_t>(PyTuple_GET_ITEM(out, 0), at::kInt, rows);
+  t.tokens = a.flat<int32_t>(PyTuple_GET_ITEM(out, 1), at::kInt, rows);
+  t.next_scores = a.flat<float>(PyTuple_GET_ITEM(out, 2), at::kFloat, rows);
+  t.all_parents = a.flat<int32_t>(PyTuple_GET_ITEM(out, 3), at::kInt, R, t.count);
+  t.all_tokens = a.flat<int32_t>(PyTuple_GET_ITEM(out, 4), at::kInt, R, t.count);
+  t.all_scores = a.flat<float>(PyTuple_GET_ITEM(out, 5), at::kFloat, R, t.count);
+  t.err = a.err(in[6]);
+  kvmi_stream_t st;
+  if (!a.stream(&st)) return answer(false);
+  const int64_t space = kvmi_select_workspace_bytes(&t);
+  if (space < 0) return answer(false);
+  at::Tensor parts = at::empty({space}, logits->options().dtype(at::kByte).requires_grad(false));
+  t.workspace = parts.data_ptr();
+  t.workspace_bytes = space;
+  return enqueue([&] { return kvmi_select_beams(&t, st); });
+} catch (...) {
+  return answer(false);
+}
+
 PyMethodDef kMethods[] = {
     {"write_kv", (PyCFunction)(void (*)(void))write_kv, METH_FASTCALL, nullptr},
     {"build_block_tables", (PyCFunction)(void (*)(void))build_block_tables, METH_FASTCALL, nullptr},
     {"tree_attention", (PyCFunction)(void (*)(void))tree_attention, METH_FASTCALL, nullptr},
     {"keep_drafts", (PyCFunction)(void (*)(void))keep_drafts, METH_FASTCALL, nullptr},
+    {"fork_block_tables", (PyCFunction)(void (*)(void))fork_block_tables, METH_FASTCALL, nullptr},
+    {"copy_blocks", (PyCFunction)(void (*)(void))copy_blocks, METH_FASTCALL, nullptr},
+    {"compact_block_tables", (PyCFunction)(void (*)(void))compact_block_tables, METH_FASTCALL, nullptr},
+    {"select_beams", (PyCFunction)(void (*)(void))select_beams, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,6 +1,6 @@
 // Decode-instance upkeep of the paged cache: block tables and slot maps from request
 // lengths, new keys and values written by slot, accepted drafts kept.
-#include "kvmi_common.hpp"
+#include "kvmi_paged.hpp"
 
 #include <algorithm>
 
@@ -8,10 +8,6 @@ namespace kvmi {
 namespace {
 
 constexpr int kThreads = 256;
-
-__device__ __forceinline__ void flag_error(int32_t* err, int32_t bits) {
-  if (err && bits) atomicOr(err, bits);
-}
 
 // Sum over the workgroup, given to every thread.
 __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* lds) {
@@ -22,7 +18,6 @@ __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* lds) {
   __syncthreads();
   return lds[0] + lds[1] + lds[2] + lds[3];
 }
-__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
 
 // ---------------------------------------------------------------- block tables
 struct Need {  // what one request's change of length asks for
@@ -46,12 +41,6 @@ __device__ __forceinline__ Need need_of(const kvmi_tables_args& a, const BlockOf
 __device__ __forceinline__ Need need_of(const kvmi_tables_args& a, const BlockOf& div, int r) {
   return need_of(a, div, a.lengths[r], a.new_lengths[r]);
 }
-// Place of the i-th entry behind `base` in a ring of N (base < N, i <= N).
-__device__ __forceinline__ uint32_t ring_at(uint32_t base, uint32_t i, uint32_t N) {
-  const uint32_t x = base + i;
-  return x < N ? x : x - N;
-}
-
 // Workgroup (r, y) makes part y of request r's table row and slots.  No workgroup waits for
 // another: each adds up what the requests before its own ask for and give back (R lengths out
 // of the L2, a few microseconds less than a scan kernel and a second launch would take), and
@@ -380,17 +369,6 @@ __global__ __launch_bounds__(kThreads) void keep_kernel(KeepArgs a) {
     }
   }
 }
-
-bool cache_ok(const kvmi_cache* c, bool base) {
-  return c && (!base || c->base) && c->num_blocks >= 1 && c->block_size >= 1 && c->num_heads >= 1 && c->head_dim >= 1 &&
-         c->part_stride >= 0 && c->block_stride >= (int64_t)c->block_size * c->num_heads * c->head_dim &&
-         (int64_t)c->num_blocks * c->block_size < 0x7fffffffLL && (int64_t)c->num_heads * c->head_dim < (1 << 24);
-}
-bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
-bool strides16(const kvmi_cache* c) {
-  return c->head_dim % 8 == 0 && c->part_stride % 8 == 0 && c->block_stride % 8 == 0;
-}
-int launched() { return hipGetLastError() == hipSuccess ? KVMI_OK : KVMI_ELAUNCH; }
 
 }  // namespace
 }  // namespace kvmi

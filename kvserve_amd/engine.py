@@ -680,6 +680,8 @@ def raise_device_error(code: int) -> None:
         raise RuntimeError("too few free blocks: a request was refused")
     if code & _lib.ERR_LENGTH:  # before the block ids: a length too long reads past its blocks
         raise ValueError("a length, token range, path or ring of free blocks is out of range")
+    if code & _lib.ERR_NOT_FINITE:
+        raise ValueError("NaN or +inf among the scores or logits")
     if code & _lib.ERR_SYMBOL_RANGE:
         raise RuntimeError("symbol exceeds bitpack_bits")
     if code & _lib.ERR_BAD_HEADER:

@@ -1,6 +1,7 @@
 """Operators of a decode instance over its paged KV caches: block tables built on the GPU from
 request lengths, keys and values written by slot, attention of drafted tokens over the cache,
-and the accepted drafts kept.
+and the accepted drafts kept; and, for requests with several answers, rows that share blocks,
+blocks copied, the pool compacted and beam search's selection.
 
 A received request is written into its blocks by `FusedKVCodec.decompress`; from there on a
 step with drafts is
@@ -11,6 +12,12 @@ step with drafts is
                          max_query=drafts, tree_mask=mask)               # each layer
     lengths = keep_drafts(layers, tables.tables, lengths, accepted)      # all layers at once
     tables.update(lengths, 0)                                            # blocks given back
+
+and one of a beam search, over `SharedBlockTables`,
+
+    best = select_beams(logits, scores, beams, 2 * beams, end_token=end)
+    slots, starts = tables.fork(best.parents, 1, rows)                   # reordered, grown by a token
+    copy_blocks(layers, tables.copies)                                   # partly filled blocks split
 
 Everything is enqueued on the current stream of the tensors' device and reads lengths, tables
 and slots on the GPU.  Errors found there (a block id outside the cache, too few free blocks, a
@@ -432,4 +439,375 @@ def keep_drafts(caches, tables: torch.Tensor, lengths: torch.Tensor, accepted: t
     if R:
         call.run("kvmi_keep_drafts", layers.struct, layers.bases.data_ptr(), len(layers.caches), tab, tables.shape[1],
                  now, path, R, accepted.shape[1], res, call.err_ptr)
+    return out
+
+
+# ------------------------------------------------------------------ rows that share blocks
+class ForkUpdate(NamedTuple):
+    """What `fork_block_tables` gives back."""
+
+    tables: torch.Tensor   # int32 [R, columns]
+    lengths: torch.Tensor  # int32 [R]
+    shares: torch.Tensor   # int32 [blocks]
+    state: torch.Tensor    # int32 [2]: head and count of the free ring
+    slots: torch.Tensor    # int64 [max_tokens], -1 where there is none
+    starts: torch.Tensor   # int32 [R + 1]: each row's first new token in `slots`
+    copies: torch.Tensor   # int32 [R, 3]: blocks to be copied, for `copy_blocks`
+
+
+def _words(size: int, device) -> torch.Tensor:
+    if size < 0:
+        raise ValueError("the sizes of a pool and its rows must be positive")
+    return torch.zeros((size + 3) // 4, dtype=torch.int32, device=device)
+
+
+def _sizes(**sizes) -> None:
+    for name, v in sizes.items():
+        if type(v) is not int or not 1 <= v <= _INT32_MAX:
+            raise ValueError(f"{name} must be a positive integer in 31 bits")
+
+
+def fork_workspace(blocks: int, rows: int, columns: int, device="cuda") -> torch.Tensor:
+    """Workspace of `fork_block_tables` for a pool of `blocks` and `rows` rows of `columns` entries.
+    A call leaves it as it found it; no two calls may use it at a time."""
+    _sizes(blocks=blocks, rows=rows, columns=columns)
+    return _words(_lib.load().kvmi_fork_workspace_bytes(blocks, rows, columns), device)
+
+
+def compact_workspace(blocks: int, device="cuda") -> torch.Tensor:
+    """Workspace of `compact_block_tables` for a pool of `blocks`; as that of `fork_workspace`."""
+    _sizes(blocks=blocks)
+    return _words(_lib.load().kvmi_compact_workspace_bytes(blocks), device)
+
+
+def _space(workspace: Optional[torch.Tensor], size: int, device) -> torch.Tensor:
+    if size < 0:
+        raise ValueError("the sizes of a pool and its rows must be positive")
+    if workspace is None:
+        return _words(size, device)
+    _tensor(workspace, "workspace", torch.int32, (None,), device)
+    if workspace.numel() * 4 < size or workspace.data_ptr() % 8:
+        raise ValueError(f"workspace must hold {(size + 3) // 4} words, 8-byte aligned")
+    return workspace
+
+
+def _in_place(pairs) -> bool:
+    """Whether the outputs are the inputs themselves: all of them, or none."""
+    same = [a.data_ptr() == b.data_ptr() and a.numel() > 0 for a, b in pairs if a.numel()]
+    if any(same) and not all(same):
+        raise ValueError("the outputs are the inputs themselves, all of them or none")
+    return any(same)
+
+
+def fork_block_tables(lengths: torch.Tensor, parents: Optional[torch.Tensor], new_lengths, tables: torch.Tensor,
+                      shares: torch.Tensor, free: torch.Tensor, state: torch.Tensor, block_size: int, max_tokens: int,
+                      *, out: Optional[Sequence] = None, workspace: Optional[torch.Tensor] = None,
+                      check: Optional[bool] = None, err: Optional[torch.Tensor] = None) -> ForkUpdate:
+    """Block tables whose rows may share blocks: row r becomes the first tokens of row parents[r]
+    and grows from there, all rows at once.  This forks a request (several rows of one parent),
+    reorders beams, takes over a prefix, lets rows join and end, and frees what no row holds any more.
+
+    lengths      int32 [R <= 4096]: tokens of each row, in ceil(n / block_size) blocks
+    parents      int32 [R]: the row that each goes on from, -1 for one that starts empty; None:
+                 every row itself
+    new_lengths  int32 [R]: tokens after the call; min(new, the parent's) of them are the
+                 parent's.  Or an integer: that many more than the parent has, and no tokens where there
+                 is no parent
+    tables       int32 [R, columns]; rows that share a block have it in the same column
+    shares       int32 [blocks]: how many rows hold a block besides the first
+    free, state  the ring of free blocks, int32 [blocks], and its head and count, as in
+                 `build_block_tables`; `free` is changed in place
+
+    Whole blocks of kept tokens are shared.  A partly kept one goes on with a single row, where no
+    other holds it; the other rows take a block for these tokens, and `copies` lists (from, to,
+    tokens): `copy_blocks` has to run on them before the new tokens are written.  Blocks that no row
+    holds any more go behind the ring's last free one, in the order of their ids.
+
+    All or nothing: with too few free blocks the call raises RuntimeError where it checks, with more
+    than `max_tokens` new tokens or a length or parent out of range ValueError; rows and ring are
+    then as they were, slots and copies -1.
+
+    `out`: the tensors of a `ForkUpdate` to write into; tables, lengths, shares and state may be the
+    inputs themselves, all four.  `workspace`: of `fork_workspace` (made here if not given)."""
+    if type(out) is tuple:
+        out = ForkUpdate(*out)
+    if type(out) is ForkUpdate and workspace is not None and _unchecked(check) and _calls.fork_block_tables(
+            lengths, parents, new_lengths, tables, shares, free, state, block_size, max_tokens, out, workspace, err):
+        return out
+    _sizes(block_size=block_size)
+    if type(max_tokens) is not int or not 0 <= max_tokens <= _INT32_MAX:
+        raise ValueError("max_tokens must be a nonnegative integer in 31 bits")
+    now = _tensor(lengths, "lengths", torch.int32, (None,))
+    dev, R = lengths.device, lengths.numel()
+    from_rows = None if parents is None else _tensor(parents, "parents", torch.int32, (R,), dev)
+    new, grow = None, 0
+    if type(new_lengths) is int:
+        grow = new_lengths
+        if not 0 <= grow <= _INT32_MAX:
+            raise ValueError("new_lengths must be a tensor, or a nonnegative integer in 31 bits")
+    else:
+        new = _tensor(new_lengths, "new_lengths", torch.int32, (R,), dev)
+    tab = _tensor(tables, "tables", torch.int32, (R, None), dev)
+    counts = _tensor(shares, "shares", torch.int32, (None,), dev)
+    N, C = shares.numel(), tables.shape[1]
+    ring = _tensor(free, "free", torch.int32, (N,), dev)
+    st = _tensor(state, "state", torch.int32, (2,), dev)
+    if R > 4096:
+        raise ValueError("fork_block_tables takes up to 4096 rows")
+    if out is None:
+        made = torch.empty(5 * R + 3 + N, dtype=torch.int32, device=dev)
+        out = ForkUpdate(torch.empty_like(tables), made[:R], made[5 * R + 3:], made[R:R + 2],
+                         torch.empty(max_tokens, dtype=torch.int64, device=dev), made[R + 2:2 * R + 3],
+                         made[2 * R + 3:5 * R + 3].view(R, 3))
+    else:
+        out = ForkUpdate(*out)
+        for name, t, like in (("out.tables", out.tables, (R, C)), ("out.lengths", out.lengths, (R,)),
+                              ("out.shares", out.shares, (N,)), ("out.state", out.state, (2,)),
+                              ("out.starts", out.starts, (R + 1,)), ("out.copies", out.copies, (R, 3))):
+            _tensor(t, name, torch.int32, like, dev)
+        _tensor(out.slots, "out.slots", torch.int64, (max_tokens,), dev)
+    in_place = _in_place(((out.tables, tables), (out.lengths, lengths), (out.shares, shares), (out.state, state)))
+    if R and out.lengths.data_ptr() in (new, from_rows):
+        raise ValueError("out.lengths must be neither new_lengths nor parents")
+    call = _Call(dev, check, err)
+    if R == 0:
+        if not in_place:
+            out.shares.copy_(shares)
+            out.state.copy_(state)
+        out.slots.fill_(-1)
+        out.starts.zero_()
+        return out
+    if N == 0 or C == 0:
+        raise ValueError("the pool and the rows of the tables must not be empty")
+    space = _space(workspace, _lib.load().kvmi_fork_workspace_bytes(N, R, C), dev)
+    args = _lib.ForkArgs(now, from_rows, new, tab, counts, ring, st, out.tables.data_ptr(), out.lengths.data_ptr(),
+                         out.shares.data_ptr(), out.state.data_ptr(), out.slots.data_ptr(), out.starts.data_ptr(),
+                         out.copies.data_ptr(), space.data_ptr(), space.numel() * 4, call.err_ptr, R, C, N, block_size,
+                         max_tokens, grow)
+    call.run("kvmi_fork_tables", args)
+    return out
+
+
+def copy_blocks(caches, copies: torch.Tensor, *, check: Optional[bool] = None,
+                err: Optional[torch.Tensor] = None) -> None:
+    """Copy blocks in every layer (`LayerCaches`, or a sequence of caches): for each row (from, to,
+    tokens) of `copies`, int32 [n, 3], the first `tokens` tokens of block `from`, keys and values, go to
+    block `to`.  Rows with a negative `from` are skipped.  No block may be written by two rows, nor
+    read by one and written by another.  A row with a block outside the cache, or more tokens than a
+    block has, copies nothing."""
+    layers = caches if isinstance(caches, LayerCaches) else LayerCaches(caches)
+    if _unchecked(check) and _calls.copy_blocks(layers._struct_at, layers.bases, copies, err):
+        return
+    rows = _tensor(copies, "copies", torch.int32, (None, 3), layers.device)
+    call = _Call(layers.device, check, err)
+    if copies.shape[0]:
+        call.run("kvmi_copy_blocks", layers.struct, layers.bases.data_ptr(), len(layers.caches), rows,
+                 copies.shape[0], call.err_ptr)
+
+
+class Compaction(NamedTuple):
+    """What `compact_block_tables` gives back."""
+
+    tables: torch.Tensor  # int32 [R, columns]
+    shares: torch.Tensor  # int32 [blocks]
+    free: torch.Tensor    # int32 [blocks]: the ring, from 0 on, -1 behind its last
+    state: torch.Tensor   # int32 [2]: 0 and the ring's count
+    copies: torch.Tensor  # int32 [blocks // 2, 3]: the moves, for `copy_blocks`
+
+
+def compact_block_tables(lengths: torch.Tensor, tables: torch.Tensor, shares: torch.Tensor, free: torch.Tensor,
+                         state: torch.Tensor, block_size: int, *, out: Optional[Sequence] = None,
+                         workspace: Optional[torch.Tensor] = None, check: Optional[bool] = None,
+                         err: Optional[torch.Tensor] = None) -> Compaction:
+    """Move the blocks that rows hold to the front of the pool.  Arguments as in
+    `fork_block_tables`.  The pool is what the rows hold and what the ring has free (a block in
+    neither stays out of it); of n held blocks those among the pool's n lowest ids stay, and the others
+    move, in order, to the free ids among these n.  Tables and shares come back under the new names, the
+    ring with the rest of the pool in order, and `copies` with the moves: `copy_blocks` has to run on
+    them before the blocks are read or handed out.
+
+    `out`: the tensors of a `Compaction` to write into; tables, shares, free and state may be the
+    inputs themselves, all four.  `workspace`: of `compact_workspace` (made here if not given)."""
+    if type(out) is tuple:
+        out = Compaction(*out)
+    if type(out) is Compaction and workspace is not None and _unchecked(check) and _calls.compact_block_tables(
+            lengths, tables, shares, free, state, block_size, out, workspace, err):
+        return out
+    _sizes(block_size=block_size)
+    now = _tensor(lengths, "lengths", torch.int32, (None,))
+    dev, R = lengths.device, lengths.numel()
+    tab = _tensor(tables, "tables", torch.int32, (R, None), dev)
+    counts = _tensor(shares, "shares", torch.int32, (None,), dev)
+    N, C = shares.numel(), tables.shape[1]
+    ring = _tensor(free, "free", torch.int32, (N,), dev)
+    st = _tensor(state, "state", torch.int32, (2,), dev)
+    if out is None:
+        out = Compaction(torch.empty_like(tables), torch.empty_like(shares), torch.empty_like(free),
+                         torch.empty_like(state), torch.empty((N // 2, 3), dtype=torch.int32, device=dev))
+    else:
+        out = Compaction(*out)
+        for name, t, like in (("out.tables", out.tables, (R, C)), ("out.shares", out.shares, (N,)),
+                              ("out.free", out.free, (N,)), ("out.state", out.state, (2,)),
+                              ("out.copies", out.copies, (N // 2, 3))):
+            _tensor(t, name, torch.int32, like, dev)
+    _in_place(((out.tables, tables), (out.shares, shares), (out.free, free), (out.state, state)))
+    if N == 0 or C == 0:
+        raise ValueError("the pool and the rows of the tables must not be empty")
+    space = _space(workspace, _lib.load().kvmi_compact_workspace_bytes(N), dev)
+    call = _Call(dev, check, err)
+    args = _lib.CompactArgs(now, tab, counts, ring, st, out.tables.data_ptr(), out.shares.data_ptr(),
+                            out.free.data_ptr(), out.state.data_ptr(), out.copies.data_ptr(), space.data_ptr(),
+                            space.numel() * 4, call.err_ptr, R, C, N, block_size)
+    call.run("kvmi_compact_tables", args)
+    return out
+
+
+class SharedBlockTables(BlockTables):
+    """`BlockTables` whose rows may share blocks: up to 4096 rows, several of which may belong to one
+    request.
+
+      shares  int32 [num_blocks]: how many rows hold a block besides the first
+      copies  int32 [requests, 3]: the blocks that the last `fork` or `update` split; `copy_blocks` on
+              them comes before the new tokens are written
+
+    Rewritten in place like the others."""
+
+    def __init__(self, num_blocks: int, block_size: int, requests: int, columns: int, device="cuda",
+                 free_blocks: Optional[Iterable[int]] = None):
+        super().__init__(num_blocks, block_size, requests, columns, device, free_blocks)
+        if requests > 4096:
+            raise ValueError("SharedBlockTables takes up to 4096 rows")
+        i32 = dict(dtype=torch.int32, device=self.tables.device)
+        self.shares = torch.zeros(num_blocks, **i32)
+        self.copies = torch.full((requests, 3), -1, **i32)
+        self._moves = torch.full((num_blocks // 2, 3), -1, **i32)
+        self._fork_space = fork_workspace(num_blocks, requests, columns, self.tables.device)
+        self._compact_space = compact_workspace(num_blocks, self.tables.device)
+
+    def fork(self, parents: Optional[torch.Tensor], new_lengths, max_tokens: int, *,
+             slots: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None,
+             check: Optional[bool] = None, err: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Row r becomes the first tokens of row parents[r] (int32 [requests]; -1: it starts empty)
+        and grows to new_lengths[r] tokens, or, where that is an integer, by so many.  Returns (slots,
+        starts) of the new tokens, at most `max_tokens`, and leaves in `copies` what `copy_blocks` has
+        to copy before they are written; see `fork_block_tables`."""
+        dev = self.tables.device
+        if slots is None:
+            slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
+        if starts is None:
+            starts = torch.empty(self.lengths.numel() + 1, dtype=torch.int32, device=dev)
+        fork_block_tables(self.lengths, parents, new_lengths, self.tables, self.shares, self.free, self.state,
+                          self.block_size, max_tokens, out=(self.tables, self.lengths, self.shares, self.state, slots,
+                                                            starts, self.copies),
+                          workspace=self._fork_space, check=check, err=err)
+        return slots, starts
+
+    def update(self, new_lengths: torch.Tensor, max_tokens: int, *, slots: Optional[torch.Tensor] = None,
+               starts: Optional[torch.Tensor] = None, check: Optional[bool] = None,
+               err: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """`fork` with every row as its own parent.  A row that shrinks into a block that others
+        hold gets one of its own (`copies`)."""
+        return self.fork(None, new_lengths, max_tokens, slots=slots, starts=starts, check=check, err=err)
+
+    def compact(self, *, check: Optional[bool] = None, err: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Bring the held blocks to the front of the pool; returns the moves, int32
+        [num_blocks // 2, 3], on which `copy_blocks` has to run next (rewritten by the next call).  See
+        `compact_block_tables`."""
+        compact_block_tables(self.lengths, self.tables, self.shares, self.free, self.state, self.block_size,
+                             out=(self.tables, self.shares, self.free, self.state, self._moves),
+                             workspace=self._compact_space, check=check, err=err)
+        return self._moves
+
+
+# ------------------------------------------------------------------ beam search's selection
+_LOGITS = {**_DTYPES, torch.float32: _lib.DTYPE_FP32}
+
+
+class BeamChoice(NamedTuple):
+    """What `select_beams` gives back."""
+
+    parents: torch.Tensor      # int32 [requests * beams]: the row that each beam goes on from, -1: none
+    tokens: torch.Tensor       # int32 [requests * beams]
+    scores: torch.Tensor       # float32 [requests * beams]
+    all_parents: torch.Tensor  # int32 [requests, count]: the candidates, best first
+    all_tokens: torch.Tensor   # int32 [requests, count]
+    all_scores: torch.Tensor   # float32 [requests, count]
+
+
+def select_beams(logits: torch.Tensor, scores: torch.Tensor, beams: int, count: Optional[int] = None, *,
+                 end_token: Optional[int] = None, out: Optional[Sequence] = None, check: Optional[bool] = None,
+                 err: Optional[torch.Tensor] = None) -> BeamChoice:
+    """Beam search's step over the vocabulary: of each request's candidates (beam, token), with the value
+    scores[beam] + log_softmax(logits[beam])[token], the `count` best, and of these the `beams` best
+    that do not end.
+
+    logits     [requests * beams, vocabulary], bfloat16, float16 or float32, a request's beams one
+               after the other; any row stride, tokens adjacent
+    scores     float32 [requests * beams]: sums of log-probabilities so far; -inf for a beam that is not
+               in use (its logits are not read)
+    count      beams <= count <= 64 candidates a request; default: beams, or with an end token twice that
+    end_token  candidates with this token are listed, but do not go on
+
+    Values are in 64 bits until their last rounding; among equal ones the lower beam comes first, then
+    the larger logit, then the lower token.  A value of -inf is no candidate: behind the last stand
+    parent and token -1 and score -inf.  So `parents` is what `fork_block_tables` takes: a row without
+    one gives its blocks back.  A beam with NaN or +inf in its score or logits has no candidates, and
+    the call raises ValueError where it checks.  No gradient flows back.
+
+    `out`: the tensors of a `BeamChoice` to write into."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise TypeError("logits must be a CUDA tensor")
+    if type(beams) is not int or not 1 <= beams <= 64:
+        raise ValueError("beams must be an integer in [1, 64]")
+    if count is None:
+        count = min(2 * beams, 64) if end_token is not None else beams
+    if type(out) is tuple:
+        out = BeamChoice(*out)
+    if type(out) is BeamChoice and _unchecked(check) and _calls.select_beams(logits, scores, beams, count, end_token,
+                                                                            out, err):
+        return out
+    if type(count) is not int or not beams <= count <= 64:
+        raise ValueError("count must be an integer in [beams, 64]")
+    if logits.dtype not in _LOGITS:
+        raise TypeError("logits must be a bfloat16, float16 or float32 tensor")
+    if logits.dim() != 2 or logits.shape[0] % beams or not 1 <= logits.shape[1] <= _INT32_MAX:
+        raise ValueError(f"logits must have shape (a multiple of {beams}, vocabulary), not {tuple(logits.shape)}")
+    n, V = logits.shape
+    if n > 65535:
+        raise ValueError("select_beams takes up to 65535 rows")
+    if V > 1 and logits.stride(1) != 1:
+        raise ValueError("a row's logits must be adjacent")
+    if end_token is None:
+        end = -1
+    elif type(end_token) is int and 0 <= end_token <= _INT32_MAX:
+        end = end_token
+    else:
+        raise ValueError("end_token must be a nonnegative integer, or None")
+    dev, R = logits.device, n // beams
+    before = _tensor(scores, "scores", torch.float32, (n,), dev)
+    if out is None:
+        whole = torch.empty(2 * n + 2 * R * count, dtype=torch.int32, device=dev)
+        real = torch.empty(n + R * count, dtype=torch.float32, device=dev)
+        out = BeamChoice(whole[:n], whole[n:2 * n], real[:n], whole[2 * n:2 * n + R * count].view(R, count),
+                         whole[2 * n + R * count:].view(R, count), real[n:].view(R, count))
+    else:
+        out = BeamChoice(*out)
+        for name, t, dtype, like in (("out.parents", out.parents, torch.int32, (n,)),
+                                     ("out.tokens", out.tokens, torch.int32, (n,)),
+                                     ("out.scores", out.scores, torch.float32, (n,)),
+                                     ("out.all_parents", out.all_parents, torch.int32, (R, count)),
+                                     ("out.all_tokens", out.all_tokens, torch.int32, (R, count)),
+                                     ("out.all_scores", out.all_scores, torch.float32, (R, count))):
+            _tensor(t, name, dtype, like, dev)
+    call = _Call(dev, check, err)
+    if n == 0:
+        return out
+    args = _lib.SelectArgs(logits.data_ptr(), before, *(t.data_ptr() for t in out), None, 0, call.err_ptr,
+                           logits.stride(0), _LOGITS[logits.dtype], R, beams, V, count, end)
+    size = _lib.load().kvmi_select_workspace_bytes(args)
+    if size < 0:
+        raise ValueError("kvmi_select_beams: invalid arguments (KVMI_EINVAL)")
+    space = torch.empty(size, dtype=torch.uint8, device=dev)
+    args.workspace, args.workspace_bytes = space.data_ptr(), size
+    call.run("kvmi_select_beams", args)
     return out
