@@ -718,7 +718,7 @@ int kvmi_compact_tables(const kvmi_compact_args* args, kvmi_stream_t stream);
  * and the `count` largest of a request are found; among equal ones the lower row comes first, then the
  * larger logit, then the lower token.  Sums and values are in 64 bits.  A value of -inf (after its
  * rounding to fp32) is no candidate, nor is anything in a row whose score or sum is not finite; NaN
- * or +inf there sets KVMI_ERR_NOT_FINITE, but for rows whose score is -inf, which are not read.
+ * or +inf there sets KVMI_ERR_NOT_FINITE, but for rows whose score is -inf, whose logits do not matter.
  *   all_parents, all_tokens (int32), all_scores (fp32)  [requests][count] the candidates, best first:
  *                  row, token, value; behind the last -1, -1, -inf
  *   parents, tokens (int32), scores (fp32)  [requests * beams] those that go on: of each request the

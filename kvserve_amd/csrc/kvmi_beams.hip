@@ -8,8 +8,9 @@ namespace kvmi {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kMostCount = 64;  // the lanes of a wave: their largest values bound the count-th
-constexpr int kRoom = 1024;     // candidates that a workgroup ranks at once
+constexpr int kMostCount = 64;  // (a lane each, where the best are listed)
+constexpr int kVectors = 128;   // of 16 bytes, in which a tile's candidates are looked for; at least kMostCount
+constexpr int kRoom = 8 * kVectors;  // candidates that are ranked at once
 constexpr double kFar = 600.0;  // logits up to here are summed as they are: exp(600) times any vocabulary is finite
 
 template <class T>
@@ -17,50 +18,64 @@ struct Logits;
 template <>
 struct Logits<__bf16> {
   static constexpr int kVec = 8;
-  static __device__ __forceinline__ float at(const uint4& v, int i) {
-    const uint32_t u = (&v.x)[i >> 1];
-    return i & 1 ? bf_hi(u) : bf_lo(u);
+  static __device__ __forceinline__ float at(const u32x4v& v, int i) {
+    return of(v[i >> 1], i);
   }
   static __device__ __forceinline__ uint32_t bits(const void* row, int64_t i) { return gld((const uint16_t*)row + i); }
+  static __device__ __forceinline__ float of(uint32_t word, int i) { return i & 1 ? bf_hi(word) : bf_lo(word); }
   static constexpr uint32_t kNone = 0xff80;  // -inf
+  static constexpr int kZeros = 16;          // bits at the end of a value in 32 bits that are all alike
 };
 template <>
 struct Logits<_Float16> {
   static constexpr int kVec = 8;
-  static __device__ __forceinline__ float at(const uint4& v, int i) {
-    const uint32_t u = (&v.x)[i >> 1];
-    return (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? u >> 16 : u));
+  static __device__ __forceinline__ float at(const u32x4v& v, int i) {
+    return of(v[i >> 1], i);
   }
   static __device__ __forceinline__ uint32_t bits(const void* row, int64_t i) { return gld((const uint16_t*)row + i); }
+  static __device__ __forceinline__ float of(uint32_t word, int i) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? word >> 16 : word));
+  }
   static constexpr uint32_t kNone = 0xfc00;
+  static constexpr int kZeros = 13;
 };
 template <>
 struct Logits<float> {
   static constexpr int kVec = 4;
-  static __device__ __forceinline__ float at(const uint4& v, int i) { return __uint_as_float((&v.x)[i]); }
+  static __device__ __forceinline__ float at(const u32x4v& v, int i) { return __uint_as_float(v[i]); }
   static __device__ __forceinline__ uint32_t bits(const void* row, int64_t i) { return gld((const uint32_t*)row + i); }
+  static __device__ __forceinline__ float of(uint32_t word, int) { return __uint_as_float(word); }
   static constexpr uint32_t kNone = 0xff800000;
+  static constexpr int kZeros = 0;
 };
 
 // A vector of a row of V logits that begins at element e; outside the row -inf, and nothing is read
 // there.
 template <class T>
-__device__ __forceinline__ uint4 load_logits(const void* row, int64_t e, int64_t V) {
+__device__ __forceinline__ u32x4v load_logits(const void* row, int64_t e, int64_t V) {
   using L = Logits<T>;
-  if (e >= 0 && e + L::kVec <= V) return gld((const uint4*)((const T*)row + e));
-  uint4 v;
+  if (e >= 0 && e + L::kVec <= V) return gld((const u32x4v*)((const T*)row + e));
+  u32x4v v;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
     if constexpr (L::kVec == 4) {
-      (&v.x)[w] = e + w >= 0 && e + w < V ? L::bits(row, e + w) : L::kNone;
+      v[w] = e + w >= 0 && e + w < V ? L::bits(row, e + w) : L::kNone;
     } else {
       const int64_t a = e + 2 * w;
       const uint32_t lo = a >= 0 && a < V ? L::bits(row, a) : L::kNone;
       const uint32_t hi = a + 1 >= 0 && a + 1 < V ? L::bits(row, a + 1) : L::kNone;
-      (&v.x)[w] = lo | hi << 16;
+      v[w] = lo | hi << 16;
     }
   }
   return v;
+}
+
+// What was unpacked of these vectors is unpacked anew behind this: kept in registers it would halve
+// the waves of a SIMD.
+template <int N>
+__device__ __forceinline__ void forget(u32x4v (&x)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) asm volatile("" : "+v"(x[j]));
 }
 
 // exp(x) for |x| <= 700: 2^(n + r), n whole and |r| <= 1/2, with a polynomial of degree 7 for 2^r
@@ -80,33 +95,62 @@ __device__ __forceinline__ double exp_near(double x) {
   p = __builtin_fma(p, r, 0x1.ebfbe0a4be818p-3);
   p = __builtin_fma(p, r, 0x1.62e42ff116290p-1);
   p = __builtin_fma(p, r, 0x1.ffffffffabbcdp-1);
-  const uint64_t bits = __builtin_bit_cast(uint64_t, p);
-  const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, t);
-  return __builtin_bit_cast(double, (uint64_t)((uint32_t)(bits >> 32) + (n << 20)) << 32 | (uint32_t)bits);
+  // 2^n: n added to the exponent, in the upper word alone
+  const u32x2v t_words = __builtin_bit_cast(u32x2v, t);
+  u32x2v words = __builtin_bit_cast(u32x2v, p);
+  words.y += t_words.x << 20;
+  return __builtin_bit_cast(double, words);
 }
 
 // The order of floats as that of unsigned words; zeros are one.
 __device__ __forceinline__ uint32_t order_of(float x) { return f2key(x + 0.0f); }
 
-// The largest of the wave, NaN if one is NaN, in every lane.
-__device__ __forceinline__ float wave_maximum(float x) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) x = __builtin_elementwise_maximum(x, __shfl_xor(x, d, 64));
-  return x;
+// The wave's reductions go from row to row of 16 lanes in registers (10 cycles a step where an exchange
+// over the LDS takes 60) and end in lane 63.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t from_lane(uint32_t mine, uint32_t none) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)mine, CTRL, ROWS, 0xf, false);
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float maximum_with(float x) {
+  return __builtin_elementwise_maximum(x, __uint_as_float(from_lane<CTRL, ROWS>(__float_as_uint(x), __float_as_uint(x))));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double sum_with(double x) {
+  const u32x2v w = __builtin_bit_cast(u32x2v, x);
+  const u32x2v other = {from_lane<CTRL, ROWS>(w.x, 0), from_lane<CTRL, ROWS>(w.y, 0)};
+  return x + __builtin_bit_cast(double, other);
+}
+// The largest of the wave, NaN if one is NaN.
+__device__ __forceinline__ float wave_maximum(float x) {
+  x = maximum_with<0x111, 0xf>(x);  // the lane 1, 2, 4, 8 before in the row
+  x = maximum_with<0x112, 0xf>(x);
+  x = maximum_with<0x114, 0xf>(x);
+  x = maximum_with<0x118, 0xf>(x);
+  x = maximum_with<0x142, 0xa>(x);  // the last lane of the row before, of the half before
+  x = maximum_with<0x143, 0xc>(x);
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
+}
+// The sum of the wave, in lane 63.
 __device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d, 64);
-  return x;
+  x = sum_with<0x111, 0xf>(x);
+  x = sum_with<0x112, 0xf>(x);
+  x = sum_with<0x114, 0xf>(x);
+  x = sum_with<0x118, 0xf>(x);
+  x = sum_with<0x142, 0xa>(x);
+  return sum_with<0x143, 0xc>(x);
 }
 
-// A word that at least `count` of the wave's 64 lanes hold or exceed, near the count-th largest: as
-// soon as exactly `count` do.
-__device__ __forceinline__ uint32_t wave_bound(uint32_t key, int count) {
-  uint32_t lo = 0, hi = 0xffffffffu;  // `count` lanes are at lo or more; fewer at hi
+// A word that at least `count` of N words a lane reach, near the count-th largest: as soon as exactly
+// `count` do.  No word is above `most`.
+template <int N>
+__device__ __forceinline__ uint32_t wave_bound(const uint32_t (&key)[N], int count, uint32_t most) {
+  uint32_t lo = 0, hi = most + 1;  // `count` are at lo or more; fewer at hi
   while (hi - lo > 1) {
     const uint32_t mid = lo + (hi - lo) / 2;
-    const int n = __popcll(__ballot(key >= mid));
+    int n = 0;
+#pragma unroll
+    for (int x = 0; x < N; ++x) n += __popcll(__ballot(key[x] >= mid));
     if (n >= count) lo = mid;
     if (n < count) hi = mid;
     if (n == count) break;
@@ -139,31 +183,41 @@ struct SelectArgs {
 };
 
 // Workgroup (tile, row): NV vectors a thread, all of them in registers: their sum of exp, and the
-// `count` best.  At least `count` elements reach the count-th largest of a wave's 64 largest (one a
-// lane), so those below it cannot be among the best; the few that reach it, by the waves' highest
-// such bound, are ranked against each other.  Where too many do (ties, or large ones in few
-// lanes) the count-th largest itself is found by bisection.
+// `count` best.  At least `count` elements reach the count-th largest of the threads' 256 largest, so
+// those below it cannot be among the best; the few that reach it are ranked against each other.
+// Where too many do (ties, or large ones in few threads) the count-th largest itself is found by
+// bisection.
 template <class T, int NV>
 __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
   using L = Logits<T>;
   constexpr int VEC = L::kVec;
   __shared__ uint64_t best[kRoom];
   __shared__ double part_sum[kWaves], part_at[kWaves];
-  __shared__ uint32_t bounds[kWaves];
-  __shared__ int found, scan[kWaves];
+  __shared__ uint32_t tops[kThreads];
+  __shared__ u32x4v hit[kVectors];
+  __shared__ int hit_at[kVectors];
+  __shared__ int found, vectors, scan[kWaves];
   const int tid = threadIdx.x, wave = tid >> 6, tile = blockIdx.x, count = s.a.count;
   const int64_t row = blockIdx.y, V = s.a.vocab;
-  // a row whose score is not finite has no candidates
+  // a row whose score is not finite has no candidates, and is not read but where a call is so small
+  // that one load after the other would be its time
   const float score = gld(s.a.scores + row);
-  if (!(__builtin_fabsf(score) < INFINITY)) return;
+  if (NV > 1 && !(__builtin_fabsf(score) < INFINITY)) return;
   const T* const logits = (const T*)s.a.logits + row * s.a.row_stride;
   // vectors lie on 16-byte places, whatever the row's
   const int64_t shift = (int64_t)((uintptr_t)logits % 16 / sizeof(T));
   const int64_t first = (int64_t)tile * (kThreads * NV * VEC) - shift;
-  uint4 x[NV];
+  u32x4v x[NV];
+  if (first >= 0 && first + kThreads * NV * VEC <= V) {
+    const u32x4v* const from = (const u32x4v*)(logits + first) + tid;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) x[j] = load_logits<T>(logits, first + (int64_t)(j * kThreads + tid) * VEC, V);
-  if (tid == 0) found = 0;
+    for (int j = 0; j < NV; ++j) x[j] = gld(from + j * kThreads);
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) x[j] = load_logits<T>(logits, first + (int64_t)(j * kThreads + tid) * VEC, V);
+  }
+  if (NV == 1 && !(__builtin_fabsf(score) < INFINITY)) return;
+  if (tid == 0) found = vectors = 0;
 
   float top[NV], lane_top = -INFINITY;
   double sum = 0.0;
@@ -174,8 +228,9 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
     for (int i = 1; i < VEC; ++i) top[j] = __builtin_elementwise_maximum(top[j], L::at(x[j], i));
     lane_top = __builtin_elementwise_maximum(lane_top, top[j]);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sum += exp_near((double)fmaxf(L::at(x[j], i), -700.0f));
+    for (int i = 0; i < VEC; ++i) sum += exp_near((double)__builtin_elementwise_maximum(L::at(x[j], i), -700.0f));
   }
+  forget(x);
   const float high = wave_maximum(lane_top);
   double at = 0.0;
   if (!(__builtin_fabsf(high) <= (float)kFar)) {
@@ -195,15 +250,17 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
     }
   }
   sum = wave_sum(sum);
-  if ((tid & 63) == 0) {
+  if ((tid & 63) == 63) {
     part_sum[wave] = sum;
     part_at[wave] = at;
   }
-  const uint32_t floor = order_of(-INFINITY) + 1;  // -inf is no candidate
-  const uint32_t wave_low = wave_bound(order_of(lane_top), count);
-  if ((tid & 63) == 0) bounds[wave] = max(wave_low, floor);
+  tops[tid] = order_of(lane_top) >> L::kZeros;
   __syncthreads();
-  uint32_t bound = max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3]));
+  uint32_t all_tops[kWaves];
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) all_tops[w] = tops[w * 64 + (tid & 63)];
+  const uint32_t bound = max(wave_bound(all_tops, count, 0xfffffffeu >> L::kZeros) << L::kZeros,
+                             order_of(-INFINITY) + 1);  // -inf is no candidate
   if (tid == 0) {
     const double m = fmax(fmax(part_at[0], part_at[1]), fmax(part_at[2], part_at[3]));
     double all = 0.0;
@@ -215,35 +272,45 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
   auto token_of = [&](int j, int i) { return (uint32_t)(first + (int64_t)(j * kThreads + tid) * VEC + i); };
   auto keep = [&](float v, uint32_t token) {
     const int n = atomicAdd(&found, 1);
-    if (n < kRoom) best[n] = (uint64_t)order_of(v) << 32 | (uint32_t)~token;
+    best[n] = (uint64_t)order_of(v) << 32 | (uint32_t)~token;
   };
+  // the vectors that reach the bound, then their elements, spread over the threads
 #pragma unroll
   for (int j = 0; j < NV; ++j)
     if (top[j] >= least) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (L::at(x[j], i) >= least) keep(L::at(x[j], i), token_of(j, i));
+      const int n = atomicAdd(&vectors, 1);
+      if (n < kVectors) {
+        hit[n] = x[j];
+        hit_at[n] = j * kThreads + tid;
+      }
     }
   __syncthreads();
-  if (found > kRoom) {
+  const int hits = vectors;
+  if (hits <= kVectors)
+    for (int i = tid; i < hits * VEC; i += kThreads) {
+      const float v = L::of(((const uint32_t*)hit)[i * (int)sizeof(T) / 4], i);
+      if (v >= least) keep(v, (uint32_t)(first + (int64_t)hit_at[i / VEC] * VEC + i % VEC));
+    }
+  __syncthreads();
+  if (hits > kVectors) {
     // the count-th largest: at least `count` elements are at lo or more, fewer at hi
     uint32_t lo = bound, hi = 0xffffffffu;
     while (hi - lo > 1) {
       const uint32_t mid = lo + (hi - lo) / 2;
+      const float at_mid = key2f(mid);  // (NaN past +inf: nothing reaches it)
       int n = 0, all;
+      forget(x);
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) n += order_of(L::at(x[j], i)) >= mid;
+        for (int i = 0; i < VEC; ++i) n += L::at(x[j], i) >= at_mid;
       before_in_block(n, scan, &all);
       if (all >= count)
         lo = mid;
       else
         hi = mid;
     }
-    __syncthreads();
-    if (tid == 0) found = 0;
-    __syncthreads();
+    forget(x);
     // fewer than `count` above it, and of those at it the first ones
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -252,6 +319,7 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
         if (order_of(L::at(x[j], i)) > lo) keep(L::at(x[j], i), token_of(j, i));
     __syncthreads();
     int left = count - found;
+    forget(x);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -268,102 +336,151 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
   }
   const int n = found;
   uint64_t* const out = s.keys + (row * s.tiles + tile) * count;
-  for (int i = tid; i < n; i += kThreads) {
-    const uint64_t mine = best[i];
+  int parts = 1;  // lanes that rank one candidate
+  while (parts < 16 && 2 * parts * n <= kThreads) parts *= 2;
+  for (int i0 = 0; i0 < n; i0 += kThreads / parts) {
+    const int i = i0 + tid / parts;
+    const uint64_t mine = best[min(i, n - 1)];
     int rank = 0;
-    for (int k = 0; k < n; ++k) rank += best[k] > mine;
-    if (rank < count) gst(out + rank, mine);
+    for (int k = tid % parts; k < n; k += parts) rank += best[k] > mine;
+    for (int d = parts / 2; d; d /= 2) rank += __shfl_xor(rank, d, 64);
+    if (i < n && tid % parts == 0 && rank < count) gst(out + rank, mine);
   }
   for (int i = n + tid; i < count; i += kThreads) gst(out + i, (uint64_t)0);
 }
 
-struct Candidate {
-  double value;
-  uint64_t key;  // (order, ~token)
-  int beam;
+// The sum of a row's exponentials as s exp(m), and two of them together.
+struct Sum {
+  double s, m;
 };
-// Whether a comes before b.
-__device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
-  if (a.value != b.value) return a.value > b.value;
-  return a.beam != b.beam ? a.beam < b.beam : a.key > b.key;
+__device__ __forceinline__ Sum join(const Sum& a, const Sum& b) {
+  if (a.m == b.m) return Sum{a.s + b.s, a.m};
+  const double m = fmax(a.m, b.m);  // (a sum at -inf is 0)
+  return Sum{(a.m == m ? a.s : a.m == -INFINITY ? 0.0 : a.s * exp(a.m - m)) +
+                 (b.m == m ? b.s : b.m == -INFINITY ? 0.0 : b.s * exp(b.m - m)),
+             m};
 }
 
-// Workgroup: a request.  The rows' sums of all tiles, then the tiles' best, 1024 at a time with the
+constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64, kEach = 4, kRound = kEach * kJoinThreads;
+
+// Workgroup: a request.  The rows' sums of all tiles, then the tiles' best, kRound at a time with the
 // best so far: those below the count-th largest of 64 lanes' best, or below the count-th so far, drop
-// out, the others are ranked against each other.
-__global__ __launch_bounds__(kThreads) void select_join_kernel(SelectArgs s) {
-  constexpr int kEach = 4, kRound = kEach * kThreads;
-  __shared__ Candidate list[kRound + kMostCount], best[kMostCount];
-  __shared__ double lse[kMostCount];
-  __shared__ uint32_t bounds[kWaves];
+// out, the others are ranked against each other, each by several lanes where they are few.  A chain
+// of loads and of barriers: the first round's keys are on their way while the sums are made.
+__global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs s) {
+  struct Candidates {
+    double value[kRound + kMostCount];
+    uint64_t key[kRound + kMostCount];  // (order, ~token)
+    uint8_t beam[kRound + kMostCount];
+  };
+  __shared__ Candidates list;
+  __shared__ double best_value[kMostCount], lse[kMostCount];
+  __shared__ uint64_t best_key[kMostCount];
+  __shared__ uint8_t best_beam[kMostCount];
+  __shared__ uint32_t bounds[kJoinWaves];
+  __shared__ float scores[kMostCount];
   __shared__ int found;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = blockIdx.x;
   const int B = s.a.beams, count = s.a.count, tiles = s.tiles;
-  for (int b = wave; b < B; b += kWaves) {
+  const int per_beam = tiles * count, all = B * per_beam;  // (at most 64 * 64 * tiles: select_ok)
+  const uint64_t* const keys = s.keys + (int64_t)r * all;
+  uint64_t key[kEach];
+#pragma unroll
+  for (int x = 0; x < kEach; ++x) key[x] = x * kJoinThreads + tid < all ? gld(keys + x * kJoinThreads + tid) : 0;
+
+  // log-sums: `group` lanes a row
+  int group = 1;
+  while (group < tiles && group < 64) group *= 2;
+  if (tid == 0) found = 0;
+  for (int b = tid / group; b < B; b += kJoinThreads / group) {
     const int64_t row = (int64_t)r * B + b;
     const float score = gld(s.a.scores + row);
-    double value = -INFINITY;
-    if (__builtin_fabsf(score) < INFINITY) {
-      double m = -INFINITY, sum = 0.0;
-      for (int t = lane; t < tiles; t += 64) m = fmax(m, s.sums[row * tiles + t].y);
-#pragma unroll
-      for (int d = 32; d; d >>= 1) m = fmax(m, __shfl_xor(m, d, 64));
-      for (int t = lane; t < tiles; t += 64) {
+    const bool used = __builtin_fabsf(score) < INFINITY;
+    Sum sum{0.0, -INFINITY};
+    if (used)
+      for (int t = tid % group; t < tiles; t += group) {
         const double2 p = s.sums[row * tiles + t];
-        sum += p.y == m ? p.x : p.y == -INFINITY ? 0.0 : p.x * exp(p.y - m);
+        sum = join(sum, Sum{p.x, p.y});
       }
-      sum = wave_sum(sum);
-      value = sum != sum ? (double)NAN : sum > 0.0 ? log(sum) + m : -INFINITY;
-    } else {
-      if (score != -INFINITY && lane == 0) flag_error(s.a.err, KVMI_ERR_NOT_FINITE);
+    for (int d = group / 2; d; d /= 2) sum = join(sum, Sum{__shfl_xor(sum.s, d, 64), __shfl_xor(sum.m, d, 64)});
+    if (tid % group == 0) {
+      const double value = sum.s != sum.s ? (double)NAN : sum.s > 0.0 ? log(sum.s) + sum.m : -INFINITY;
+      lse[b] = value;
+      scores[b] = score;
+      if (used ? value != value : score != -INFINITY) flag_error(s.a.err, KVMI_ERR_NOT_FINITE);
     }
-    if (value != value && lane == 0) flag_error(s.a.err, KVMI_ERR_NOT_FINITE);
-    if (lane == 0) lse[b] = value;
   }
-  if (tid == 0) found = 0;
   __syncthreads();
   int have = 0;
-  const int64_t per_beam = (int64_t)tiles * count, all = B * per_beam;
-  for (int64_t begin = 0; begin < all; begin += kRound) {
-    Candidate c[kEach];
+  for (int begin = 0; begin < all; begin += kRound) {
+    double value[kEach];
+    int beam[kEach];
     float top = -INFINITY;
 #pragma unroll
     for (int x = 0; x < kEach; ++x) {
-      const int64_t i = begin + x * kThreads + tid;
-      c[x].value = -INFINITY;
+      const int i = begin + x * kJoinThreads + tid;
+      value[x] = -INFINITY;
+      if (begin) key[x] = i < all ? gld(keys + i) : 0;
       if (i < all) {
-        c[x].beam = (int)(i / per_beam);
-        const double sum = lse[c[x].beam];
-        if (__builtin_fabs(sum) < INFINITY) {  // (else nothing was written)
-          c[x].key = gld(s.keys + r * all + i);
-          if (c[x].key) {
-            const double v = (double)gld(s.a.scores + (int64_t)r * B + c[x].beam) +
-                             ((double)key2f((uint32_t)(c[x].key >> 32)) - sum);
-            if ((float)v > -INFINITY) c[x].value = v;
-          }
+        beam[x] = i / per_beam;
+        const double sum = lse[beam[x]];
+        if (__builtin_fabs(sum) < INFINITY && key[x]) {  // (a row without a sum has no keys)
+          const double v = (double)scores[beam[x]] + ((double)key2f((uint32_t)(key[x] >> 32)) - sum);
+          if ((float)v > -INFINITY) value[x] = v;
         }
       }
-      top = fmaxf(top, (float)c[x].value);
+      top = fmaxf(top, (float)value[x]);
     }
-    const uint32_t floor = order_of(-INFINITY) + 1, low = wave_bound(order_of(top), count);
+    const uint32_t floor = order_of(-INFINITY) + 1, tops[1] = {order_of(top)}, low = wave_bound(tops, count, 0xfffffffeu);
     if (lane == 0) bounds[wave] = max(low, floor);
     __syncthreads();
-    uint32_t bound = max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3]));
-    if (have == count) bound = max(bound, order_of((float)best[count - 1].value));
+    uint32_t bound = have == count ? order_of((float)best_value[count - 1]) : floor;
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) bound = max(bound, bounds[w]);
 #pragma unroll
     for (int x = 0; x < kEach; ++x)
-      if (order_of((float)c[x].value) >= bound) list[atomicAdd(&found, 1)] = c[x];
+      if (order_of((float)value[x]) >= bound) {
+        const int at = atomicAdd(&found, 1);
+        list.value[at] = value[x];
+        list.key[at] = key[x];
+        list.beam[at] = (uint8_t)beam[x];
+      }
     __syncthreads();
-    const int fresh = found;
+    const int fresh = found, n = fresh + have;
     if (fresh) {
-      for (int i = tid; i < have; i += kThreads) list[fresh + i] = best[i];
+      if (tid < have) {
+        list.value[fresh + tid] = best_value[tid];
+        list.key[fresh + tid] = best_key[tid];
+        list.beam[fresh + tid] = best_beam[tid];
+      }
       __syncthreads();
-      const int n = fresh + have;
-      for (int i = tid; i < n; i += kThreads) {
-        const Candidate mine = list[i];
+      int parts = 1;  // lanes that rank one candidate
+      while (parts < 16 && 2 * parts * n <= kJoinThreads) parts *= 2;
+      for (int i0 = 0; i0 < n; i0 += kJoinThreads / parts) {
+        const int i = i0 + tid / parts;
         int rank = 0;
-        for (int k = 0; k < n; ++k) rank += before(list[k], mine);
-        if (rank < count) best[rank] = mine;
+        double mine = 0.0;
+        uint64_t my_key = 0;
+        int my_beam = 0;
+        if (i < n) {
+          mine = list.value[i];
+          my_key = list.key[i];
+          my_beam = list.beam[i];
+          for (int k = tid % parts; k < n; k += parts) {
+            const double other = list.value[k];
+            rank += other > mine;
+            if (other == mine && k != i) {  // the lower beam, then the larger logit, then the lower token
+              const int other_beam = list.beam[k];
+              rank += other_beam != my_beam ? other_beam < my_beam : list.key[k] > my_key;
+            }
+          }
+        }
+        for (int d = parts / 2; d; d /= 2) rank += __shfl_xor(rank, d, 64);
+        if (i < n && tid % parts == 0 && rank < count) {
+          best_value[rank] = mine;
+          best_key[rank] = my_key;
+          best_beam[rank] = (uint8_t)my_beam;
+        }
       }
       have = min(n, count);
     }
@@ -373,9 +490,9 @@ __global__ __launch_bounds__(kThreads) void select_join_kernel(SelectArgs s) {
   }
   if (wave) return;
   const bool there = lane < have;
-  const int64_t parent = there ? (int64_t)r * B + best[lane].beam : -1;
-  const int token = there ? (int)~(uint32_t)best[lane].key : -1;
-  const float value = there ? (float)best[lane].value : -INFINITY;
+  const int64_t parent = there ? (int64_t)r * B + best_beam[lane] : -1;
+  const int token = there ? (int)~(uint32_t)best_key[lane] : -1;
+  const float value = there ? (float)best_value[lane] : -INFINITY;
   if (lane < count) {
     const int64_t at = (int64_t)r * count + lane;
     gst(s.a.all_parents + at, (int32_t)parent);
@@ -400,7 +517,9 @@ __global__ __launch_bounds__(kThreads) void select_join_kernel(SelectArgs s) {
   }
 }
 
-// Vectors a thread: as many as leave the chip full.
+// Vectors a thread: as many as leave 384 workgroups, for what a tile does besides its sums costs the
+// same for any tile (32 rows x 4 beams x 131072: 21.9 us at 8 vectors, 25.6 at 4; 8 x 4: 13.9 at 4, 18.1
+// at 1; 13 x 5 x 50021: 15.0 at 2 in 845 workgroups, 17.0 at 8).
 struct Shape {
   int nv, tiles;
 };
@@ -408,15 +527,17 @@ inline Shape shape_of(const kvmi_select_args& a) {
   const int vec = a.dtype == KVMI_DTYPE_FP32 ? 4 : 8;
   Shape s;
   for (s.nv = 8; s.nv > 1; s.nv /= 2)
-    if ((int64_t)a.requests * a.beams * a.vocab >= 1024LL * kThreads * s.nv * vec) break;
+    if ((int64_t)a.requests * a.beams * a.vocab >= 384LL * kThreads * s.nv * vec) break;
   const int64_t tile = (int64_t)kThreads * s.nv * vec;
-  s.tiles = (int)((a.vocab + vec - 1 + tile - 1) / tile);  // (a row may begin inside a vector)
+  // rows may begin inside a vector
+  const bool whole = (uintptr_t)a.logits % 16 == 0 && a.row_stride % vec == 0;
+  s.tiles = (int)(((int64_t)a.vocab + (whole ? 0 : vec - 1) + tile - 1) / tile);
   return s;
 }
 bool select_ok(const kvmi_select_args& a) {
   return a.requests >= 0 && a.beams >= 1 && a.count >= a.beams && a.count <= kMostCount && a.vocab >= 1 &&
          a.vocab <= kMostPlaces && a.end_token >= -1 && a.row_stride >= 0 &&
-         (int64_t)a.requests * a.beams <= 65535 &&
+         (int64_t)a.requests * a.beams <= 65535 && (int64_t)a.beams * a.count * (a.vocab / 1024 + 2) <= 0x7fffffffLL - kRound &&
          (a.dtype == KVMI_DTYPE_BF16 || a.dtype == KVMI_DTYPE_FP16 || a.dtype == KVMI_DTYPE_FP32);
 }
 template <class T>
@@ -461,6 +582,6 @@ extern "C" int kvmi_select_beams(const kvmi_select_args* args, kvmi_stream_t str
     launch_tiles<_Float16>(s, shape.nv, st);
   else
     launch_tiles<float>(s, shape.nv, st);
-  hipLaunchKernelGGL(select_join_kernel, dim3((unsigned)a.requests), dim3(kThreads), 0, st, s);
+  hipLaunchKernelGGL(select_join_kernel, dim3((unsigned)a.requests), dim3(kJoinThreads), 0, st, s);
   return launched();
 }

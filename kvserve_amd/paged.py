@@ -744,7 +744,7 @@ def select_beams(logits: torch.Tensor, scores: torch.Tensor, beams: int, count: 
     logits     [requests * beams, vocabulary], bfloat16, float16 or float32, a request's beams one
                after the other; any row stride, tokens adjacent
     scores     float32 [requests * beams]: sums of log-probabilities so far; -inf for a beam that is not
-               in use (its logits are not read)
+               in use (its logits do not matter)
     count      beams <= count <= 64 candidates a request; default: beams, or with an end token twice that
     end_token  candidates with this token are listed, but do not go on
 
