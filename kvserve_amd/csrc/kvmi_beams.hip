@@ -141,19 +141,36 @@ __device__ __forceinline__ double wave_sum(double x) {
   return sum_with<0x143, 0xc>(x);
 }
 
-// A word that at least `count` of N words a lane reach, near the count-th largest: as soon as exactly
-// `count` do.  No word is above `most`.
+// Of 64 words, one a lane: the smallest of the largest of each 16 neighbours (`wide`), or of each 4.  So
+// many words as there are such groups reach it.
+__device__ __forceinline__ uint32_t least_of_groups(uint32_t x, bool wide) {
+  x = max(x, from_lane<0xb1, 0xf>(x, x));  // lanes 1, 2 away within four
+  x = max(x, from_lane<0x4e, 0xf>(x, x));
+  const uint32_t y4 = from_lane<0x124, 0xf>(x, x);  // 4, 8 away within the row of 16
+  x = wide ? max(x, y4) : min(x, y4);
+  const uint32_t y8 = from_lane<0x128, 0xf>(x, x);
+  x = wide ? max(x, y8) : min(x, y8);
+  const uint32_t a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16);
+  const uint32_t c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
+  return min(min(a, b), min(c, d));
+}
+
+// A word that at least `count` of N words a lane reach, and not many more, where they differ.
+// `count` reach lo; no word is above `most`.
 template <int N>
-__device__ __forceinline__ uint32_t wave_bound(const uint32_t (&key)[N], int count, uint32_t most) {
-  uint32_t lo = 0, hi = most + 1;  // `count` are at lo or more; fewer at hi
+__device__ __forceinline__ uint32_t near_bound(const uint32_t (&key)[N], int count, uint32_t lo, uint32_t most) {
+  uint64_t hi = (uint64_t)most + 1;  // fewer than `count` are here or above
   while (hi - lo > 1) {
-    const uint32_t mid = lo + (hi - lo) / 2;
+    const uint32_t mid = (uint32_t)(lo + (hi - lo) / 2);
     int n = 0;
 #pragma unroll
     for (int x = 0; x < N; ++x) n += __popcll(__ballot(key[x] >= mid));
-    if (n >= count) lo = mid;
-    if (n < count) hi = mid;
-    if (n == count) break;
+    if (n >= count) {
+      lo = mid;
+      if (n <= count + count / 2) break;
+    } else {
+      hi = mid;
+    }
   }
   return lo;
 }
@@ -184,7 +201,8 @@ struct SelectArgs {
 
 // Workgroup (tile, row): NV vectors a thread, all of them in registers: their sum of exp, and the
 // `count` best.  At least `count` elements reach the count-th largest of the threads' 256 largest, so
-// those below it cannot be among the best; the few that reach it are ranked against each other.
+// those below it cannot be among the best; the few that reach it, or a word a little below it, are
+// ranked against each other.
 // Where too many do (ties, or large ones in few threads) the count-th largest itself is found by
 // bisection.
 template <class T, int NV>
@@ -193,7 +211,7 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
   constexpr int VEC = L::kVec;
   __shared__ uint64_t best[kRoom];
   __shared__ double part_sum[kWaves], part_at[kWaves];
-  __shared__ uint32_t tops[kThreads];
+  __shared__ uint32_t tops[kThreads], lows[kWaves], highs[kWaves];
   __shared__ u32x4v hit[kVectors];
   __shared__ int hit_at[kVectors];
   __shared__ int found, vectors, scan[kWaves];
@@ -254,13 +272,21 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
     part_sum[wave] = sum;
     part_at[wave] = at;
   }
-  tops[tid] = order_of(lane_top) >> L::kZeros;
+  const uint32_t top_key = order_of(lane_top) >> L::kZeros;
+  const uint32_t low = least_of_groups(top_key, count <= 4 * kWaves);
+  tops[tid] = top_key;
+  if ((tid & 63) == 0) {
+    lows[wave] = low;
+    highs[wave] = order_of(high) >> L::kZeros;
+  }
   __syncthreads();
   uint32_t all_tops[kWaves];
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) all_tops[w] = tops[w * 64 + (tid & 63)];
-  const uint32_t bound = max(wave_bound(all_tops, count, 0xfffffffeu >> L::kZeros) << L::kZeros,
-                             order_of(-INFINITY) + 1);  // -inf is no candidate
+  const uint32_t bound = max(
+      near_bound(all_tops, count, min(min(lows[0], lows[1]), min(lows[2], lows[3])),
+                 max(max(highs[0], highs[1]), max(highs[2], highs[3]))) << L::kZeros,
+      order_of(-INFINITY) + 1);  // -inf is no candidate
   if (tid == 0) {
     const double m = fmax(fmax(part_at[0], part_at[1]), fmax(part_at[2], part_at[3]));
     double all = 0.0;
@@ -431,7 +457,7 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs s)
       }
       top = fmaxf(top, (float)value[x]);
     }
-    const uint32_t floor = order_of(-INFINITY) + 1, tops[1] = {order_of(top)}, low = wave_bound(tops, count, 0xfffffffeu);
+    const uint32_t floor = order_of(-INFINITY) + 1, tops[1] = {order_of(top)}, low = near_bound(tops, count, 0, 0xffffffffu);
     if (lane == 0) bounds[wave] = max(low, floor);
     __syncthreads();
     uint32_t bound = have == count ? order_of((float)best_value[count - 1]) : floor;
