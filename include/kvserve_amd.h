@@ -637,13 +637,15 @@ int kvmi_keep_drafts(const kvmi_cache* cache, void* const* bases, int32_t layers
  *   slots, starts  as in kvmi_build_tables, rows in the place of requests
  *   copies         int32 [R][3]: (from, to, tokens) for kvmi_copy_blocks, which has to run before
  *                  the new tokens are written; -1 behind the last
- *   workspace      kvmi_fork_workspace_bytes, 8-byte aligned: zero before the first call, and left
+ *   workspace      kvmi_fork_workspace_bytes, 16-byte aligned: zero before the first call, and left
  *                  so that the next call of the same sizes can use it
  * All or nothing: where the blocks asked for exceed the free ones (KVMI_ERR_NO_BLOCKS), the new
  * tokens exceed max_tokens, or a parent, a length or the ring's count is out of range
  * (KVMI_ERR_LENGTH), rows and ring stay as they are, all slots and copies are -1 and starts 0.
- * A row's id outside the pool is handed on, and sets KVMI_ERR_BLOCK_ID where its holders change.
- * Two launches; R <= 4096.
+ * A row's id outside the pool is handed on, and sets KVMI_ERR_BLOCK_ID where its holders change.  A
+ * row's last block has no other holder while it is partly filled, as every call leaves it; one that has
+ * sets KVMI_ERR_BLOCK_ID too, and the row goes on in it.
+ * Two launches, three past 256 rows; R <= 4096.
  */
 typedef struct kvmi_fork_args {
   const int32_t* lengths;
@@ -687,7 +689,7 @@ int kvmi_copy_blocks(const kvmi_cache* cache, void* const* bases, int32_t layers
  *                  pool's other ids in order.  All of them the inputs themselves, or none
  *   copies         int32 [blocks / 2][3]: the moves (from, to, block_size) for kvmi_copy_blocks,
  *                  -1 behind the last
- *   workspace      kvmi_compact_workspace_bytes, 8-byte aligned, as in kvmi_fork_tables
+ *   workspace      kvmi_compact_workspace_bytes, 16-byte aligned, as in kvmi_fork_tables
  * Ids outside the pool set KVMI_ERR_BLOCK_ID and keep their names; so do blocks that are both held and
  * free (held counts).  A length or count out of range sets KVMI_ERR_LENGTH and is cut.
  */

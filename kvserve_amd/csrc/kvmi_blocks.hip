@@ -10,17 +10,33 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kRange = 1024;        // block ids of a workgroup that goes through the pool, 4 a thread
-constexpr int kMostForkRows = 4096;  // 20 bytes of LDS each
+constexpr int kCounted = 64;        // block ids of a count
+constexpr int kMostForkRows = 4096;  // 32 bytes of LDS each
 
 inline int ranges_of(int blocks) { return (blocks + kRange - 1) / kRange; }
 
+// The wave's sums go from row to row of 16 lanes in registers.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t sum_with(uint32_t x) {
+  return add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false));
+}
+// Sum of the lanes up to this one.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x = sum_with<0x111, 0xf>(x);  // the lane 1, 2, 4, 8 before in the row
+  x = sum_with<0x112, 0xf>(x);
+  x = sum_with<0x114, 0xf>(x);
+  x = sum_with<0x118, 0xf>(x);
+  x = sum_with<0x142, 0xa>(x);  // the last lane of the row before, of the half before
+  return sum_with<0x143, 0xc>(x);
+}
+__device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(x), 63);
+}
 // Sums over the workgroup, given to every thread.
 template <int N>
 __device__ __forceinline__ void block_sums(uint32_t (&v)[N], uint32_t (*lds)[kWaves]) {
 #pragma unroll
-  for (int d = 32; d; d >>= 1)
-#pragma unroll
-    for (int x = 0; x < N; ++x) v[x] = add_sat(v[x], __shfl_xor(v[x], d, 64));
+  for (int x = 0; x < N; ++x) v[x] = wave_sum(v[x]);
   __syncthreads();
   if ((threadIdx.x & 63) == 0)
 #pragma unroll
@@ -32,12 +48,7 @@ __device__ __forceinline__ void block_sums(uint32_t (&v)[N], uint32_t (*lds)[kWa
 
 // Sum of the threads before this one; `lds` has a word a wave.
 __device__ __forceinline__ uint32_t before_in_block(uint32_t v, uint32_t* lds) {
-  uint32_t s = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t t = __shfl_up(s, d, 64);
-    if ((threadIdx.x & 63) >= d) s += t;
-  }
+  const uint32_t s = wave_scan(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = s;
   __syncthreads();
@@ -47,127 +58,231 @@ __device__ __forceinline__ uint32_t before_in_block(uint32_t v, uint32_t* lds) {
 }
 
 // ---------------------------------------------------------------- forked tables
+// What one row becomes, and what the rows before it take.
+struct ForkRow {
+  int parent, kept, next;
+  int stay;                         // blocks that it has from its parent
+  uint32_t takes, tokens, copies;   // of the rows before it
+  int kids, shortest, longest;      // its children, and the whole blocks that they keep of it
+  int own_column;                   // the block in which one of them goes on, or -1
+  int length;                       // before the call
+};
+struct ForkSum {
+  int taken;  // blocks out of the ring; -1 where the call changes nothing
+  uint32_t tokens, copies;
+  int head;   // of the ring
+};
 // Workspace, in 32-bit words.  `words` counts what happens to a block's holders: rows that go on
 // without it in the upper half, rows that come to it besides one in the lower (at most
 // kMostForkRows of either, so the halves do not meet).
 struct ForkSpace {
-  int64_t words, counts, ticket, taken, lengths, tables, size;
+  int64_t words, counts, ticket, sum, rows, lengths, tables, size;
 };
 __host__ __device__ inline ForkSpace fork_space(int blocks, int rows, int columns) {
   ForkSpace s;
   s.words = 0;
-  s.counts = blocks;  // freed blocks of each range of ids
-  s.ticket = s.counts + (blocks + kRange - 1) / kRange;
-  s.taken = s.ticket + 1;  // blocks taken out of the ring, -1 where the call changes nothing
-  s.lengths = s.taken + 1;
+  s.counts = blocks;  // freed blocks of each 64 ids: counted by 1024, thousands met at one address (34 us of 15)
+  s.ticket = s.counts + ((int64_t)blocks + kCounted - 1) / kCounted;
+  s.sum = (s.ticket + 4) / 4 * 4;
+  s.rows = s.sum + 4;
+  s.lengths = s.rows + 12 * (int64_t)rows;
   s.tables = (s.lengths + rows + 3) / 4 * 4;
   s.size = s.tables + (int64_t)rows * columns;
   return s;
 }
 
-// Workgroup (r, y) makes part y of row r, and counts what becomes of the blocks that row r held.
-// Every workgroup goes through all rows for itself, as the tables of unshared blocks are made: who
-// goes on in a partly kept block, and what the rows before take, so nobody waits.  Counts are sums of
-// integers, so the order of the atomics does not matter: a block is free when all that held it
-// have let go, which the last of them sees.
-__global__ __launch_bounds__(kThreads) void fork_rows_kernel(kvmi_fork_args a, BlockOf div, bool in_place) {
-  extern __shared__ int lds[];
-  __shared__ uint32_t sums[6][kWaves];
-  __shared__ int children, shortest;
-  const int R = a.rows, C = a.columns, N = a.blocks, S = a.block_size, tid = threadIdx.x, r = blockIdx.x;
-  int *const most = lds, *const owner = most + R, *const parent = owner + R, *const kept = parent + R,
-            *const next = kept + R;
-  const int top = C * S;
-  const int head = (int)((uint32_t)a.state[0] % (uint32_t)N), count = a.state[1];
-  int bad = count < 0 || count > N;
-  for (int i = tid; i < R; i += kThreads) {
-    most[i] = -1;
-    owner[i] = INT_MAX;
-  }
-  if (tid == 0) {
-    children = 0;
-    shortest = INT_MAX;
-  }
-  __syncthreads();
-  for (int i = tid; i < R; i += kThreads) {
-    int p = a.parents ? gld(a.parents + i) : i;
-    const int mine = gld(a.lengths + i);
-    if (p < -1 || p >= R || (uint32_t)mine > (uint32_t)top) {
+// The plan of all rows, made by one workgroup in its LDS, 32 bytes a row: one trip to memory, and one more
+// only where a row is cut inside a block, which others may hold (a row's own last block is held by
+// nobody else while it is partly filled).
+struct ForkPlan {
+  int *length, *parent, *kept, *next, *most, *owner, *kids, *shortest;
+  int* bad;  // one word
+};
+template <int THREADS>
+__device__ __forceinline__ ForkPlan plan_rows(const kvmi_fork_args& a, const BlockOf& div, int* lds) {
+  const int R = a.rows, C = a.columns, N = a.blocks, S = a.block_size, top = C * S, tid = threadIdx.x;
+  ForkPlan f{lds, lds + R, lds + 2 * R, lds + 3 * R, lds + 4 * R, lds + 5 * R, lds + 6 * R, lds + 7 * R, lds + 8 * R};
+  int bad = 0;
+  auto unshared = [&](int row, int column) -> int {
+    const int b = gld(a.tables + (int64_t)row * C + column);
+    return (uint32_t)b < (uint32_t)N && gld(a.shares + b) == 0;
+  };
+  for (int i = tid; i < R; i += THREADS) {
+    int p = a.parents ? gld(a.parents + i) : i, n = a.new_lengths ? gld(a.new_lengths + i) : 0;
+    int length = gld(a.lengths + i);
+    if (p < -1 || p >= R || (uint32_t)length > (uint32_t)top || (uint32_t)n > (uint32_t)top) {
       bad = 1;
       p = -1;
+      length = n = 0;
     }
-    int base = p >= 0 ? gld(a.lengths + p) : 0;
-    int64_t n = a.new_lengths ? (int64_t)gld(a.new_lengths + i) : p >= 0 ? (int64_t)base + a.grow : 0;
-    if ((uint32_t)base > (uint32_t)top || n < 0 || n > top) {
-      bad = 1;
-      base = 0;
-      n = 0;
+    f.length[i] = length;
+    f.parent[i] = p;
+    f.next[i] = n;
+    f.most[i] = -1;
+    f.owner[i] = f.shortest[i] = INT_MAX;
+    f.kids[i] = 0;
+  }
+  if (tid == 0) *f.bad = 0;
+  __syncthreads();
+  for (int i = tid; i < R; i += THREADS) {
+    const int p = f.parent[i], base = p >= 0 ? f.length[p] : 0;
+    if (!a.new_lengths) {
+      const int64_t n = p >= 0 ? (int64_t)base + a.grow : 0;
+      if (n > top) bad = 1;
+      f.next[i] = (int)min(n, (int64_t)top);
     }
-    parent[i] = p;
-    kept[i] = min(base, (int)n);
-    next[i] = (int)n;
-    if (p >= 0) atomicMax(&most[p], kept[i]);
+    const int kept = min(base, f.next[i]), whole = div(kept);
+    f.kept[i] = kept;
+    if (p >= 0) {
+      atomicMax(&f.most[p], kept);
+      atomicMin(&f.shortest[p], whole);
+      atomicAdd(&f.kids[p], 1);
+    }
+  }
+  if (bad) *f.bad = 1;
+  __syncthreads();
+  for (int i = tid; i < R; i += THREADS) {
+    const int p = f.parent[i], kept = f.kept[i], whole = div(kept);
+    if (p < 0 || kept == whole * S || div(f.most[p]) != whole) continue;
+    if (kept == f.length[p] || unshared(p, whole)) atomicMin(&f.owner[p], i);
   }
   __syncthreads();
-  for (int i = tid; i < R; i += kThreads) {
-    const int p = parent[i], full = div(kept[i]);
-    if (p < 0 || kept[i] == full * S || div(most[p]) != full) continue;
-    const int b = gld(a.tables + (int64_t)p * C + full);
-    if ((uint32_t)b < (uint32_t)N && gld(a.shares + b) == 0) atomicMin(&owner[p], i);
-  }
-  __syncthreads();
+  return f;
+}
+// What row i adds to the sums: blocks taken, new tokens, copies.
+__device__ __forceinline__ int stays(const ForkPlan& f, const BlockOf& div, int S, int i) {
+  const int whole = div(f.kept[i]);
+  return whole + (f.kept[i] != whole * S && f.owner[f.parent[i]] == i);
+}
+__device__ __forceinline__ void row_adds(const ForkPlan& f, const BlockOf& div, int S, int i, uint32_t (&v)[3]) {
+  const int whole = div(f.kept[i]), stay = stays(f, div, S, i), want = f.next[i] ? div(f.next[i] - 1) + 1 : 0;
+  v[0] = want - stay;
+  v[1] = f.next[i] - f.kept[i];
+  v[2] = f.kept[i] != whole * S && stay == whole;
+}
+__device__ __forceinline__ ForkRow row_of(const ForkPlan& f, const BlockOf& div, int S, int i, const uint32_t* before) {
+  return ForkRow{f.parent[i], f.kept[i],     f.next[i],           stays(f, div, S, i), before[0], before[1],
+                 before[2],   f.kids[i],     f.shortest[i],       div(max(f.most[i], 0)),
+                 f.owner[i] == INT_MAX ? -1 : div(f.most[i]),     f.length[i]};
+}
+// The sums of all rows, whether the call can be done, and its error.
+__device__ __forceinline__ ForkSum sum_of(const kvmi_fork_args& a, int head, int count, const uint32_t* all, int bad,
+                                          int32_t* error) {
+  bad |= count < 0 || count > a.blocks || all[1] > (uint32_t)a.max_tokens;
+  const bool fits = all[0] <= (uint32_t)max(count, 0);
+  *error = bad ? KVMI_ERR_LENGTH : fits ? 0 : KVMI_ERR_NO_BLOCKS;
+  return ForkSum{bad || !fits ? -1 : (int)all[0], all[1], all[2], (int)((uint32_t)head % (uint32_t)a.blocks)};
+}
 
-  // blocks taken, new tokens and copies of all rows, and of those before this one
-  uint32_t sum[6] = {0, 0, 0, 0, 0, 0};
-  for (int i = tid; i < R; i += kThreads) {
-    const int p = parent[i], full = div(kept[i]), want = next[i] ? div(next[i] - 1) + 1 : 0;
-    const bool rest = kept[i] != full * S, goes_on = rest && owner[p] == i;
-    const uint32_t v[3] = {(uint32_t)(want - full - goes_on), (uint32_t)(next[i] - kept[i]), rest && !goes_on};
+// What becomes of the blocks that row r held.  n entries from k on: their shares and atomics are on
+// their way in `begin`, and looked at in `end`, with what else there is to do between the two.
+// Counts are sums of integers, so the order of the atomics does not matter: a block is free when all that
+// held it have let go, which the last of them sees.  (A call that is refused clears them all the same.)
+template <int n>
+struct Settled {
+  int b[n], holders[n], shares[n];
+  uint32_t before[n];
+};
+struct Settler {
+  const kvmi_fork_args& a;
+  const ForkSpace& at;
+  const ForkRow& row;
+  int have, listed;
+  const int* list;
+  bool foreign;
+
+  template <int n>
+  __device__ __forceinline__ void begin(int k, Settled<n>& s) {
 #pragma unroll
-    for (int x = 0; x < 3; ++x) {
-      sum[x] = add_sat(sum[x], v[x]);
-      if (i < r) sum[3 + x] = add_sat(sum[3 + x], v[x]);
+    for (int x = 0; x < n; ++x) {
+      int holders = k + x == row.own_column;
+      if (k + x < row.shortest)
+        holders += row.kids;
+      else if (k + x < row.longest)
+        for (int c = 0; c < listed; ++c) holders += list[c] > k + x;
+      // (where a row goes on in its partly filled block, nobody else may hold it)
+      const bool changes = k + x < have && (holders != 1 || k + x == row.own_column);
+      const bool inside = (uint32_t)s.b[x] < (uint32_t)a.blocks;
+      foreign |= changes && !inside;
+      s.holders[x] = changes && inside ? holders : -1;
+      s.shares[x] = s.holders[x] == 0 || s.holders[x] == 1 ? gld(a.shares + s.b[x]) : 0;
+    }
+    uint32_t* const words = (uint32_t*)a.workspace + at.words;
+#pragma unroll
+    for (int x = 0; x < n; ++x)
+      if (s.holders[x] == 0)
+        s.before[x] = atomicAdd(words + s.b[x], 0x10000u);
+      else if (s.holders[x] > 1)
+        atomicAdd(words + s.b[x], (uint32_t)(s.holders[x] - 1));
+  }
+  template <int n>
+  __device__ __forceinline__ void end(const Settled<n>& s) {
+#pragma unroll
+    for (int x = 0; x < n; ++x) {
+      if (s.holders[x] == 0 && (int)(s.before[x] >> 16) == s.shares[x])
+        atomicAdd(a.workspace + at.counts + s.b[x] / kCounted, 1);
+      foreign |= s.holders[x] == 1 && s.shares[x];
     }
   }
-  block_sums(sum, sums);
-  bad = __syncthreads_or(bad);
-  const bool fits = sum[0] <= (uint32_t)max(count, 0), ok = !bad && fits && sum[1] <= (uint32_t)a.max_tokens;
-  const ForkSpace at = fork_space(N, R, C);
-  const int step = kThreads * gridDim.y, lane = blockIdx.y * kThreads + tid;
-  if (r == 0 && lane == 0) {
-    flag_error(a.err, bad || sum[1] > (uint32_t)a.max_tokens ? KVMI_ERR_LENGTH : fits ? 0 : KVMI_ERR_NO_BLOCKS);
-    a.workspace[at.taken] = ok ? (int)sum[0] : -1;
-    a.starts[0] = 0;
+};
+// The settler of row r, for which `child(i)` tells the whole blocks that row i keeps of it, -1 if it is no
+// child.  `list` has room for all rows.
+template <class F>
+__device__ __forceinline__ Settler settler_of(const kvmi_fork_args& a, const BlockOf& div, const ForkSpace& at,
+                                              const ForkRow& row, int* list, F child) {
+  __shared__ int children;
+  Settler s{a, at, row, row.length ? div(row.length - 1) + 1 : 0, 0, list, false};
+  if (row.kids && row.shortest < row.longest && row.shortest < s.have) {
+    // children that keep more and less: who holds a block between is counted
+    if (threadIdx.x == 0) children = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.rows; i += kThreads) {
+      const int keeps = child(i);
+      if (keeps >= 0) list[atomicAdd(&children, 1)] = keeps;
+    }
+    __syncthreads();
+    s.listed = children;
   }
-  const int32_t* const old = a.tables + (int64_t)r * C;
+  return s;
+}
+// Rows are read four entries at a time where they are aligned so.
+__device__ __forceinline__ Settled<4> four(const uint4& v) {
+  return Settled<4>{{(int)v.x, (int)v.y, (int)v.z, (int)v.w}, {-1, -1, -1, -1}, {}, {}};
+}
+
+// Part blockIdx.y of row r: its entries, slots and copy.  `ahead`: the parent's first entries, where rows
+// are read in fours.
+__device__ __forceinline__ void fork_row(const kvmi_fork_args& a, const BlockOf& div, bool in_place, const ForkSpace& at,
+                                         const ForkRow& row, const ForkSum& all, int r, bool fours,
+                                         const uint4& ahead) {
+  const int R = a.rows, C = a.columns, N = a.blocks, S = a.block_size, tid = threadIdx.x;
+  const int step = kThreads * gridDim.y, lane = blockIdx.y * kThreads + tid;
   int32_t* const out = (in_place ? a.workspace + at.tables : a.out_tables) + (int64_t)r * C;
-  int32_t* const copy = a.copies + 3 * (int64_t)r;
-  if (!ok) {
+  if (r == 0 && lane == 0) a.starts[0] = 0;
+  if (all.taken < 0) {
     if (!in_place)
-      for (int k = lane; k < C; k += step) gst(out + k, gld(old + k));
+      for (int k = lane; k < C; k += step) gst(out + k, gld(a.tables + (int64_t)r * C + k));
     for (int64_t k = (int64_t)r * step + lane; k < a.max_tokens; k += (int64_t)R * step) gst(a.slots + k, (int64_t)-1);
     if (lane == 0) {
-      if (!in_place) a.out_lengths[r] = a.lengths[r];
+      if (!in_place) a.out_lengths[r] = gld(a.lengths + r);  // (row.length is 0 where it is out of range)
       a.starts[r + 1] = 0;
+      int32_t* const copy = a.copies + 3 * (int64_t)r;
       copy[0] = copy[1] = copy[2] = -1;
     }
     return;
   }
-
-  // the new row
-  const int p = parent[r], from_kept = kept[r], n = next[r];
-  const int full = div(from_kept), rest = from_kept - full * S, want = n ? div(n - 1) + 1 : 0;
-  const int stay = full + (rest && owner[p] == r);
-  const uint32_t from = ring_at(head, sum[3], N);
-  const int32_t* const source = a.tables + (int64_t)max(p, 0) * C;
+  const int whole = div(row.kept), rest = row.kept - whole * S, want = row.next ? div(row.next - 1) + 1 : 0;
+  const int stay = row.stay;
+  const uint32_t from = ring_at(all.head, row.takes, N);
+  const int32_t* const source = a.tables + (int64_t)max(row.parent, 0) * C;
   auto entry = [&](int k) -> int32_t {
     return k >= want ? -1 : gld(k < stay ? source + k : a.free_blocks + ring_at(from, k - stay, N));
   };
-  if ((C & 3) == 0 && (((uintptr_t)a.tables | (uintptr_t)out) & 15) == 0) {
+  if (fours) {
     for (int k = 4 * lane; k < C; k += 4 * step) {
       uint4 v = make_uint4(~0u, ~0u, ~0u, ~0u);
       if (k + 4 <= stay) {
-        v = gld((const uint4*)(source + k));
+        v = k == 4 * lane ? ahead : gld((const uint4*)(source + k));
       } else if (k < want) {
         v.x = entry(k);
         v.y = entry(k + 1);
@@ -179,56 +294,171 @@ __global__ __launch_bounds__(kThreads) void fork_rows_kernel(kvmi_fork_args a, B
   } else {
     for (int k = lane; k < C; k += step) gst(out + k, entry(k));
   }
-  int64_t* const slots = a.slots + sum[4];
-  for (int i = lane; i < n - from_kept; i += step) {
-    const int pos = from_kept + i, k = div(pos);
+  int64_t* const slots = a.slots + row.tokens;
+  for (int i = lane; i < row.next - row.kept; i += step) {
+    const int pos = row.kept + i, k = div(pos);
     gst(slots + i, (int64_t)entry(k) * S + (pos - k * S));
   }
   if (r == R - 1)
-    for (int64_t k = (int64_t)sum[1] + lane; k < a.max_tokens; k += step) gst(a.slots + k, (int64_t)-1);
+    for (int64_t k = (int64_t)all.tokens + lane; k < a.max_tokens; k += step) gst(a.slots + k, (int64_t)-1);
   if (lane == 0) {
-    (in_place ? a.workspace + at.lengths : a.out_lengths)[r] = n;
-    a.starts[r + 1] = (int)sum[4] + (n - from_kept);
+    (in_place ? a.workspace + at.lengths : a.out_lengths)[r] = row.next;
+    a.starts[r + 1] = (int)row.tokens + (row.next - row.kept);
     // copies first, in the order of their rows
-    const bool copies = rest && stay == full;
-    int32_t* const to = a.copies + 3 * (int64_t)(copies ? sum[5] : sum[2] + (r - sum[5]));
-    to[0] = copies ? gld(source + full) : -1;
-    to[1] = copies ? entry(full) : -1;
+    const bool copies = rest && stay == whole;
+    const int b = copies ? gld(source + whole) : -1, fresh = copies ? entry(whole) : -1;
+    int32_t* const to = a.copies + 3 * (int64_t)(copies ? row.copies : all.copies + (r - row.copies));
+    to[0] = b;
+    to[1] = fresh;
     to[2] = copies ? rest : -1;
   }
-
-  // what becomes of the blocks that row r held: its children's whole blocks, and the block in
-  // which one of them goes on
-  const int mine = a.lengths[r], have = mine ? div(mine - 1) + 1 : 0;
-  const int own_column = owner[r] == INT_MAX ? -1 : div(most[r]);
-  __syncthreads();  // `most` becomes the list of this row's children
-  for (int i = tid; i < R; i += kThreads)
-    if (parent[i] == r) {
-      const int whole = div(kept[i]);
-      most[atomicAdd(&children, 1)] = whole;
-      atomicMin(&shortest, whole);
+}
+// The rest of what row r held, behind the first four entries of each thread.
+__device__ __forceinline__ void settle_rest(Settler& settler, int r, bool fours) {
+  const int step = kThreads * gridDim.y, lane = blockIdx.y * kThreads + threadIdx.x;
+  const int32_t* const old = settler.a.tables + (int64_t)r * settler.a.columns;
+  if (fours) {
+    for (int k = 4 * (lane + step); k < settler.have; k += 4 * step) {
+      Settled<4> s = four(gld((const uint4*)(old + k)));
+      settler.begin(k, s);
+      settler.end(s);
     }
-  __syncthreads();
-  const int kids = children, all_below = shortest;
-  bool foreign = false;
-  for (int k = lane; k < have; k += step) {
-    int holders = k == own_column;
-    if (k < all_below)
-      holders += kids;
-    else
-      for (int c = 0; c < kids; ++c) holders += most[c] > k;
-    if (holders == 1) continue;
-    const int b = gld(old + k);
-    if ((uint32_t)b >= (uint32_t)N) {
-      foreign = true;
-    } else if (holders == 0) {
-      const uint32_t before = atomicAdd((uint32_t*)a.workspace + at.words + b, 0x10000u);
-      if ((int)(before >> 16) == gld(a.shares + b)) atomicAdd(a.workspace + at.counts + b / kRange, 1);
-    } else {
-      atomicAdd((uint32_t*)a.workspace + at.words + b, (uint32_t)(holders - 1));
+  } else {
+    for (int k = lane; k < settler.have; k += step) {
+      Settled<1> s{{gld(old + k)}, {}, {}, {}};
+      settler.begin(k, s);
+      settler.end(s);
     }
   }
-  if (foreign) flag_error(a.err, KVMI_ERR_BLOCK_ID);
+}
+__device__ __forceinline__ bool in_fours(const kvmi_fork_args& a, const ForkSpace& at, bool in_place) {
+  const void* const out = in_place ? a.workspace + at.tables : a.out_tables;
+  return (a.columns & 3) == 0 && (((uintptr_t)a.tables | (uintptr_t)out) & 15) == 0;
+}
+
+// Up to kFused rows: every workgroup (row, part) plans them all for itself, while its entries are on
+// their way, and no workgroup waits for another.  4 rows of 32 blocks 4.6 us, 256 rows of up to 750
+// FUSED_FIGURE.
+#ifndef FUSED
+#define FUSED 256
+#endif
+constexpr int kFused = FUSED;
+__global__ __launch_bounds__(kThreads) void fork_fused_kernel(kvmi_fork_args a, BlockOf div, bool in_place) {
+  __shared__ int lds[8 * kFused + 1], list[kFused];
+  const int R = a.rows, C = a.columns, tid = threadIdx.x, r = blockIdx.x;
+  const ForkSpace at = fork_space(a.blocks, R, C);
+  const bool fours = in_fours(a, at, in_place);
+  const int head = gld(a.state), count = gld(a.state + 1);
+  const int k = 4 * (blockIdx.y * kThreads + tid);
+  uint4 old = make_uint4(0, 0, 0, 0), source = old;
+  if (fours && k < C) {
+    int p = a.parents ? a.parents[r] : r;
+    p = p < 0 || p >= R ? r : p;
+    old = gld((const uint4*)(a.tables + (int64_t)r * C + k));
+    source = gld((const uint4*)(a.tables + (int64_t)p * C + k));
+  }
+  const ForkPlan f = plan_rows<kThreads>(a, div, lds);
+  // the row's own plan but for what the rows before it take; its blocks' holders are on their way
+  // while that is summed, by every wave for itself
+  const uint32_t none[3] = {0, 0, 0};
+  ForkRow row = row_of(f, div, a.block_size, r, none);
+  Settler settler = settler_of(a, div, at, row, list, [&](int i) { return f.parent[i] == r ? div(f.kept[i]) : -1; });
+  Settled<4> held = four(old);
+  if (fours && k < settler.have) settler.begin(k, held);
+  uint32_t sum[6] = {0, 0, 0, 0, 0, 0};
+  for (int i = tid & 63; i < R; i += 64) {
+    uint32_t v[3];
+    row_adds(f, div, a.block_size, i, v);
+#pragma unroll
+    for (int x = 0; x < 3; ++x) {
+      sum[x] = add_sat(sum[x], v[x]);
+      sum[3 + x] = add_sat(sum[3 + x], i < r ? v[x] : 0);
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < 6; ++x) sum[x] = wave_sum(sum[x]);
+  int32_t error;
+  const ForkSum all = sum_of(a, head, count, sum, *f.bad, &error);
+  row.takes = sum[3];
+  row.tokens = sum[4];
+  row.copies = sum[5];
+  if (r == 0 && blockIdx.y == 0 && tid == 0) {
+    flag_error(a.err, error);
+    a.workspace[at.sum] = all.taken;
+  }
+  fork_row(a, div, in_place, at, row, all, r, fours, source);
+  settler.end(held);
+  settle_rest(settler, r, fours);
+  if (settler.foreign) flag_error(a.err, KVMI_ERR_BLOCK_ID);
+}
+
+// More rows: one workgroup plans them, the others read their rows' plans.  1024 rows planned by each of
+// 2048 workgroups took 39 us.
+constexpr int kPlanThreads = 1024;
+__global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(kvmi_fork_args a, BlockOf div) {
+  extern __shared__ int plan_lds[];
+  __shared__ uint32_t wave_sums[3][kPlanThreads / 64], carry[3];
+  const int R = a.rows, tid = threadIdx.x, head = gld(a.state), count = gld(a.state + 1);
+  const ForkSpace at = fork_space(a.blocks, R, a.columns);
+  const ForkPlan f = plan_rows<kPlanThreads>(a, div, plan_lds);
+  if (tid < 3) carry[tid] = 0;
+  __syncthreads();
+  for (int i0 = 0; i0 < R; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    uint32_t v[3] = {0, 0, 0}, before[3];
+    if (i < R) row_adds(f, div, a.block_size, i, v);
+#pragma unroll
+    for (int x = 0; x < 3; ++x) {
+      before[x] = wave_scan(v[x]);
+      if ((tid & 63) == 63) wave_sums[x][tid >> 6] = before[x];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 3; ++x) {
+      uint32_t s = carry[x];
+      for (int w = 0; w < (tid >> 6); ++w) s = add_sat(s, wave_sums[x][w]);
+      before[x] = add_sat(s, before[x]) - v[x];  // (a saturated sum is refused)
+    }
+    if (i < R) {
+      const ForkRow row = row_of(f, div, a.block_size, i, before);
+      uint4* const to = (uint4*)(a.workspace + at.rows + 12 * (int64_t)i);
+#pragma unroll
+      for (int w = 0; w < 3; ++w) gst(to + w, ((const uint4*)&row)[w]);
+    }
+    __syncthreads();
+    if (tid < 3) {
+      uint32_t s = carry[tid];
+      for (int w = 0; w < kPlanThreads / 64; ++w) s = add_sat(s, wave_sums[tid][w]);
+      carry[tid] = s;
+    }
+    __syncthreads();
+  }
+  if (tid == 0) {
+    int32_t error;
+    const ForkSum all = sum_of(a, head, count, carry, *f.bad, &error);
+    flag_error(a.err, error);
+    gst((uint4*)(a.workspace + at.sum), *(const uint4*)&all);
+  }
+}
+__global__ __launch_bounds__(kThreads) void fork_rows_kernel(kvmi_fork_args a, BlockOf div, bool in_place) {
+  __shared__ int list[kMostForkRows];
+  const int R = a.rows, C = a.columns, r = blockIdx.x;
+  const ForkSpace at = fork_space(a.blocks, R, C);
+  const bool fours = in_fours(a, at, in_place);
+  const int k = 4 * (blockIdx.y * kThreads + threadIdx.x);
+  const ForkRow* const rows = (const ForkRow*)(a.workspace + at.rows);
+  uint4 old = make_uint4(0, 0, 0, 0), source = old;
+  if (fours && k < C) old = gld((const uint4*)(a.tables + (int64_t)r * C + k));
+  const ForkRow row = rows[r];
+  const ForkSum all = *(const ForkSum*)(a.workspace + at.sum);
+  if (fours && k < C) source = gld((const uint4*)(a.tables + (int64_t)max(row.parent, 0) * C + k));
+  Settler settler = settler_of(a, div, at, row, list, [&](int i) { return rows[i].parent == r ? div(rows[i].kept) : -1; });
+  Settled<4> held = four(old);
+  if (fours && k < settler.have) settler.begin(k, held);
+  fork_row(a, div, in_place, at, row, all, r, fours, source);
+  settler.end(held);
+  settle_rest(settler, r, fours);
+  if (settler.foreign) flag_error(a.err, KVMI_ERR_BLOCK_ID);
 }
 
 // Workgroup g < ranges goes through 1024 block ids: their new shares, and the free ones behind the
@@ -240,7 +470,7 @@ __global__ __launch_bounds__(kThreads) void fork_blocks_kernel(kvmi_fork_args a,
   __shared__ int last;
   const int N = a.blocks, tid = threadIdx.x, g = blockIdx.x;
   const ForkSpace at = fork_space(N, a.rows, a.columns);
-  const int taken = a.workspace[at.taken];
+  const int taken = a.workspace[at.sum];
   if (g >= ranges) {
     if (taken < 0) return;
     const int64_t all = (int64_t)a.rows * a.columns, step = (int64_t)(gridDim.x - ranges) * kThreads;
@@ -257,22 +487,24 @@ __global__ __launch_bounds__(kThreads) void fork_blocks_kernel(kvmi_fork_args a,
   const int head = (int)((uint32_t)a.state[0] % (uint32_t)N), given = a.state[1];
   const int count = given < 0 ? 0 : given > N ? N : given;
   int32_t* const counts = a.workspace + at.counts;
-  uint32_t sum[2] = {0, 0};  // freed before this range, and in all
-  for (int i = tid; i < ranges; i += kThreads) {
-    const uint32_t v = gld(counts + i);
-    sum[1] += v;
-    if (i < g) sum[0] += v;
-  }
-  block_sums(sum, sums);
-  uint32_t word[4];
+  uint32_t held[4], word[4];  // (a refused call has counted, too)
   int shares[4];
   const int first = g * kRange + 4 * tid;
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
     const bool in = first + x < N;
-    word[x] = in ? gld((const uint32_t*)a.workspace + at.words + first + x) : 0;
+    held[x] = in ? gld((const uint32_t*)a.workspace + at.words + first + x) : 0;
+    word[x] = taken < 0 ? 0 : held[x];
     shares[x] = in ? gld(a.shares + first + x) : 0;
   }
+  uint32_t sum[2] = {0, 0};  // freed before this range, and in all
+  const int counted = (N + kCounted - 1) / kCounted;
+  for (int i = tid; i < counted; i += kThreads) {
+    const uint32_t v = gld(counts + i);
+    sum[1] += v;
+    if (i < g * (kRange / kCounted)) sum[0] += v;
+  }
+  block_sums(sum, sums);
   uint32_t free = 0;
 #pragma unroll
   for (int x = 0; x < 4; ++x) free += word[x] >> 16 && (int)(word[x] >> 16) > shares[x];
@@ -284,7 +516,7 @@ __global__ __launch_bounds__(kThreads) void fork_blocks_kernel(kvmi_fork_args a,
     const int gone = (int)(word[x] >> 16), b = first + x;
     const int now = max(0, shares[x] + (int)(word[x] & 0xffffu) - gone);
     if (!in_place || now != shares[x]) a.out_shares[b] = now;
-    if (word[x]) a.workspace[at.words + b] = 0;
+    if (held[x]) a.workspace[at.words + b] = 0;
     if (gone && gone > shares[x]) {
       if (place < (uint32_t)(N - count))
         a.free_blocks[((int64_t)head + count + place) % N] = b;
@@ -298,7 +530,7 @@ __global__ __launch_bounds__(kThreads) void fork_blocks_kernel(kvmi_fork_args a,
   if (tid == 0) last = atomicAdd(a.workspace + at.ticket, 1) == ranges - 1;
   __syncthreads();
   if (!last) return;
-  for (int i = tid; i < ranges; i += kThreads) counts[i] = 0;
+  for (int i = tid; i < counted; i += kThreads) counts[i] = 0;
   if (tid == 0) {
     a.workspace[at.ticket] = 0;
     const int out = max(taken, 0), back = min((int)sum[1], N - count);
@@ -618,14 +850,20 @@ extern "C" int kvmi_fork_tables(const kvmi_fork_args* args, kvmi_stream_t stream
   if (in_place != (a.out_lengths == a.lengths) || in_place != (a.out_shares == a.shares) ||
       in_place != (a.out_state == a.state))
     return KVMI_EINVAL;
-  if (a.new_lengths == a.out_lengths || a.parents == a.out_lengths || (uintptr_t)a.workspace % 8 ||
+  if (a.new_lengths == a.out_lengths || a.parents == a.out_lengths || (uintptr_t)a.workspace % 16 ||
       a.workspace_bytes < kvmi_fork_workspace_bytes(a.blocks, a.rows, a.columns))
     return KVMI_EINVAL;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int64_t most = std::max<int64_t>((a.columns + 1023) / 1024, ((int64_t)a.max_tokens + 4095) / 4096);
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(most, std::min(64, 2048 / a.rows)));
-  hipLaunchKernelGGL(fork_rows_kernel, dim3((unsigned)a.rows, (unsigned)parts), dim3(kThreads), 20 * (size_t)a.rows,
-                     st, a, block_of(a.block_size), in_place);
+  const BlockOf div = block_of(a.block_size);
+  const dim3 grid((unsigned)a.rows, (unsigned)parts);
+  if (a.rows <= kFused) {
+    hipLaunchKernelGGL(fork_fused_kernel, grid, dim3(kThreads), 0, st, a, div, in_place);
+  } else {
+    hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kPlanThreads), 32 * (size_t)a.rows + 4, st, a, div);
+    hipLaunchKernelGGL(fork_rows_kernel, grid, dim3(kThreads), 0, st, a, div, in_place);
+  }
   const int ranges = ranges_of(a.blocks);
   const int64_t copies = in_place ? std::min<int64_t>(1024, ((int64_t)a.rows * a.columns + 4095) / 4096) : 0;
   hipLaunchKernelGGL(fork_blocks_kernel, dim3((unsigned)(ranges + copies)), dim3(kThreads), 0, st, a, ranges,
@@ -668,7 +906,7 @@ extern "C" int kvmi_compact_tables(const kvmi_compact_args* args, kvmi_stream_t 
     return KVMI_EINVAL;
   const bool in_place = a.out_shares == a.shares;
   if ((a.rows && in_place != (a.out_tables == a.tables)) || in_place != (a.out_free == a.free_blocks) ||
-      in_place != (a.out_state == a.state) || (uintptr_t)a.workspace % 8 ||
+      in_place != (a.out_state == a.state) || (uintptr_t)a.workspace % 16 ||
       a.workspace_bytes < kvmi_compact_workspace_bytes(a.blocks))
     return KVMI_EINVAL;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);

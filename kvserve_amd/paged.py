@@ -486,8 +486,8 @@ def _space(workspace: Optional[torch.Tensor], size: int, device) -> torch.Tensor
     if workspace is None:
         return _words(size, device)
     _tensor(workspace, "workspace", torch.int32, (None,), device)
-    if workspace.numel() * 4 < size or workspace.data_ptr() % 8:
-        raise ValueError(f"workspace must hold {(size + 3) // 4} words, 8-byte aligned")
+    if workspace.numel() * 4 < size or workspace.data_ptr() % 16:
+        raise ValueError(f"workspace must hold {(size + 3) // 4} words, 16-byte aligned")
     return workspace
 
 
@@ -513,7 +513,8 @@ def fork_block_tables(lengths: torch.Tensor, parents: Optional[torch.Tensor], ne
     new_lengths  int32 [R]: tokens after the call; min(new, the parent's) of them are the
                  parent's.  Or an integer: that many more than the parent has, and no tokens where there
                  is no parent
-    tables       int32 [R, columns]; rows that share a block have it in the same column
+    tables       int32 [R, columns]; rows that share a block have it in the same column, and a row's last
+                 block is its own while it is partly filled (every call leaves them so)
     shares       int32 [blocks]: how many rows hold a block besides the first
     free, state  the ring of free blocks, int32 [blocks], and its head and count, as in
                  `build_block_tables`; `free` is changed in place
