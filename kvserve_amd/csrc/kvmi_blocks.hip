@@ -46,15 +46,22 @@ __device__ __forceinline__ void block_sums(uint32_t (&v)[N], uint32_t (*lds)[kWa
   for (int x = 0; x < N; ++x) v[x] = add_sat(add_sat(lds[x][0], lds[x][1]), add_sat(lds[x][2], lds[x][3]));
 }
 
-// Sum of the threads before this one; `lds` has a word a wave.
-__device__ __forceinline__ uint32_t before_in_block(uint32_t v, uint32_t* lds) {
-  const uint32_t s = wave_scan(v);
+// Sums of the threads before this one.
+template <int N>
+__device__ __forceinline__ void before_in_block(uint32_t (&v)[N], uint32_t (*lds)[kWaves]) {
+  uint32_t s[N];
+#pragma unroll
+  for (int x = 0; x < N; ++x) s[x] = wave_scan(v[x]);
   __syncthreads();
-  if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = s;
+  if ((threadIdx.x & 63) == 63)
+#pragma unroll
+    for (int x = 0; x < N; ++x) lds[x][threadIdx.x >> 6] = s[x];
   __syncthreads();
-  uint32_t carry = 0;
-  for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) carry += lds[w];
-  return s - v + carry;
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+    v[x] = s[x] - v[x];
+    for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) v[x] += lds[x][w];
+  }
 }
 
 // ---------------------------------------------------------------- forked tables
@@ -466,7 +473,7 @@ __global__ __launch_bounds__(kThreads) void fork_rows_kernel(kvmi_fork_args a, B
 // the counts, when nobody reads them any more.  The other workgroups bring rows that are made in
 // place from the workspace to their table.
 __global__ __launch_bounds__(kThreads) void fork_blocks_kernel(kvmi_fork_args a, int ranges, bool in_place) {
-  __shared__ uint32_t sums[2][kWaves], scan[kWaves];
+  __shared__ uint32_t sums[2][kWaves];
   __shared__ int last;
   const int N = a.blocks, tid = threadIdx.x, g = blockIdx.x;
   const ForkSpace at = fork_space(N, a.rows, a.columns);
@@ -508,7 +515,9 @@ __global__ __launch_bounds__(kThreads) void fork_blocks_kernel(kvmi_fork_args a,
   uint32_t free = 0;
 #pragma unroll
   for (int x = 0; x < 4; ++x) free += word[x] >> 16 && (int)(word[x] >> 16) > shares[x];
-  uint32_t place = sum[0] + before_in_block(free, scan);
+  uint32_t place[1] = {free};
+  before_in_block(place, sums);
+  place[0] += sum[0];
   bool lost = false;
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
@@ -518,11 +527,11 @@ __global__ __launch_bounds__(kThreads) void fork_blocks_kernel(kvmi_fork_args a,
     if (!in_place || now != shares[x]) a.out_shares[b] = now;
     if (held[x]) a.workspace[at.words + b] = 0;
     if (gone && gone > shares[x]) {
-      if (place < (uint32_t)(N - count))
-        a.free_blocks[((int64_t)head + count + place) % N] = b;
+      if (place[0] < (uint32_t)(N - count))
+        a.free_blocks[((int64_t)head + count + place[0]) % N] = b;
       else
         lost = true;
-      ++place;
+      ++place[0];
     }
   }
   if (lost) flag_error(a.err, KVMI_ERR_LENGTH);
@@ -682,86 +691,87 @@ __global__ __launch_bounds__(kThreads) void compact_count_kernel(kvmi_compact_ar
 // stay or are taken (n: held blocks), so the number of moves is that of the free ones among them:
 // those of the ranges below the one where n falls, and some in it, which each looks up for itself.
 __global__ __launch_bounds__(kThreads) void compact_rank_kernel(kvmi_compact_args a, int ranges) {
-  __shared__ uint32_t sums[4][kWaves], scan[kWaves], cut[3];
-  const int N = a.blocks, tid = threadIdx.x, g = blockIdx.x;
+  __shared__ uint32_t sums[2][kWaves], mine[2], cut[3];
+  const int N = a.blocks, tid = threadIdx.x, g = blockIdx.x, first = g * kRange + 4 * tid;
   const CompactSpace at = compact_space(N);
   uint8_t* const space = (uint8_t*)a.workspace;
   const uint32_t* const counts = (const uint32_t*)(space + at.counts);
-  uint32_t sum[4] = {0, 0, 0, 0};  // held and pool before this range, and in all
+  uint32_t free;
+  const uint32_t held = marks_of(space, at, N, first, &free), pool = held | free;
+  int shares[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) shares[x] = (held >> (8 * x) & 1) && first + x < N ? gld(a.shares + first + x) : 0;
+  uint32_t total[2] = {0, 0};  // held, and in the pool
   for (int i = tid; i < ranges; i += kThreads) {
-    const uint32_t h = gld(counts + 2 * i), u = gld(counts + 2 * i + 1);
-    sum[2] += h;
-    sum[3] += u;
-    if (i < g) {
-      sum[0] += h;
-      sum[1] += u;
-    }
+    total[0] += gld(counts + 2 * i);
+    total[1] += gld(counts + 2 * i + 1);
   }
-  block_sums(sum, sums);
-  const uint32_t n = sum[2];
-  // the range in which the pool's n-th id falls, and what is held and in the pool before it
-  uint32_t held_before = 0, pool_before = 0;
+  block_sums(total, sums);
+  const uint32_t n = total[0];
+  // what is held and in the pool before this range, and before the one in which the pool's n-th id falls
   if (tid == 0) cut[0] = 0x7fffffff;
+  uint32_t carry[2] = {0, 0};
   for (int i0 = 0; i0 < ranges; i0 += kThreads) {
     const int i = i0 + tid;
     const uint32_t h = i < ranges ? gld(counts + 2 * i) : 0, u = i < ranges ? gld(counts + 2 * i + 1) : 0;
-    const uint32_t hb = held_before + before_in_block(h, scan);
-    const uint32_t ub = pool_before + before_in_block(u, scan);
-    if (ub < n && ub + u >= n) {
-      cut[0] = i;
-      cut[1] = hb;
-      cut[2] = ub;
+    uint32_t before[2] = {h, u};
+    before_in_block(before, sums);
+    before[0] += carry[0];
+    before[1] += carry[1];
+    if (i == g) {
+      mine[0] = before[0];
+      mine[1] = before[1];
     }
-    uint32_t all[2] = {h, u};
-    block_sums(all, sums);
-    held_before += all[0];
-    pool_before += all[1];
+    if (before[1] < n && before[1] + u >= n) {
+      cut[0] = i;
+      cut[1] = before[0];
+      cut[2] = before[1];
+    }
+    if (i0 + kThreads < ranges) {
+      uint32_t all[2] = {h, u};
+      block_sums(all, sums);
+      carry[0] += all[0];
+      carry[1] += all[1];
+    }
   }
-  __syncthreads();
+  // this range's places; both counts fit half a word
+  uint32_t place[1] = {(uint32_t)__popc(held) | (uint32_t)__popc(pool) << 16};
+  before_in_block(place, sums);  // (its barriers are for `mine` and `cut` too)
+  uint32_t h = mine[0] + (place[0] & 0xffffu), u = mine[1] + (place[0] >> 16);
   uint32_t moves = 0;
   if (cut[0] != 0x7fffffff) {
-    uint32_t free;
-    const uint32_t held = marks_of(space, at, N, cut[0] * kRange + 4 * tid, &free), pool = held | free;
-    uint32_t u = cut[2] + before_in_block(__popc(pool), scan);
+    uint32_t cut_free;
+    const uint32_t cut_held = marks_of(space, at, N, cut[0] * kRange + 4 * tid, &cut_free), cut_pool = cut_held | cut_free;
+    uint32_t rank[1] = {(uint32_t)__popc(cut_pool)};
+    before_in_block(rank, sums);
+    rank[0] += cut[2];
     uint32_t low[1] = {0};  // held in the range below the cut
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      if (!(pool >> (8 * x) & 1)) continue;
-      low[0] += u < n && (held >> (8 * x) & 1);
-      ++u;
+      if (!(cut_pool >> (8 * x) & 1)) continue;
+      low[0] += rank[0] < n && (cut_held >> (8 * x) & 1);
+      ++rank[0];
     }
     block_sums(low, sums);
     moves = n - cut[1] - low[0];
   }
-  // this range
-  const int first = g * kRange + 4 * tid;
-  uint32_t free;
-  const uint32_t held = marks_of(space, at, N, first, &free), pool = held | free;
-  uint32_t h = sum[0] + before_in_block(__popc(held), scan), u = sum[1] + before_in_block(__popc(pool), scan);
   int32_t* const names = (int32_t*)(space + at.names);
-  const uint32_t left = sum[3] - n;  // free blocks afterwards
+  const uint32_t left = total[1] - n;  // free blocks afterwards
   int bits = 0;
-  for (int x = 0; x < 4 && first + x < N; ++x) {
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    if (first + x >= N) break;
     const int b = first + x;
     const bool is_held = held >> (8 * x) & 1, in_pool = pool >> (8 * x) & 1;
     if (is_held && (free >> (8 * x) & 1)) bits |= KVMI_ERR_BLOCK_ID;
-    int shares = is_held ? gld(a.shares + b) : 0, name = b;
-    bool write = true;
-    if (in_pool && u >= n) {
-      gst(a.out_free + (u - n), b);
-      if (is_held) {
-        const uint32_t i = h - (n - moves);
-        gst((int32_t*)(space + at.from) + i, b);
-        gst((int32_t*)(space + at.shares) + i, shares);
-        name = -1 - (int)i;
-        shares = 0;
-      }
-    } else if (in_pool && !is_held) {
-      gst((int32_t*)(space + at.to) + (u - h), b);
-      write = false;  // comes from the block that moves here
-    }
-    gst(names + b, name);
-    if (write) gst(a.out_shares + b, shares);
+    const bool high = in_pool && u >= n, moved = high && is_held, taken = in_pool && !high && !is_held;
+    const uint32_t i = h - (n - moves);  // of a block that moves
+    gst(names + b, moved ? -1 - (int)i : b);
+    if (!taken) gst(a.out_shares + b, moved ? 0 : shares[x]);  // (what is taken has those of the block that comes)
+    if (taken) gst((int32_t*)(space + at.to) + (u - h), b);
+    if (moved) gst((int32_t*)(space + at.from) + i, b);
+    if (moved) gst((int32_t*)(space + at.shares) + i, shares[x]);
+    if (high) gst(a.out_free + (u - n), b);
     if ((uint32_t)b >= left) gst(a.out_free + b, -1);
     h += is_held;
     u += in_pool;
