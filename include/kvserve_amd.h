@@ -645,7 +645,8 @@ int kvmi_keep_drafts(const kvmi_cache* cache, void* const* bases, int32_t layers
  * A row's id outside the pool is handed on, and sets KVMI_ERR_BLOCK_ID where its holders change.  A
  * row's last block has no other holder while it is partly filled, as every call leaves it; one that has
  * sets KVMI_ERR_BLOCK_ID too, and the row goes on in it.
- * Two launches, three past 256 rows; R <= 4096.
+ * Two launches, three past 256 rows; at most 4096 rows, and 2^24 blocks here and in
+ * kvmi_compact_tables.
  */
 typedef struct kvmi_fork_args {
   const int32_t* lengths;

@@ -159,7 +159,8 @@ __device__ __forceinline__ uint32_t least_of_groups(uint32_t x, bool wide) {
 // `count` reach lo; no word is above `most`.
 template <int N>
 __device__ __forceinline__ uint32_t near_bound(const uint32_t (&key)[N], int count, uint32_t lo, uint32_t most) {
-  uint64_t hi = (uint64_t)most + 1;  // fewer than `count` are here or above
+  // fewer than `count` are at hi or above (NaN may have any place: hi stays above lo, so the loop ends)
+  uint64_t hi = (uint64_t)max(most, lo) + 1;
   while (hi - lo > 1) {
     const uint32_t mid = (uint32_t)(lo + (hi - lo) / 2);
     int n = 0;

@@ -12,6 +12,9 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kRange = 1024;        // block ids of a workgroup that goes through the pool, 4 a thread
 constexpr int kCounted = 64;        // block ids of a count
 constexpr int kMostForkRows = 4096;  // 32 bytes of LDS each
+// Every workgroup that goes through the pool adds up the counts of all: past this that would take longer
+// than the pool itself.
+constexpr int kMostBlocks = 1 << 24;
 
 inline int ranges_of(int blocks) { return (blocks + kRange - 1) / kRange; }
 
@@ -838,7 +841,7 @@ __global__ __launch_bounds__(kThreads) void compact_name_kernel(kvmi_compact_arg
 }  // namespace kvmi
 
 extern "C" int64_t kvmi_fork_workspace_bytes(int32_t blocks, int32_t rows, int32_t columns) {
-  if (blocks < 1 || rows < 0 || columns < 1) return KVMI_EINVAL;
+  if (blocks < 1 || blocks > kvmi::kMostBlocks || rows < 0 || columns < 1) return KVMI_EINVAL;
   return 4 * kvmi::fork_space(blocks, rows, columns).size;
 }
 
@@ -846,7 +849,8 @@ extern "C" int kvmi_fork_tables(const kvmi_fork_args* args, kvmi_stream_t stream
   using namespace kvmi;
   if (!args) return KVMI_EINVAL;
   const kvmi_fork_args& a = *args;
-  if (a.rows < 0 || a.rows > kMostForkRows || a.columns < 1 || a.blocks < 1 || a.block_size < 1 || a.max_tokens < 0 ||
+  if (a.rows < 0 || a.rows > kMostForkRows || a.columns < 1 || a.blocks < 1 || a.blocks > kMostBlocks ||
+      a.block_size < 1 || a.max_tokens < 0 ||
       a.grow < 0)
     return KVMI_EINVAL;
   if ((int64_t)a.columns * a.block_size > kMostPlaces || (int64_t)a.blocks * a.block_size > 0x7fffffffLL ||
@@ -899,7 +903,7 @@ extern "C" int kvmi_copy_blocks(const kvmi_cache* cache, void* const* bases, int
 }
 
 extern "C" int64_t kvmi_compact_workspace_bytes(int32_t blocks) {
-  if (blocks < 1) return KVMI_EINVAL;
+  if (blocks < 1 || blocks > kvmi::kMostBlocks) return KVMI_EINVAL;
   return kvmi::compact_space(blocks).size;
 }
 
@@ -907,7 +911,7 @@ extern "C" int kvmi_compact_tables(const kvmi_compact_args* args, kvmi_stream_t 
   using namespace kvmi;
   if (!args) return KVMI_EINVAL;
   const kvmi_compact_args& a = *args;
-  if (a.rows < 0 || a.columns < 1 || a.blocks < 1 || a.block_size < 1) return KVMI_EINVAL;
+  if (a.rows < 0 || a.columns < 1 || a.blocks < 1 || a.blocks > kMostBlocks || a.block_size < 1) return KVMI_EINVAL;
   if ((int64_t)a.columns * a.block_size > kMostPlaces || (int64_t)a.blocks * a.block_size > 0x7fffffffLL ||
       (int64_t)a.columns * a.rows > 0x7fffffffLL)
     return KVMI_EINVAL;

@@ -293,7 +293,7 @@ PyObject* fork_block_tables(PyObject*, PyObject* const* in, Py_ssize_t n) try {
   t.workspace_bytes = space->numel() * 4;
   t.err = a.err(in[11]);
   kvmi_stream_t st;
-  if (!a.stream(&st)) return answer(false);
+  if (!a.stream(&st) || kvmi_fork_workspace_bytes(t.blocks, t.rows, t.columns) != t.workspace_bytes) return answer(false);
   return enqueue([&] { return kvmi_fork_tables(&t, st); });
 } catch (...) {
   return answer(false);
@@ -352,7 +352,7 @@ PyObject* compact_block_tables(PyObject*, PyObject* const* in, Py_ssize_t n) try
   t.workspace_bytes = space->numel() * 4;
   t.err = a.err(in[8]);
   kvmi_stream_t st;
-  if (!a.stream(&st)) return answer(false);
+  if (!a.stream(&st) || kvmi_compact_workspace_bytes(t.blocks) != t.workspace_bytes) return answer(false);
   return enqueue([&] { return kvmi_compact_tables(&t, st); });
 } catch (...) {
   return answer(false);

@@ -457,7 +457,7 @@ class ForkUpdate(NamedTuple):
 
 def _words(size: int, device) -> torch.Tensor:
     if size < 0:
-        raise ValueError("the sizes of a pool and its rows must be positive")
+        raise ValueError("the sizes of a pool and its rows must be positive, and the pool's at most 2**24 blocks")
     return torch.zeros((size + 3) // 4, dtype=torch.int32, device=device)
 
 
@@ -469,7 +469,8 @@ def _sizes(**sizes) -> None:
 
 def fork_workspace(blocks: int, rows: int, columns: int, device="cuda") -> torch.Tensor:
     """Workspace of `fork_block_tables` for a pool of `blocks` and `rows` rows of `columns` entries.
-    A call leaves it as it found it; no two calls may use it at a time."""
+    A call leaves it ready for the next one of the same sizes; no two calls may use it at a time, nor
+    two captured graphs that may run at a time."""
     _sizes(blocks=blocks, rows=rows, columns=columns)
     return _words(_lib.load().kvmi_fork_workspace_bytes(blocks, rows, columns), device)
 
@@ -482,12 +483,12 @@ def compact_workspace(blocks: int, device="cuda") -> torch.Tensor:
 
 def _space(workspace: Optional[torch.Tensor], size: int, device) -> torch.Tensor:
     if size < 0:
-        raise ValueError("the sizes of a pool and its rows must be positive")
+        raise ValueError("the sizes of a pool and its rows must be positive, and the pool's at most 2**24 blocks")
     if workspace is None:
         return _words(size, device)
     _tensor(workspace, "workspace", torch.int32, (None,), device)
-    if workspace.numel() * 4 < size or workspace.data_ptr() % 16:
-        raise ValueError(f"workspace must hold {(size + 3) // 4} words, 16-byte aligned")
+    if workspace.numel() != (size + 3) // 4 or workspace.data_ptr() % 16:
+        raise ValueError(f"workspace must be one made for these sizes: {(size + 3) // 4} words, 16-byte aligned")
     return workspace
 
 
@@ -515,7 +516,7 @@ def fork_block_tables(lengths: torch.Tensor, parents: Optional[torch.Tensor], ne
                  is no parent
     tables       int32 [R, columns]; rows that share a block have it in the same column, and a row's last
                  block is its own while it is partly filled (every call leaves them so)
-    shares       int32 [blocks]: how many rows hold a block besides the first
+    shares       int32 [blocks <= 2**24]: how many rows hold a block besides the first
     free, state  the ring of free blocks, int32 [blocks], and its head and count, as in
                  `build_block_tables`; `free` is changed in place
 

@@ -171,6 +171,29 @@ def test_beams_not_in_use_and_not_finite(cuda):
         assert int(err) == 256 and 3 not in got.all_parents.tolist()[1]
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_nan_of_either_sign_in_every_wave(cuda, dtype):
+    """Words of NaN lie above or below all others: the search for the best ends whatever they are."""
+    V = 5000
+    x, s = rand_logits(cuda, 6, V, DTYPES[dtype], 11)
+    bits = x.view(torch.int32 if dtype == "fp32" else torch.int16)
+    exp = {"bf16": 0x7f80, "fp16": 0x7c00, "fp32": 0x7f800000}[dtype]
+    top = 0x7fffffff if dtype == "fp32" else 0x7fff
+    signed = lambda v: v - 2 * (top + 1)  # with the sign
+    bits[0, ::7], bits[1, ::7] = top, signed(exp + top + 1 + 1)
+    bits[2, 100:164], bits[3, ::2] = signed(2 * top + 1), exp + 1
+    bits[4, :] = signed(2 * top + 1)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    for count in (3, 16, 17, 64):
+        err.zero_()
+        got = paged.select_beams(x, s, 3, count, check=False, err=err)
+        assert int(err) == 256 and got.all_parents[0].tolist() == [-1] * count
+        z = s.clone()
+        z[:5] = -math.inf
+        for a, b in zip(got, paged.select_beams(torch.where(torch.isnan(x), torch.zeros_like(x), x), z, 3, count)):
+            assert torch.equal(a, b)
+
+
 def test_scores_far_and_near(cuda):
     """Sums of log-probabilities far from zero, and beams a rounding apart."""
     x, s = rand_logits(cuda, 8, 4000, torch.float32, 9)

@@ -369,3 +369,54 @@ def test_rows_behind_a_sequence_do_not_matter(cuda):
     assert got.tables.tolist() == [[0, -1, -1]]
     got = paged.fork_block_tables(i([4]), None, 1, i([[2, 1 << 30, -9]]), i([0] * 3), i([0, 1, -1]), i([0, 2]), 4, 1)
     assert got.tables.tolist() == [[2, 0, -1]] and got.slots.tolist() == [0]
+
+
+def test_on_another_stream_with_work_before_it(cuda):
+    """Every call goes to the stream that is current, behind what is there."""
+    side = torch.cuda.Stream()
+    big = torch.randn((3000, 3000), device=cuda)
+    cache = torch.zeros((2, 8, 4, 1, 8), dtype=torch.bfloat16, device=cuda)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        own = paged.SharedBlockTables(8, 4, 3, 2, cuda)
+        for _ in range(20):
+            big = big @ big * 1e-3
+        first = i32([6, 0, 0], cuda)
+        logits = torch.zeros((3, 50), device=cuda) + big.sum() * 0
+        logits[0, 7], logits[0, 9] = 3.0, 2.0
+        scores = torch.tensor([0.0, float("-inf"), float("-inf")], device=cuda)
+        slots, _ = own.update(first, 6, check=False)
+        rows = torch.arange(48, device=cuda).view(6, 1, 8).to(torch.bfloat16)
+        paged.write_kv(rows, rows, cache, slots, check=False)
+        best = paged.select_beams(logits, scores, 3, check=False)
+        slots, starts = own.fork(best.parents, 1, 3, check=False)
+        paged.copy_blocks([cache], own.copies, check=False)
+        paged.copy_blocks([cache], own.compact(check=False), check=False)
+    side.synchronize()
+    assert best.tokens.tolist() == [7, 9, 0] and own.lengths.tolist() == [7, 7, 7] and own.shares.tolist()[0] == 2
+    for row in own.tables.tolist():
+        assert torch.equal(torch.cat([cache[0, row[0]], cache[0, row[1], :2]]), rows)
+
+
+def test_two_tables_side_by_side(cuda):
+    """Tables have workspaces of their own: their calls may overlap."""
+    r, streams = random.Random(9), [torch.cuda.Stream() for _ in range(2)]
+    R, C, S, N = 40, 12, 4, 600
+    own = [paged.SharedBlockTables(N, S, R, C, cuda) for _ in streams]
+    pools = [Pool(random.Random(0), R, C, S, N) for _ in streams]
+    for pool in pools:
+        pool.ring, pool.state = list(range(N)), [0, N]
+    for _ in range(6):
+        steps = []
+        for pool in pools:
+            parents, new = random_step(r, pool.lengths, C, S)
+            steps.append((i32(parents, cuda), i32(new, cuda)))
+            pool.take(fork(pool.lengths, parents, new, pool.tables, pool.shares, pool.ring, pool.state, S, 4000))
+        torch.cuda.synchronize()
+        for stream, tables, (parents, new) in zip(streams, own, steps):
+            with torch.cuda.stream(stream):
+                tables.fork(parents, new, 4000, check=False)
+        torch.cuda.synchronize()
+        for tables, pool in zip(own, pools):
+            got = (tables.tables, tables.lengths, tables.shares, tables.state, tables.free)
+            assert [t.tolist() for t in got] == [pool.tables, pool.lengths, pool.shares, pool.state, pool.ring]

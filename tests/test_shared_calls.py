@@ -27,13 +27,12 @@ def arguments(dev):
                               i32([[0] * 3] * 3, dev))
     best = paged.BeamChoice(i32([0] * 4, dev), i32([0] * 4, dev), torch.zeros(4, device=dev), i32([[0] * 4] * 2, dev),
                             i32([[0] * 4] * 2, dev), torch.zeros((2, 4), device=dev))
-    space = lambda n: torch.zeros(n, dtype=torch.int32, device=dev)
     return {
         "fork_block_tables": [lengths, i32([1, 1], dev), i32([18, 17], dev), tables, shares, ring, state, 16, 6, fork,
-                              space(400), None],
+                              paged.fork_workspace(6, 2, 2, dev), None],
         "copy_blocks": [ctypes.addressof(layers), torch.tensor([cache.data_ptr()], device=dev),
                         i32([[0, 4, 16], [1, 5, 3]], dev), None],
-        "compact_block_tables": [lengths, tables, shares, ring, state, 16, packed, space(400), None],
+        "compact_block_tables": [lengths, tables, shares, ring, state, 16, packed, paged.compact_workspace(6, dev), None],
         "select_beams": [torch.arange(36, device=dev).view(4, 9).to(BF16), torch.zeros(4, device=dev), 2, 4, 8, best, None],
     }, (layers, cache)
 
@@ -84,7 +83,8 @@ WRONG += [("fork_block_tables", 7, lambda v: 0), ("fork_block_tables", 8, lambda
           ("fork_block_tables", 2, lambda t: -1), ("fork_block_tables", 2, lambda t: None)]
 WRONG += [("compact_block_tables", i, f) for i in (0, 1, 2, 3, 4, 7) for f in (lambda t: t.long(), lambda t: t.cpu())]
 WRONG += [("compact_block_tables", 5, lambda v: 0), ("compact_block_tables", 6, lambda o: o[:4]),
-          ("compact_block_tables", 6, lambda o: tuple(o[:4]) + (o[4][:2],)), ("compact_block_tables", 7, lambda t: t[:9])]
+          ("compact_block_tables", 6, lambda o: tuple(o[:4]) + (o[4][:2],)), ("compact_block_tables", 7, lambda t: t[:9]),
+          ("compact_block_tables", 7, lambda t: torch.cat([t, t]))]
 WRONG += [("copy_blocks", 2, lambda t: t.long()), ("copy_blocks", 2, lambda t: t[:, :2]), ("copy_blocks", 2, lambda t: t[0]),
           ("copy_blocks", 1, lambda t: t.int()), ("copy_blocks", 3, lambda e: 0)]
 WRONG += [("select_beams", 0, lambda t: t.double()), ("select_beams", 0, lambda t: t[:3]), ("select_beams", 0, lambda t: t.t()),

@@ -29,7 +29,7 @@ def fork_args(**kw):
 
 @pytest.mark.parametrize("kw", [
     dict(rows=-1), dict(rows=4097), dict(columns=0), dict(blocks=0), dict(block_size=0), dict(max_tokens=-1),
-    dict(grow=-1), dict(columns=1 << 27), dict(blocks=1 << 27), dict(rows=4096, columns=1 << 20, block_size=1),
+    dict(grow=-1), dict(columns=1 << 27), dict(blocks=1 << 27), dict(blocks=(1 << 24) + 1, block_size=1), dict(rows=4096, columns=1 << 20, block_size=1),
     dict(workspace_bytes=0), dict(workspace=None), dict(workspace=P + 4), dict(lengths=None), dict(tables=None),
     dict(shares=None), dict(free_blocks=None), dict(state=None), dict(out_tables=None), dict(out_lengths=None),
     dict(out_shares=None), dict(out_state=None), dict(slots=None), dict(starts=None), dict(copies=None)])
@@ -51,7 +51,7 @@ def test_fork_refuses_outputs_over_some_inputs():
 
 @pytest.mark.parametrize("kw", [
     dict(rows=-1), dict(columns=0), dict(blocks=0), dict(block_size=0), dict(columns=1 << 27), dict(blocks=1 << 27),
-    dict(rows=1 << 20, columns=1 << 20, block_size=1), dict(workspace=None), dict(workspace=P + 4),
+    dict(blocks=(1 << 24) + 1, block_size=1), dict(rows=1 << 20, columns=1 << 20, block_size=1), dict(workspace=None), dict(workspace=P + 4),
     dict(workspace_bytes=8), dict(lengths=None), dict(tables=None), dict(shares=None), dict(free_blocks=None),
     dict(state=None), dict(out_tables=None), dict(out_shares=None), dict(out_free=None), dict(out_state=None),
     dict(copies=None), dict(out_tables=2 * P), dict(out_shares=3 * P), dict(out_free=4 * P), dict(out_state=5 * P)])
@@ -104,6 +104,7 @@ def test_workspaces_take_positive_sizes():
     lib = _lib.load()
     assert lib.kvmi_fork_workspace_bytes(0, 1, 1) == _lib.EINVAL and lib.kvmi_fork_workspace_bytes(1, -1, 1) == _lib.EINVAL
     assert lib.kvmi_compact_workspace_bytes(0) == _lib.EINVAL
+    assert lib.kvmi_compact_workspace_bytes((1 << 24) + 1) == lib.kvmi_fork_workspace_bytes((1 << 24) + 1, 1, 1) == _lib.EINVAL
     assert paged.fork_workspace(100, 4, 8, "cpu").sum() == 0 and paged.compact_workspace(100, "cpu").numel() > 50
     for bad in ((0, 1, 1), (1, 0, 1), (1, 1, 1 << 31), (1.0, 1, 1), (True, 1, 1)):
         with pytest.raises(ValueError):
