@@ -80,21 +80,27 @@ struct ForkRow {
 struct ForkSum {
   int taken;  // blocks out of the ring; -1 where the call changes nothing
   uint32_t tokens, copies;
-  int head;   // of the ring
+  int head, count;  // of the ring, as given (the head inside it)
+  int turn;         // which of the two counts this call uses
+  int unused;
 };
 // Workspace, in 32-bit words.  `words` counts what happens to a block's holders: rows that go on
 // without it in the upper half, rows that come to it besides one in the lower (at most
-// kMostForkRows of either, so the halves do not meet).
+// kMostForkRows of either, so the halves do not meet).  Of the two sets of `counts`, freed blocks of each
+// 64 ids, a call uses the one that `turn` names and clears the other, which nobody reads then.  (Counted
+// by 1024 ids, thousands of atomics met at one address: 34 us of 15.)
 struct ForkSpace {
-  int64_t words, counts, ticket, sum, rows, lengths, tables, size;
+  int64_t words, counts, turn, sum, rows, lengths, tables, size;
+  int counted;  // counts of a set
 };
 __host__ __device__ inline ForkSpace fork_space(int blocks, int rows, int columns) {
   ForkSpace s;
   s.words = 0;
-  s.counts = blocks;  // freed blocks of each 64 ids: counted by 1024, thousands met at one address (34 us of 15)
-  s.ticket = s.counts + ((int64_t)blocks + kCounted - 1) / kCounted;
-  s.sum = (s.ticket + 4) / 4 * 4;
-  s.rows = s.sum + 4;
+  s.counts = blocks;
+  s.counted = (blocks + kCounted - 1) / kCounted;
+  s.turn = s.counts + 2 * (int64_t)s.counted;
+  s.sum = (s.turn + 4) / 4 * 4;
+  s.rows = s.sum + 8;
   s.lengths = s.rows + 12 * (int64_t)rows;
   s.tables = (s.lengths + rows + 3) / 4 * 4;
   s.size = s.tables + (int64_t)rows * columns;
@@ -176,12 +182,12 @@ __device__ __forceinline__ ForkRow row_of(const ForkPlan& f, const BlockOf& div,
                  f.owner[i] == INT_MAX ? -1 : div(f.most[i]),     f.length[i]};
 }
 // The sums of all rows, whether the call can be done, and its error.
-__device__ __forceinline__ ForkSum sum_of(const kvmi_fork_args& a, int head, int count, const uint32_t* all, int bad,
-                                          int32_t* error) {
+__device__ __forceinline__ ForkSum sum_of(const kvmi_fork_args& a, int head, int count, int turn, const uint32_t* all,
+                                          int bad, int32_t* error) {
   bad |= count < 0 || count > a.blocks || all[1] > (uint32_t)a.max_tokens;
   const bool fits = all[0] <= (uint32_t)max(count, 0);
   *error = bad ? KVMI_ERR_LENGTH : fits ? 0 : KVMI_ERR_NO_BLOCKS;
-  return ForkSum{bad || !fits ? -1 : (int)all[0], all[1], all[2], (int)((uint32_t)head % (uint32_t)a.blocks)};
+  return ForkSum{bad || !fits ? -1 : (int)all[0], all[1], all[2], (int)((uint32_t)head % (uint32_t)a.blocks), count, turn, 0};
 }
 
 // What becomes of the blocks that row r held.  n entries from k on: their shares and atomics are on
@@ -199,6 +205,7 @@ struct Settler {
   const ForkRow& row;
   int have, listed;
   const int* list;
+  int32_t* counts;
   bool foreign;
 
   template <int n>
@@ -230,7 +237,7 @@ struct Settler {
 #pragma unroll
     for (int x = 0; x < n; ++x) {
       if (s.holders[x] == 0 && (int)(s.before[x] >> 16) == s.shares[x])
-        atomicAdd(a.workspace + at.counts + s.b[x] / kCounted, 1);
+        atomicAdd(counts + s.b[x] / kCounted, 1);
       foreign |= s.holders[x] == 1 && s.shares[x];
     }
   }
@@ -239,9 +246,10 @@ struct Settler {
 // child.  `list` has room for all rows.
 template <class F>
 __device__ __forceinline__ Settler settler_of(const kvmi_fork_args& a, const BlockOf& div, const ForkSpace& at,
-                                              const ForkRow& row, int* list, F child) {
+                                              const ForkRow& row, int turn, int* list, F child) {
   __shared__ int children;
-  Settler s{a, at, row, row.length ? div(row.length - 1) + 1 : 0, 0, list, false};
+  Settler s{a, at, row, row.length ? div(row.length - 1) + 1 : 0, 0, list,
+            a.workspace + at.counts + (turn ? at.counted : 0), false};
   if (row.kids && row.shortest < row.longest && row.shortest < s.have) {
     // children that keep more and less: who holds a block between is counted
     if (threadIdx.x == 0) children = 0;
@@ -358,7 +366,7 @@ __global__ __launch_bounds__(kThreads) void fork_fused_kernel(kvmi_fork_args a, 
   const int R = a.rows, C = a.columns, tid = threadIdx.x, r = blockIdx.x;
   const ForkSpace at = fork_space(a.blocks, R, C);
   const bool fours = in_fours(a, at, in_place);
-  const int head = gld(a.state), count = gld(a.state + 1);
+  const int head = gld(a.state), count = gld(a.state + 1), turn = gld(a.workspace + at.turn);
   const int k = 4 * (blockIdx.y * kThreads + tid);
   uint4 old = make_uint4(0, 0, 0, 0), source = old;
   if (fours && k < C) {
@@ -372,7 +380,7 @@ __global__ __launch_bounds__(kThreads) void fork_fused_kernel(kvmi_fork_args a, 
   // while that is summed, by every wave for itself
   const uint32_t none[3] = {0, 0, 0};
   ForkRow row = row_of(f, div, a.block_size, r, none);
-  Settler settler = settler_of(a, div, at, row, list, [&](int i) { return f.parent[i] == r ? div(f.kept[i]) : -1; });
+  Settler settler = settler_of(a, div, at, row, turn, list, [&](int i) { return f.parent[i] == r ? div(f.kept[i]) : -1; });
   Settled<4> held = four(old);
   if (fours && k < settler.have) settler.begin(k, held);
   uint32_t sum[6] = {0, 0, 0, 0, 0, 0};
@@ -388,13 +396,13 @@ __global__ __launch_bounds__(kThreads) void fork_fused_kernel(kvmi_fork_args a, 
 #pragma unroll
   for (int x = 0; x < 6; ++x) sum[x] = wave_sum(sum[x]);
   int32_t error;
-  const ForkSum all = sum_of(a, head, count, sum, *f.bad, &error);
+  const ForkSum all = sum_of(a, head, count, turn, sum, *f.bad, &error);
   row.takes = sum[3];
   row.tokens = sum[4];
   row.copies = sum[5];
   if (r == 0 && blockIdx.y == 0 && tid == 0) {
     flag_error(a.err, error);
-    a.workspace[at.sum] = all.taken;
+    *(ForkSum*)(a.workspace + at.sum) = all;
   }
   fork_row(a, div, in_place, at, row, all, r, fours, source);
   settler.end(held);
@@ -410,6 +418,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(kvmi_fork_args 
   __shared__ uint32_t wave_sums[3][kPlanThreads / 64], carry[3];
   const int R = a.rows, tid = threadIdx.x, head = gld(a.state), count = gld(a.state + 1);
   const ForkSpace at = fork_space(a.blocks, R, a.columns);
+  const int turn = gld(a.workspace + at.turn);
   const ForkPlan f = plan_rows<kPlanThreads>(a, div, plan_lds);
   if (tid < 3) carry[tid] = 0;
   __syncthreads();
@@ -445,9 +454,9 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(kvmi_fork_args 
   }
   if (tid == 0) {
     int32_t error;
-    const ForkSum all = sum_of(a, head, count, carry, *f.bad, &error);
+    const ForkSum all = sum_of(a, head, count, turn, carry, *f.bad, &error);
     flag_error(a.err, error);
-    gst((uint4*)(a.workspace + at.sum), *(const uint4*)&all);
+    *(ForkSum*)(a.workspace + at.sum) = all;
   }
 }
 __global__ __launch_bounds__(kThreads) void fork_rows_kernel(kvmi_fork_args a, BlockOf div, bool in_place) {
@@ -462,7 +471,7 @@ __global__ __launch_bounds__(kThreads) void fork_rows_kernel(kvmi_fork_args a, B
   const ForkRow row = rows[r];
   const ForkSum all = *(const ForkSum*)(a.workspace + at.sum);
   if (fours && k < C) source = gld((const uint4*)(a.tables + (int64_t)max(row.parent, 0) * C + k));
-  Settler settler = settler_of(a, div, at, row, list, [&](int i) { return rows[i].parent == r ? div(rows[i].kept) : -1; });
+  Settler settler = settler_of(a, div, at, row, all.turn, list, [&](int i) { return rows[i].parent == r ? div(rows[i].kept) : -1; });
   Settled<4> held = four(old);
   if (fours && k < settler.have) settler.begin(k, held);
   fork_row(a, div, in_place, at, row, all, r, fours, source);
@@ -472,15 +481,14 @@ __global__ __launch_bounds__(kThreads) void fork_rows_kernel(kvmi_fork_args a, B
 }
 
 // Workgroup g < ranges goes through 1024 block ids: their new shares, and the free ones behind the
-// ring's last, after those of the ranges before.  The last to arrive writes the state and clears
-// the counts, when nobody reads them any more.  The other workgroups bring rows that are made in
+// ring's last, after those of the ranges before.  The other workgroups bring rows that are made in
 // place from the workspace to their table.
 __global__ __launch_bounds__(kThreads) void fork_blocks_kernel(kvmi_fork_args a, int ranges, bool in_place) {
   __shared__ uint32_t sums[2][kWaves];
-  __shared__ int last;
   const int N = a.blocks, tid = threadIdx.x, g = blockIdx.x;
   const ForkSpace at = fork_space(N, a.rows, a.columns);
-  const int taken = a.workspace[at.sum];
+  const ForkSum call = *(const ForkSum*)(a.workspace + at.sum);
+  const int taken = call.taken;
   if (g >= ranges) {
     if (taken < 0) return;
     const int64_t all = (int64_t)a.rows * a.columns, step = (int64_t)(gridDim.x - ranges) * kThreads;
@@ -494,9 +502,9 @@ __global__ __launch_bounds__(kThreads) void fork_blocks_kernel(kvmi_fork_args a,
     for (int64_t i = first; i < a.rows; i += step) a.out_lengths[i] = a.workspace[at.lengths + i];
     return;
   }
-  const int head = (int)((uint32_t)a.state[0] % (uint32_t)N), given = a.state[1];
-  const int count = given < 0 ? 0 : given > N ? N : given;
-  int32_t* const counts = a.workspace + at.counts;
+  const int count = call.count < 0 ? 0 : min(call.count, N);
+  const int32_t* const counts = a.workspace + at.counts + (call.turn ? at.counted : 0);
+  int32_t* const others = a.workspace + at.counts + (call.turn ? 0 : at.counted);
   uint32_t held[4], word[4];  // (a refused call has counted, too)
   int shares[4];
   const int first = g * kRange + 4 * tid;
@@ -508,8 +516,7 @@ __global__ __launch_bounds__(kThreads) void fork_blocks_kernel(kvmi_fork_args a,
     shares[x] = in ? gld(a.shares + first + x) : 0;
   }
   uint32_t sum[2] = {0, 0};  // freed before this range, and in all
-  const int counted = (N + kCounted - 1) / kCounted;
-  for (int i = tid; i < counted; i += kThreads) {
+  for (int i = tid; i < at.counted; i += kThreads) {
     const uint32_t v = gld(counts + i);
     sum[1] += v;
     if (i < g * (kRange / kCounted)) sum[0] += v;
@@ -521,6 +528,7 @@ __global__ __launch_bounds__(kThreads) void fork_blocks_kernel(kvmi_fork_args a,
   uint32_t place[1] = {free};
   before_in_block(place, sums);
   place[0] += sum[0];
+  const uint32_t tail = ring_at(call.head, count, N);
   bool lost = false;
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
@@ -531,23 +539,20 @@ __global__ __launch_bounds__(kThreads) void fork_blocks_kernel(kvmi_fork_args a,
     if (held[x]) a.workspace[at.words + b] = 0;
     if (gone && gone > shares[x]) {
       if (place[0] < (uint32_t)(N - count))
-        a.free_blocks[((int64_t)head + count + place[0]) % N] = b;
+        a.free_blocks[ring_at(tail, place[0], N)] = b;
       else
         lost = true;
       ++place[0];
     }
   }
   if (lost) flag_error(a.err, KVMI_ERR_LENGTH);
-  __syncthreads();
-  if (tid == 0) last = atomicAdd(a.workspace + at.ticket, 1) == ranges - 1;
-  __syncthreads();
-  if (!last) return;
-  for (int i = tid; i < counted; i += kThreads) counts[i] = 0;
-  if (tid == 0) {
-    a.workspace[at.ticket] = 0;
-    const int out = max(taken, 0), back = min((int)sum[1], N - count);
-    a.out_state[0] = taken < 0 ? a.state[0] : (head + out) % N;
-    a.out_state[1] = taken < 0 ? given : count - out + back;
+  const int mine = g * (kRange / kCounted) + tid;
+  if (tid < kRange / kCounted && mine < at.counted) others[mine] = 0;
+  if (g == 0 && tid == 0) {  // (the other workgroups have state and turn from `call`)
+    a.workspace[at.turn] = !call.turn;
+    const int back = min((int)sum[1], N - count);
+    a.out_state[0] = taken < 0 ? a.state[0] : (int)ring_at(call.head, taken, N);
+    a.out_state[1] = taken < 0 ? call.count : count - taken + back;
   }
 }
 
@@ -690,11 +695,41 @@ __global__ __launch_bounds__(kThreads) void compact_count_kernel(kvmi_compact_ar
   }
 }
 
+// Pools of up to kSelf ids: every workgroup adds up all marks for itself (32 KB out of the L2 at the most)
+// instead of reading counts that a launch before it has made.  A thread takes the same power of two of ids,
+// 16 or more, so ranges begin with a thread.
+constexpr int kSelf = 16384, kSelfRanges = kSelf / kRange;
+__device__ __forceinline__ void count_all(const uint8_t* space, const CompactSpace& at, int N, uint32_t (*sums)[kWaves],
+                                          uint32_t (*ranges)[kSelfRanges + 1], uint32_t (&total)[2]) {
+  int log2 = 4;
+  while ((kThreads << log2) < N) ++log2;
+  const int first = threadIdx.x << log2;
+  uint32_t v[2] = {0, 0};
+  for (int i = first; i < min(first + (1 << log2), N); i += 16) {  // (the marks reach to a multiple of 16)
+    const uint4 h = gld((const uint4*)(space + at.held + i)), f = gld((const uint4*)(space + at.free + i));
+    v[0] += __popc(h.x) + __popc(h.y) + __popc(h.z) + __popc(h.w);
+    v[1] += __popc(h.x | f.x) + __popc(h.y | f.y) + __popc(h.z | f.z) + __popc(h.w | f.w);
+  }
+  total[0] = v[0];
+  total[1] = v[1];
+  before_in_block(v, sums);
+  if (first % kRange == 0 && first < kSelf) {
+    ranges[0][first / kRange] = v[0];
+    ranges[1][first / kRange] = v[1];
+  }
+  if (threadIdx.x == kThreads - 1) {  // (ranges behind the last hold nothing)
+    const int last = (kThreads << log2) / kRange;
+    ranges[0][last] = v[0] + total[0];
+    ranges[1][last] = v[1] + total[1];
+  }
+  block_sums(total, sums);
+}
+
 // Workgroup g: the places of 1024 ids among the held blocks and in the pool.  The pool's first n ids
 // stay or are taken (n: held blocks), so the number of moves is that of the free ones among them:
 // those of the ranges below the one where n falls, and some in it, which each looks up for itself.
 __global__ __launch_bounds__(kThreads) void compact_rank_kernel(kvmi_compact_args a, int ranges) {
-  __shared__ uint32_t sums[2][kWaves], mine[2], cut[3];
+  __shared__ uint32_t sums[2][kWaves], starts[2][kSelfRanges + 1], mine[2], cut[3];
   const int N = a.blocks, tid = threadIdx.x, g = blockIdx.x, first = g * kRange + 4 * tid;
   const CompactSpace at = compact_space(N);
   uint8_t* const space = (uint8_t*)a.workspace;
@@ -704,39 +739,55 @@ __global__ __launch_bounds__(kThreads) void compact_rank_kernel(kvmi_compact_arg
   int shares[4];
 #pragma unroll
   for (int x = 0; x < 4; ++x) shares[x] = (held >> (8 * x) & 1) && first + x < N ? gld(a.shares + first + x) : 0;
-  uint32_t total[2] = {0, 0};  // held, and in the pool
-  for (int i = tid; i < ranges; i += kThreads) {
-    total[0] += gld(counts + 2 * i);
-    total[1] += gld(counts + 2 * i + 1);
-  }
-  block_sums(total, sums);
-  const uint32_t n = total[0];
-  // what is held and in the pool before this range, and before the one in which the pool's n-th id falls
+  // held, and in the pool: in all, before this range, and before the one in which the pool's n-th id falls
+  uint32_t total[2] = {0, 0};
   if (tid == 0) cut[0] = 0x7fffffff;
-  uint32_t carry[2] = {0, 0};
-  for (int i0 = 0; i0 < ranges; i0 += kThreads) {
-    const int i = i0 + tid;
-    const uint32_t h = i < ranges ? gld(counts + 2 * i) : 0, u = i < ranges ? gld(counts + 2 * i + 1) : 0;
-    uint32_t before[2] = {h, u};
-    before_in_block(before, sums);
-    before[0] += carry[0];
-    before[1] += carry[1];
-    if (i == g) {
-      mine[0] = before[0];
-      mine[1] = before[1];
+  if (N <= kSelf) {
+    count_all(space, at, N, sums, starts, total);
+    if (tid < ranges) {
+      const uint32_t u = starts[1][tid];
+      if (u < total[0] && starts[1][tid + 1] >= total[0]) {
+        cut[0] = tid;
+        cut[1] = starts[0][tid];
+        cut[2] = u;
+      }
+      if (tid == g) {
+        mine[0] = starts[0][g];
+        mine[1] = u;
+      }
     }
-    if (before[1] < n && before[1] + u >= n) {
-      cut[0] = i;
-      cut[1] = before[0];
-      cut[2] = before[1];
+  } else {
+    for (int i = tid; i < ranges; i += kThreads) {
+      total[0] += gld(counts + 2 * i);
+      total[1] += gld(counts + 2 * i + 1);
     }
-    if (i0 + kThreads < ranges) {
-      uint32_t all[2] = {h, u};
-      block_sums(all, sums);
-      carry[0] += all[0];
-      carry[1] += all[1];
+    block_sums(total, sums);
+    uint32_t carry[2] = {0, 0};
+    for (int i0 = 0; i0 < ranges; i0 += kThreads) {
+      const int i = i0 + tid;
+      const uint32_t h = i < ranges ? gld(counts + 2 * i) : 0, u = i < ranges ? gld(counts + 2 * i + 1) : 0;
+      uint32_t before[2] = {h, u};
+      before_in_block(before, sums);
+      before[0] += carry[0];
+      before[1] += carry[1];
+      if (i == g) {
+        mine[0] = before[0];
+        mine[1] = before[1];
+      }
+      if (before[1] < total[0] && before[1] + u >= total[0]) {
+        cut[0] = i;
+        cut[1] = before[0];
+        cut[2] = before[1];
+      }
+      if (i0 + kThreads < ranges) {
+        uint32_t all[2] = {h, u};
+        block_sums(all, sums);
+        carry[0] += all[0];
+        carry[1] += all[1];
+      }
     }
   }
+  const uint32_t n = total[0];
   // this range's places; both counts fit half a word
   uint32_t place[1] = {(uint32_t)__popc(held) | (uint32_t)__popc(pool) << 16};
   before_in_block(place, sums);  // (its barriers are for `mine` and `cut` too)
@@ -779,22 +830,15 @@ __global__ __launch_bounds__(kThreads) void compact_rank_kernel(kvmi_compact_arg
     h += is_held;
     u += in_pool;
   }
-  if (first < N) {  // the marks are left zero for the next call; no other workgroup but at the cut reads them
-    if (cut[0] != (uint32_t)g) {
-      gst((uint32_t*)(space + at.held + first), 0u);
-      gst((uint32_t*)(space + at.free + first), 0u);
-    }
-  }
   flag_error(a.err, bits);
   if (g == 0 && tid == 0) {
-    ((uint32_t*)(space + at.moves))[0] = moves;
-    ((uint32_t*)(space + at.moves))[1] = cut[0];
+    *(uint32_t*)(space + at.moves) = moves;
     a.out_state[0] = 0;
     a.out_state[1] = (int)left;
   }
 }
 
-// The rows under the new names, and the list of moves.
+// The rows under the new names; the list of moves, and the marks cleared.
 __global__ __launch_bounds__(kThreads) void compact_name_kernel(kvmi_compact_args a, BlockOf div, int parts) {
   const int N = a.blocks, tid = threadIdx.x;
   const CompactSpace at = compact_space(N);
@@ -819,7 +863,7 @@ __global__ __launch_bounds__(kThreads) void compact_name_kernel(kvmi_compact_arg
     }
     return;
   }
-  const int moves = gld((const int32_t*)(space + at.moves)), range = gld((const int32_t*)(space + at.moves) + 1);
+  const int moves = gld((const int32_t*)(space + at.moves));
   const int first = (int)(blockIdx.x - rows) * kRange;
   for (int i = first + tid; i < min(N / 2, first + kRange); i += kThreads) {
     const bool moved = i < moves;
@@ -829,11 +873,9 @@ __global__ __launch_bounds__(kThreads) void compact_name_kernel(kvmi_compact_arg
     gst(a.copies + 3 * (int64_t)i + 2, moved ? a.block_size : -1);
     if (moved) gst(a.out_shares + b, gld((const int32_t*)(space + at.shares) + i));
   }
-  // the marks that all workgroups looked at before
-  const int id = range * kRange + 4 * tid;
-  if ((int64_t)blockIdx.x == rows && range != 0x7fffffff && id < N) {
-    gst((uint32_t*)(space + at.held + id), 0u);
-    gst((uint32_t*)(space + at.free + id), 0u);
+  if (first + 4 * tid < N) {  // the marks are left zero for the next call
+    gst((uint32_t*)(space + at.held + first + 4 * tid), 0u);
+    gst((uint32_t*)(space + at.free + first + 4 * tid), 0u);
   }
 }
 
@@ -929,7 +971,7 @@ extern "C" int kvmi_compact_tables(const kvmi_compact_args* args, kvmi_stream_t 
   if (rows + ranges > 0x7fffffffLL) return KVMI_EINVAL;
   const BlockOf div = block_of(a.block_size);
   hipLaunchKernelGGL(compact_mark_kernel, dim3((unsigned)(rows + ranges)), dim3(kThreads), 0, st, a, div, parts);
-  hipLaunchKernelGGL(compact_count_kernel, dim3((unsigned)ranges), dim3(kThreads), 0, st, a);
+  if (a.blocks > kSelf) hipLaunchKernelGGL(compact_count_kernel, dim3((unsigned)ranges), dim3(kThreads), 0, st, a);
   hipLaunchKernelGGL(compact_rank_kernel, dim3((unsigned)ranges), dim3(kThreads), 0, st, a, ranges);
   hipLaunchKernelGGL(compact_name_kernel, dim3((unsigned)(rows + ranges)), dim3(kThreads), 0, st, a, div, parts);
   return launched();
