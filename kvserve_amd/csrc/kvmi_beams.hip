@@ -13,6 +13,12 @@ constexpr int kVectors = 128;   // of 16 bytes, in which a tile's candidates are
 constexpr int kRoom = 8 * kVectors;  // candidates that are ranked at once
 constexpr double kFar = 600.0;  // logits up to here are summed as they are: exp(600) times any vocabulary is finite
 
+// Word w of a vector, w known only at run time.
+__device__ __forceinline__ uint32_t word_of(const u32x4v& v, int w) {
+  return w & 2 ? (w & 1 ? v.w : v.z) : (w & 1 ? v.y : v.x);
+}
+
+// The types of logits: element i of a vector, or of its word, and what stands for no logit.
 template <class T>
 struct Logits;
 template <>
@@ -23,6 +29,7 @@ struct Logits<__bf16> {
   }
   static __device__ __forceinline__ uint32_t bits(const void* row, int64_t i) { return gld((const uint16_t*)row + i); }
   static __device__ __forceinline__ float of(uint32_t word, int i) { return i & 1 ? bf_hi(word) : bf_lo(word); }
+  static __device__ __forceinline__ uint32_t word(const u32x4v& v, int i) { return word_of(v, i >> 1); }
   static constexpr uint32_t kNone = 0xff80;  // -inf
   static constexpr int kZeros = 16;          // bits at the end of a value in 32 bits that are all alike
 };
@@ -36,6 +43,7 @@ struct Logits<_Float16> {
   static __device__ __forceinline__ float of(uint32_t word, int i) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? word >> 16 : word));
   }
+  static __device__ __forceinline__ uint32_t word(const u32x4v& v, int i) { return word_of(v, i >> 1); }
   static constexpr uint32_t kNone = 0xfc00;
   static constexpr int kZeros = 13;
 };
@@ -45,6 +53,7 @@ struct Logits<float> {
   static __device__ __forceinline__ float at(const u32x4v& v, int i) { return __uint_as_float(v[i]); }
   static __device__ __forceinline__ uint32_t bits(const void* row, int64_t i) { return gld((const uint32_t*)row + i); }
   static __device__ __forceinline__ float of(uint32_t word, int) { return __uint_as_float(word); }
+  static __device__ __forceinline__ uint32_t word(const u32x4v& v, int i) { return word_of(v, i); }
   static constexpr uint32_t kNone = 0xff800000;
   static constexpr int kZeros = 0;
 };
@@ -68,14 +77,6 @@ __device__ __forceinline__ u32x4v load_logits(const void* row, int64_t e, int64_
     }
   }
   return v;
-}
-
-// What was unpacked of these vectors is unpacked anew behind this: kept in registers it would halve
-// the waves of a SIMD.
-template <int N>
-__device__ __forceinline__ void forget(u32x4v (&x)[N]) {
-#pragma unroll
-  for (int j = 0; j < N; ++j) asm volatile("" : "+v"(x[j]));
 }
 
 // exp(x) for |x| <= 700: 2^(n + r), n whole and |r| <= 1/2, with a polynomial of degree 7 for 2^r
@@ -203,9 +204,11 @@ struct SelectArgs {
 // Workgroup (tile, row): NV vectors a thread, all of them in registers: their sum of exp, and the
 // `count` best.  At least `count` elements reach the count-th largest of the threads' 256 largest, so
 // those below it cannot be among the best; the few that reach it, or a word a little below it, are
-// ranked against each other.
-// Where too many do (ties, or large ones in few threads) the count-th largest itself is found by
-// bisection.
+// ranked against each other.  Where too many do (ties, or large ones in few threads) the count-th
+// largest itself is found by bisection.
+// 64 requests x 8 beams x 131072 in bf16: 45 us; reading alone takes 22, the vector unit's 15.5
+// instructions an element and 260 a tile about 36 at 1.9 ns each (multiply-adds of 64 bits issue like
+// those of 32): bound by instructions.
 template <class T, int NV>
 __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
   using L = Logits<T>;
@@ -236,6 +239,12 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
     for (int j = 0; j < NV; ++j) x[j] = load_logits<T>(logits, first + (int64_t)(j * kThreads + tid) * VEC, V);
   }
   if (NV == 1 && !(__builtin_fabsf(score) < INFINITY)) return;
+  // What is seldom done goes through the tile in memory again, f(vector, j): unpacked from registers it
+  // would take twice those of what is always done.
+  auto over_tile = [&](auto f) {
+#pragma unroll 1
+    for (int j = 0; j < NV; ++j) f(load_logits<T>(logits, first + (int64_t)(j * kThreads + tid) * VEC, V), j);
+  };
   if (tid == 0) found = vectors = 0;
 
   float top[NV], lane_top = -INFINITY;
@@ -248,8 +257,10 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
     lane_top = __builtin_elementwise_maximum(lane_top, top[j]);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) sum += exp_near((double)__builtin_elementwise_maximum(L::at(x[j], i), -700.0f));
+    // (a vector's values are done with here: summed behind all the largest, they would all be kept, and
+    // take half the waves of a SIMD)
+    asm volatile("" : "+v"(sum));
   }
-  forget(x);
   const float high = wave_maximum(lane_top);
   double at = 0.0;
   if (!(__builtin_fabsf(high) <= (float)kFar)) {
@@ -260,10 +271,10 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
       at = -INFINITY;
     } else if (high < INFINITY) {
       at = high;
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) sum += exp_near(fmax((double)L::at(x[j], i) - at, -700.0));
+      over_tile([&](const u32x4v& v, int) {
+#pragma unroll 1
+        for (int i = 0; i < VEC; ++i) sum += exp_near(fmax((double)L::of(L::word(v, i), i) - at, -700.0));
+      });
     } else {
       sum = (double)NAN;
     }
@@ -326,39 +337,35 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
       const uint32_t mid = lo + (hi - lo) / 2;
       const float at_mid = key2f(mid);  // (NaN past +inf: nothing reaches it)
       int n = 0, all;
-      forget(x);
+      over_tile([&](const u32x4v& v, int) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) n += L::at(x[j], i) >= at_mid;
+        for (int i = 0; i < VEC; ++i) n += L::at(v, i) >= at_mid;
+      });
       before_in_block(n, scan, &all);
       if (all >= count)
         lo = mid;
       else
         hi = mid;
     }
-    forget(x);
     // fewer than `count` above it, and of those at it the first ones
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
+    over_tile([&](const u32x4v& v, int j) {
+#pragma unroll 1
       for (int i = 0; i < VEC; ++i)
-        if (order_of(L::at(x[j], i)) > lo) keep(L::at(x[j], i), token_of(j, i));
+        if (order_of(L::of(L::word(v, i), i)) > lo) keep(L::of(L::word(v, i), i), token_of(j, i));
+    });
     __syncthreads();
     int left = count - found;
-    forget(x);
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
+    over_tile([&](const u32x4v& v, int j) {
       int n = 0, all;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) n += order_of(L::at(x[j], i)) == lo;
+      for (int i = 0; i < VEC; ++i) n += order_of(L::at(v, i)) == lo;
       int before = before_in_block(n, scan, &all);
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < VEC; ++i)
-        if (order_of(L::at(x[j], i)) == lo && before++ < left) keep(L::at(x[j], i), token_of(j, i));
+        if (order_of(L::of(L::word(v, i), i)) == lo && before++ < left) keep(L::of(L::word(v, i), i), token_of(j, i));
       left -= all;  // (may go below zero: then none is taken)
-    }
+    });
     __syncthreads();
   }
   const int n = found;
@@ -393,7 +400,8 @@ constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64, kEach = 4, kRo
 // Workgroup: a request.  The rows' sums of all tiles, then the tiles' best, kRound at a time with the
 // best so far: those below the count-th largest of 64 lanes' best, or below the count-th so far, drop
 // out, the others are ranked against each other, each by several lanes where they are few.  A chain
-// of loads and of barriers: the first round's keys are on their way while the sums are made.
+// of loads and of barriers, 5.7 us for 4 beams x 16 tiles x 8 and 9 for 64 requests of 8 x 8 x 16: the first
+// round's keys are on their way while the sums are made.
 __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs s) {
   struct Candidates {
     double value[kRound + kMostCount];
@@ -546,15 +554,18 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs s)
 
 // Vectors a thread: as many as leave 384 workgroups, for what a tile does besides its sums costs the
 // same for any tile (32 rows x 4 beams x 131072: 21.9 us at 8 vectors, 25.6 at 4; 8 x 4: 13.9 at 4, 18.1
-// at 1; 13 x 5 x 50021: 15.0 at 2 in 845 workgroups, 17.0 at 8).
+// at 1; 13 x 5 x 50021: 15.0 at 4 in 455 workgroups, 15.1 at 2, 17.0 at 8); 16 only where 1536 are left, six
+// for a CU, whose loads and sums overlap (64 x 8 x 131072: 52.6 in 2048 workgroups, 56.4 at 8; but 16 x 4 x
+// 152064 in 32 bits 21.7 in 640, 19.1 at 8).
 struct Shape {
   int nv, tiles;
 };
 inline Shape shape_of(const kvmi_select_args& a) {
   const int vec = a.dtype == KVMI_DTYPE_FP32 ? 4 : 8;
   Shape s;
-  for (s.nv = 8; s.nv > 1; s.nv /= 2)
-    if ((int64_t)a.requests * a.beams * a.vocab >= 384LL * kThreads * s.nv * vec) break;
+  const int64_t vectors = (int64_t)a.requests * a.beams * a.vocab / vec;
+  for (s.nv = 16; s.nv > 1; s.nv /= 2)
+    if (vectors >= (s.nv == 16 ? 1536LL : 384LL) * kThreads * s.nv) break;
   const int64_t tile = (int64_t)kThreads * s.nv * vec;
   // rows may begin inside a vector
   const bool whole = (uintptr_t)a.logits % 16 == 0 && a.row_stride % vec == 0;
@@ -571,6 +582,7 @@ template <class T>
 void launch_tiles(const SelectArgs& s, int nv, hipStream_t st) {
   const dim3 grid((unsigned)s.tiles, (unsigned)(s.a.requests * s.a.beams));
   switch (nv) {
+    case 16: hipLaunchKernelGGL((select_tile_kernel<T, 16>), grid, dim3(kThreads), 0, st, s); break;
     case 8: hipLaunchKernelGGL((select_tile_kernel<T, 8>), grid, dim3(kThreads), 0, st, s); break;
     case 4: hipLaunchKernelGGL((select_tile_kernel<T, 4>), grid, dim3(kThreads), 0, st, s); break;
     case 2: hipLaunchKernelGGL((select_tile_kernel<T, 2>), grid, dim3(kThreads), 0, st, s); break;

@@ -355,12 +355,10 @@ __device__ __forceinline__ bool in_fours(const kvmi_fork_args& a, const ForkSpac
 }
 
 // Up to kFused rows: every workgroup (row, part) plans them all for itself, while its entries are on
-// their way, and no workgroup waits for another.  4 rows of 32 blocks 4.6 us, 256 rows of up to 750
-// FUSED_FIGURE.
-#ifndef FUSED
-#define FUSED 256
-#endif
-constexpr int kFused = FUSED;
+// their way, and no workgroup waits for another.  A chain of a trip to memory, the plan in the LDS,
+// the sums, the entries out of the ring, and the atomics' answers: 4 rows of 32 blocks 6.2 us, 256 rows of
+// up to 750 blocks 9.9 (7.2 without the atomics, of which it makes some 60,000).
+constexpr int kFused = 256;
 __global__ __launch_bounds__(kThreads) void fork_fused_kernel(kvmi_fork_args a, BlockOf div, bool in_place) {
   __shared__ int lds[8 * kFused + 1], list[kFused];
   const int R = a.rows, C = a.columns, tid = threadIdx.x, r = blockIdx.x;
@@ -410,8 +408,8 @@ __global__ __launch_bounds__(kThreads) void fork_fused_kernel(kvmi_fork_args a, 
   if (settler.foreign) flag_error(a.err, KVMI_ERR_BLOCK_ID);
 }
 
-// More rows: one workgroup plans them, the others read their rows' plans.  1024 rows planned by each of
-// 2048 workgroups took 39 us.
+// More rows: one workgroup plans them, the others read their rows' plans.  1024 rows of up to 500 blocks: 5.9
+// and 15.0 us (9.1 without the atomics); planned by each of 2048 workgroups for itself 31.
 constexpr int kPlanThreads = 1024;
 __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(kvmi_fork_args a, BlockOf div) {
   extern __shared__ int plan_lds[];
@@ -482,7 +480,8 @@ __global__ __launch_bounds__(kThreads) void fork_rows_kernel(kvmi_fork_args a, B
 
 // Workgroup g < ranges goes through 1024 block ids: their new shares, and the free ones behind the
 // ring's last, after those of the ranges before.  The other workgroups bring rows that are made in
-// place from the workspace to their table.
+// place from the workspace to their table.  34,000 blocks 3.9 us, 100,000 4.9: loads, two sums over the
+// workgroup, stores.
 __global__ __launch_bounds__(kThreads) void fork_blocks_kernel(kvmi_fork_args a, int ranges, bool in_place) {
   __shared__ uint32_t sums[2][kWaves];
   const int N = a.blocks, tid = threadIdx.x, g = blockIdx.x;
@@ -567,7 +566,9 @@ struct CopyArgs {
 
 // Workgroups (x, layer and part): each looks at every gridDim.x-th row, 64 at a time, a row a lane,
 // and copies those that are to be copied in units of V (16 bytes, or 2 where something is not
-// aligned), eight loads of a thread before its stores.
+// aligned), eight loads of a thread before its stores.  200 blocks of 64 KB in 32 layers 150 to 160 us (5.2 to
+// 5.6 TB/s read and written: memory); 24 pieces of 8 KB in 28 layers 8.3: the list, the base, the rows, the
+// stores, one after the other.
 template <class V>
 __global__ __launch_bounds__(kThreads) void copy_kernel(CopyArgs a) {
   constexpr int U = sizeof(V) / 2, kAtOnce = 8;
@@ -633,6 +634,9 @@ __device__ __forceinline__ int row_blocks(const kvmi_compact_args& a, const Bloc
   return cut ? div(cut - 1) + 1 : 0;
 }
 
+// Four launches (three for small pools): marks, counts, places, names.  Each is a trip or two to memory: a
+// pool of 65,536 with 512 rows 3.8 + 2.2 + 5.9 + 5.4 us, one of 1,024 with 16 rows 2.4 + 4.4 + 2.7.
+
 // Marks what the rows hold (workgroups of `parts` a row) and what the ring has free.
 __global__ __launch_bounds__(kThreads) void compact_mark_kernel(kvmi_compact_args a, BlockOf div, int parts) {
   const int N = a.blocks, tid = threadIdx.x;
@@ -697,7 +701,8 @@ __global__ __launch_bounds__(kThreads) void compact_count_kernel(kvmi_compact_ar
 
 // Pools of up to kSelf ids: every workgroup adds up all marks for itself (32 KB out of the L2 at the most)
 // instead of reading counts that a launch before it has made.  A thread takes the same power of two of ids,
-// 16 or more, so ranges begin with a thread.
+// 16 or more, so ranges begin with a thread.  16,384 blocks: a call in 13.5 us, 15.0 with the counts; 65,536:
+// 18.8, 16.5 with them.
 constexpr int kSelf = 16384, kSelfRanges = kSelf / kRange;
 __device__ __forceinline__ void count_all(const uint8_t* space, const CompactSpace& at, int N, uint32_t (*sums)[kWaves],
                                           uint32_t (*ranges)[kSelfRanges + 1], uint32_t (&total)[2]) {

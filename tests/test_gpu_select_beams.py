@@ -52,10 +52,11 @@ def test_beams_and_counts(cuda, beams, count):
     check(x, s, beams, count, end=int(x[0].float().argmax()))
 
 
-# enough rows that a thread takes 2, 4 and 8 vectors, in rows that begin off the 16-byte places
+# enough rows that a thread takes 2, 4, 8 and 16 vectors, in rows that begin off the 16-byte places
 @pytest.mark.parametrize("dtype,rows,V,pad", [("bf16", 96, 40001, 0), ("bf16", 160, 70000, 3), ("bf16", 192, 100003, 1),
                                               ("fp16", 128, 70001, 0), ("fp32", 32, 70001, 0), ("fp32", 96, 60001, 2),
-                                              ("fp32", 128, 70000, 0)])
+                                              ("fp32", 128, 70000, 0), ("bf16", 504, 100003, 0),
+                                              ("fp32", 256, 98400, 8)])
 def test_many_rows(cuda, dtype, rows, V, pad):
     x, s = rand_logits(cuda, rows, V, DTYPES[dtype], rows, pad)
     check(x, s, 4, 8, end=5)
