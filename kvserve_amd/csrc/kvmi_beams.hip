@@ -199,7 +199,15 @@ struct SelectArgs {
   int tiles;       // of a row
   double2* sums;   // [rows][tiles]: (s, m), the tile's sum of exp(x) is s exp(m); s NaN where it is not finite
   uint64_t* keys;  // [rows][tiles][count]: (order, ~token), best first; 0 behind the last
+  BlockOf per_row;  // by a row's keys
 };
+
+// Candidates that are ranked against each other: 2^l lanes for each of n, at most 16.
+__device__ __forceinline__ int rankers_log2(int n, int threads) {
+  int l = 0;
+  while (l < 4 && (2 * n << l) <= threads) ++l;
+  return l;
+}
 
 // Workgroup (tile, row): NV vectors a thread, all of them in registers: their sum of exp, and the
 // `count` best.  At least `count` elements reach the count-th largest of the threads' 256 largest, so
@@ -370,15 +378,14 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
   }
   const int n = found;
   uint64_t* const out = s.keys + (row * s.tiles + tile) * count;
-  int parts = 1;  // lanes that rank one candidate
-  while (parts < 16 && 2 * parts * n <= kThreads) parts *= 2;
-  for (int i0 = 0; i0 < n; i0 += kThreads / parts) {
-    const int i = i0 + tid / parts;
+  const int log2 = rankers_log2(n, kThreads), parts = 1 << log2, part = tid & (parts - 1);
+  for (int i0 = 0; i0 < n; i0 += kThreads >> log2) {
+    const int i = i0 + (tid >> log2);
     const uint64_t mine = best[min(i, n - 1)];
     int rank = 0;
-    for (int k = tid % parts; k < n; k += parts) rank += best[k] > mine;
+    for (int k = part; k < n; k += parts) rank += best[k] > mine;
     for (int d = parts / 2; d; d /= 2) rank += __shfl_xor(rank, d, 64);
-    if (i < n && tid % parts == 0 && rank < count) gst(out + rank, mine);
+    if (i < n && part == 0 && rank < count) gst(out + rank, mine);
   }
   for (int i = n + tid; i < count; i += kThreads) gst(out + i, (uint64_t)0);
 }
@@ -400,7 +407,7 @@ constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64, kEach = 4, kRo
 // Workgroup: a request.  The rows' sums of all tiles, then the tiles' best, kRound at a time with the
 // best so far: those below the count-th largest of 64 lanes' best, or below the count-th so far, drop
 // out, the others are ranked against each other, each by several lanes where they are few.  A chain
-// of loads and of barriers, 5.7 us for 4 beams x 16 tiles x 8 and 9 for 64 requests of 8 x 8 x 16: the first
+// of loads and of barriers, 5.2 us for 4 beams x 16 tiles x 8 and 6.0 for 64 requests of 8 x 4 x 16: the first
 // round's keys are on their way while the sums are made.
 __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs s) {
   struct Candidates {
@@ -417,28 +424,28 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs s)
   __shared__ int found;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = blockIdx.x;
   const int B = s.a.beams, count = s.a.count, tiles = s.tiles;
-  const int per_beam = tiles * count, all = B * per_beam;  // (at most 64 * 64 * tiles: select_ok)
+  const int all = B * tiles * count;  // (at most 64 * 64 * tiles: select_ok)
   const uint64_t* const keys = s.keys + (int64_t)r * all;
   uint64_t key[kEach];
 #pragma unroll
   for (int x = 0; x < kEach; ++x) key[x] = x * kJoinThreads + tid < all ? gld(keys + x * kJoinThreads + tid) : 0;
 
-  // log-sums: `group` lanes a row
-  int group = 1;
-  while (group < tiles && group < 64) group *= 2;
+  // log-sums: 2^group lanes a row
+  int group = 0;
+  while ((1 << group) < tiles && group < 6) ++group;
+  const int member = tid & ((1 << group) - 1);
   if (tid == 0) found = 0;
-  for (int b = tid / group; b < B; b += kJoinThreads / group) {
+  for (int b = tid >> group; b < B; b += kJoinThreads >> group) {
     const int64_t row = (int64_t)r * B + b;
     const float score = gld(s.a.scores + row);
     const bool used = __builtin_fabsf(score) < INFINITY;
     Sum sum{0.0, -INFINITY};
-    if (used)
-      for (int t = tid % group; t < tiles; t += group) {
-        const double2 p = s.sums[row * tiles + t];
-        sum = join(sum, Sum{p.x, p.y});
-      }
-    for (int d = group / 2; d; d /= 2) sum = join(sum, Sum{__shfl_xor(sum.s, d, 64), __shfl_xor(sum.m, d, 64)});
-    if (tid % group == 0) {
+    for (int t = member; t < tiles; t += 1 << group) {
+      const double2 p = s.sums[row * tiles + t];  // (anything, where the row is not used)
+      if (used) sum = join(sum, Sum{p.x, p.y});
+    }
+    for (int d = 1 << group >> 1; d; d /= 2) sum = join(sum, Sum{__shfl_xor(sum.s, d, 64), __shfl_xor(sum.m, d, 64)});
+    if (member == 0) {
       const double value = sum.s != sum.s ? (double)NAN : sum.s > 0.0 ? log(sum.s) + sum.m : -INFINITY;
       lse[b] = value;
       scores[b] = score;
@@ -457,7 +464,7 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs s)
       value[x] = -INFINITY;
       if (begin) key[x] = i < all ? gld(keys + i) : 0;
       if (i < all) {
-        beam[x] = i / per_beam;
+        beam[x] = s.per_row(i);
         const double sum = lse[beam[x]];
         if (__builtin_fabs(sum) < INFINITY && key[x]) {  // (a row without a sum has no keys)
           const double v = (double)scores[beam[x]] + ((double)key2f((uint32_t)(key[x] >> 32)) - sum);
@@ -466,7 +473,9 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs s)
       }
       top = fmaxf(top, (float)value[x]);
     }
-    const uint32_t floor = order_of(-INFINITY) + 1, tops[1] = {order_of(top)}, low = near_bound(tops, count, 0, 0xffffffffu);
+    const uint32_t floor = order_of(-INFINITY) + 1, tops[1] = {order_of(top)};
+    const uint32_t least = count <= 16 ? least_of_groups(tops[0], count <= 4) : 0;  // (16 groups, or 4)
+    const uint32_t low = near_bound(tops, count, least, order_of(wave_maximum(top)));
     if (lane == 0) bounds[wave] = max(low, floor);
     __syncthreads();
     uint32_t bound = have == count ? order_of((float)best_value[count - 1]) : floor;
@@ -483,16 +492,17 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs s)
     __syncthreads();
     const int fresh = found, n = fresh + have;
     if (fresh) {
-      if (tid < have) {
-        list.value[fresh + tid] = best_value[tid];
-        list.key[fresh + tid] = best_key[tid];
-        list.beam[fresh + tid] = best_beam[tid];
+      if (have) {
+        if (tid < have) {
+          list.value[fresh + tid] = best_value[tid];
+          list.key[fresh + tid] = best_key[tid];
+          list.beam[fresh + tid] = best_beam[tid];
+        }
+        __syncthreads();
       }
-      __syncthreads();
-      int parts = 1;  // lanes that rank one candidate
-      while (parts < 16 && 2 * parts * n <= kJoinThreads) parts *= 2;
-      for (int i0 = 0; i0 < n; i0 += kJoinThreads / parts) {
-        const int i = i0 + tid / parts;
+      const int log2 = rankers_log2(n, kJoinThreads), parts = 1 << log2, part = tid & (parts - 1);
+      for (int i0 = 0; i0 < n; i0 += kJoinThreads >> log2) {
+        const int i = i0 + (tid >> log2);
         int rank = 0;
         double mine = 0.0;
         uint64_t my_key = 0;
@@ -501,7 +511,7 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs s)
           mine = list.value[i];
           my_key = list.key[i];
           my_beam = list.beam[i];
-          for (int k = tid % parts; k < n; k += parts) {
+          for (int k = part; k < n; k += parts) {
             const double other = list.value[k];
             rank += other > mine;
             if (other == mine && k != i) {  // the lower beam, then the larger logit, then the lower token
@@ -511,7 +521,7 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs s)
           }
         }
         for (int d = parts / 2; d; d /= 2) rank += __shfl_xor(rank, d, 64);
-        if (i < n && tid % parts == 0 && rank < count) {
+        if (i < n && part == 0 && rank < count) {
           best_value[rank] = mine;
           best_key[rank] = my_key;
           best_beam[rank] = (uint8_t)my_beam;
@@ -520,8 +530,10 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs s)
       have = min(n, count);
     }
     __syncthreads();
-    if (tid == 0) found = 0;
-    __syncthreads();
+    if (begin + kRound < all) {
+      if (tid == 0) found = 0;
+      __syncthreads();
+    }
   }
   if (wave) return;
   const bool there = lane < have;
@@ -614,6 +626,7 @@ extern "C" int kvmi_select_beams(const kvmi_select_args* args, kvmi_stream_t str
   s.tiles = shape.tiles;
   s.sums = (double2*)a.workspace;
   s.keys = (uint64_t*)(s.sums + (int64_t)a.requests * a.beams * s.tiles);
+  s.per_row = block_of(s.tiles * a.count);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (a.dtype == KVMI_DTYPE_BF16)
     launch_tiles<__bf16>(s, shape.nv, st);

@@ -522,8 +522,9 @@ def fork_block_tables(lengths: torch.Tensor, parents: Optional[torch.Tensor], ne
 
     Whole blocks of kept tokens are shared.  A partly kept one goes on with a single row, where no
     other holds it; the other rows take a block for these tokens, and `copies` lists (from, to,
-    tokens): `copy_blocks` has to run on them before the new tokens are written.  Blocks that no row
-    holds any more go behind the ring's last free one, in the order of their ids.
+    tokens): `copy_blocks` has to run on them before the new tokens are written, and before the next
+    call, which may hand out the blocks copied from.  Blocks that no row holds any more go behind the
+    ring's last free one, in the order of their ids.
 
     All or nothing: with too few free blocks the call raises RuntimeError where it checks, with more
     than `max_tokens` new tokens or a length or parent out of range ValueError; rows and ring are
@@ -670,7 +671,7 @@ class SharedBlockTables(BlockTables):
 
       shares  int32 [num_blocks]: how many rows hold a block besides the first
       copies  int32 [requests, 3]: the blocks that the last `fork` or `update` split; `copy_blocks` on
-              them comes before the new tokens are written
+              them comes before the new tokens are written, and before the next of these calls
 
     Rewritten in place like the others."""
 
