@@ -719,7 +719,8 @@ int kvmi_compact_tables(const kvmi_compact_args* args, kvmi_stream_t stream);
  * far is scores[row].  Candidate (row, token) has the value
  *   scores[row] + (logits[row][token] - log(sum over t of exp(logits[row][t])))
  * and the `count` largest of a request are found; among equal ones the lower row comes first, then the
- * larger logit, then the lower token.  Sums and values are in 64 bits.  A value of -inf (after its
+ * larger logit, then the lower token.  Sums and values are in 64 bits, and a sum is right to 1e-10 of it:
+ * values of two rows that are closer may stand in either order, unless the rows' logits are the same.  A value of -inf (after its
  * rounding to fp32) is no candidate, nor is anything in a row whose score or sum is not finite; NaN
  * or +inf there sets KVMI_ERR_NOT_FINITE, but for rows whose score is -inf, whose logits do not matter.
  *   all_parents, all_tokens (int32), all_scores (fp32)  [requests][count] the candidates, best first:
