@@ -753,8 +753,8 @@ def select_beams(logits: torch.Tensor, scores: torch.Tensor, beams: int, count: 
 
     Values are in 64 bits until their last rounding; among equal ones the lower beam comes first, then
     the larger logit, then the lower token (a row's sum is right to 1e-10 of it: beams whose values are closer
-    than that may stand in either order, unless their logits are the same).  A value of -inf is no candidate: behind the last stand
-    parent and token -1 and score -inf.  So `parents` is what `fork_block_tables` takes: a row without
+    than that may stand in either order, unless their logits are the same).  A value of -inf is no
+    candidate: behind the last stand parent and token -1 and score -inf.  So `parents` is what `fork_block_tables` takes: a row without
     one gives its blocks back.  A beam with NaN or +inf in its score or logits has no candidates, and
     the call raises ValueError where it checks.  No gradient flows back.
 
