@@ -318,7 +318,7 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
   auto token_of = [&](int j, int i) { return (uint32_t)(first + (int64_t)(j * kThreads + tid) * VEC + i); };
   auto keep = [&](float v, uint32_t token) {
     const int n = atomicAdd(&found, 1);
-    best[n] = (uint64_t)order_of(v) << 32 | (uint32_t)~token;
+    if (n < kRoom) best[n] = (uint64_t)order_of(v) << 32 | (uint32_t)~token;  // (more only if the logits change meanwhile)
   };
   // the vectors that reach the bound, then their elements, spread over the threads
 #pragma unroll
@@ -355,14 +355,18 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
       else
         hi = mid;
     }
-    // fewer than `count` above it, and of those at it the first ones
+    // fewer than `count` above it, found by the comparison that they were counted with (which NaN never
+    // passes: its words lie above +inf's, and any number of them may be there), and of those at it the first
+    const float above = key2f(lo + 1);
     over_tile([&](const u32x4v& v, int j) {
 #pragma unroll 1
-      for (int i = 0; i < VEC; ++i)
-        if (order_of(L::of(L::word(v, i), i)) > lo) keep(L::of(L::word(v, i), i), token_of(j, i));
+      for (int i = 0; i < VEC; ++i) {
+        const float y = L::of(L::word(v, i), i);
+        if (y >= above) keep(y, token_of(j, i));
+      }
     });
     __syncthreads();
-    int left = count - found;
+    int left = count - min(found, count);
     __syncthreads();
     over_tile([&](const u32x4v& v, int j) {
       int n = 0, all;
@@ -376,7 +380,7 @@ __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
     });
     __syncthreads();
   }
-  const int n = found;
+  const int n = min(found, kRoom);
   uint64_t* const out = s.keys + (row * s.tiles + tile) * count;
   const int log2 = rankers_log2(n, kThreads), parts = 1 << log2, part = tid & (parts - 1);
   for (int i0 = 0; i0 < n; i0 += kThreads >> log2) {
