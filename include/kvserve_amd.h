@@ -720,14 +720,20 @@ int kvmi_compact_tables(const kvmi_compact_args* args, kvmi_stream_t stream);
  *   scores[row] + (logits[row][token] - log(sum over t of exp(logits[row][t])))
  * and the `count` largest of a request are found; among equal ones the lower row comes first, then the
  * larger logit, then the lower token.  Sums and values are in 64 bits, and a sum is right to 1e-10 of it:
- * values of two rows that are closer may stand in either order, unless the rows' logits are the same.  A value of -inf (after its
- * rounding to fp32) is no candidate, nor is anything in a row whose score or sum is not finite; NaN
- * or +inf there sets KVMI_ERR_NOT_FINITE, but for rows whose score is -inf, whose logits do not matter.
+ * values of two rows that are closer may stand in either order, unless the rows' logits are the same
+ * (these have the same sum, wherever they begin).  A value of -inf (after its rounding to fp32) is no
+ * candidate, nor is anything in a row whose score or sum is not finite; NaN or +inf there sets
+ * KVMI_ERR_NOT_FINITE, but for rows whose score is -inf, whose logits do not matter.
+ * The logarithm is in 64 bits too, right to 2^-53 of the row's largest logit: in a row that holds bf16's or
+ * fp32's lowest value throughout the number of its tokens is lost, and each gets the row's score (fp16's
+ * lowest is no such number).  A row with nothing allowed is left out by a score of -inf, or by logits
+ * of -inf.
  *   all_parents, all_tokens (int32), all_scores (fp32)  [requests][count] the candidates, best first:
  *                  row, token, value; behind the last -1, -1, -inf
  *   parents, tokens (int32), scores (fp32)  [requests * beams] those that go on: of each request the
  *                  first `beams` candidates with a token other than end_token, filled up alike
- * 1 <= beams <= count <= 64, at most 65535 rows; end_token -1: there is none.
+ * 1 <= beams <= count <= 64, at most 65535 rows; end_token -1: there is none.  With a count of at least
+ * beams + the beams that may end (2 * beams), as many go on as there are candidates for.
  */
 typedef struct kvmi_select_args {
   const void* logits;

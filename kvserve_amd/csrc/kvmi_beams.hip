@@ -222,9 +222,9 @@ __device__ __forceinline__ int rankers_log2(int n, int threads) {
 // those below it cannot be among the best; the few that reach it, or a word a little below it, are
 // ranked against each other.  Where too many do (ties, or large ones in few threads) the count-th
 // largest itself is found by bisection.
-// 64 requests x 8 beams x 131072 in bf16: 45 us; reading alone takes 22, the vector unit's 15.5
-// instructions an element and 260 a tile about 36 at 1.9 ns each (multiply-adds of 64 bits issue like
-// those of 32): bound by instructions.
+// 64 requests x 8 beams x 131072 in bf16: 45 to 47 us; reading alone takes 22, the vector unit's 18
+// instructions an element, a tile's end among them, about 35 at 1.9 ns each (multiply-adds of 64 bits
+// issue like those of 32): bound by instructions.
 template <class T, int NV>
 __global__ __launch_bounds__(kThreads) void select_tile_kernel(SelectArgs s) {
   using L = Logits<T>;
@@ -575,7 +575,7 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectArgs s)
 }
 
 // Vectors a thread: as many as leave 384 workgroups, for what a tile does besides its sums costs the
-// same for any tile (32 rows x 4 beams x 131072: 21.9 us at 8 vectors, 25.6 at 4; 8 x 4: 13.9 at 4, 18.1
+// same for any tile (us a call with its join: 32 rows x 4 beams x 131072 21.9 at 8 vectors, 25.6 at 4; 8 x 4: 13.9 at 4, 18.1
 // at 1; 13 x 5 x 50021: 15.0 at 4 in 455 workgroups, 15.1 at 2, 17.0 at 8); 16 only where 1536 are left, six
 // for a CU, whose loads and sums overlap (64 x 8 x 131072: 52.6 in 2048 workgroups, 56.4 at 8; but 16 x 4 x
 // 152064 in 32 bits 21.7 in 640, 19.1 at 8).

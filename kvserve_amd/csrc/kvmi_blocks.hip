@@ -12,8 +12,9 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kRange = 1024;        // block ids of a workgroup that goes through the pool, 4 a thread
 constexpr int kCounted = 64;        // block ids of a count
 constexpr int kMostForkRows = 4096;  // 32 bytes of LDS each
-// Every workgroup that goes through the pool adds up the counts of all: past this that would take longer
-// than the pool itself.
+// Every workgroup of kRange ids adds up the counts of the whole pool, work that goes with its square: a fork
+// of 8 rows takes 13 us in a pool of 2^18 blocks, 27 of 2^20, 106 of 2^22 and 1060 of 2^24, a compaction 15, 25,
+// 84 and 760, nearly all of it these sums in the largest two.
 constexpr int kMostBlocks = 1 << 24;
 
 inline int ranges_of(int blocks) { return (blocks + kRange - 1) / kRange; }
@@ -88,7 +89,7 @@ struct ForkSum {
 // without it in the upper half, rows that come to it besides one in the lower (at most
 // kMostForkRows of either, so the halves do not meet).  Of the two sets of `counts`, freed blocks of each
 // 64 ids, a call uses the one that `turn` names and clears the other, which nobody reads then.  (Counted
-// by 1024 ids, thousands of atomics met at one address: 34 us of 15.)
+// by 1024 ids, thousands of atomics met at one address: 1024 rows 44 us a call, 27 by 64.)
 struct ForkSpace {
   int64_t words, counts, turn, sum, rows, lengths, tables, size;
   int counted;  // counts of a set
@@ -356,8 +357,9 @@ __device__ __forceinline__ bool in_fours(const kvmi_fork_args& a, const ForkSpac
 
 // Up to kFused rows: every workgroup (row, part) plans them all for itself, while its entries are on
 // their way, and no workgroup waits for another.  A chain of a trip to memory, the plan in the LDS,
-// the sums, the entries out of the ring, and the atomics' answers: 4 rows of 32 blocks 6.2 us, 256 rows of
-// up to 750 blocks 9.9 (7.2 without the atomics, of which it makes some 60,000).
+// the sums, the entries out of the ring, and the atomics' answers: 4 rows of 32 blocks 6.4 us, 256 rows of
+// up to 750 blocks 9.9 (7.2 without the atomics, of which it makes some 60,000).  Rows that are made in
+// place: 256 rows 10.6, and 0.1 us more to bring them back; 64 rows of up to 8192 blocks 18.6 and 1.0 more.
 constexpr int kFused = 256;
 __global__ __launch_bounds__(kThreads) void fork_fused_kernel(kvmi_fork_args a, BlockOf div, bool in_place) {
   __shared__ int lds[8 * kFused + 1], list[kFused];
@@ -409,7 +411,9 @@ __global__ __launch_bounds__(kThreads) void fork_fused_kernel(kvmi_fork_args a, 
 }
 
 // More rows: one workgroup plans them, the others read their rows' plans.  1024 rows of up to 500 blocks: 5.9
-// and 15.0 us (9.1 without the atomics); planned by each of 2048 workgroups for itself 31.
+// and 15.9 us (some 6 of it the atomics).  Rows of up to 750 blocks, us a call with this launch or planned
+// by every workgroup for itself: 128 rows 14.1 / 11.8, 256 15.8 / 13.8, 384 18.1 / 17.0, 512 18.8 / 18.2, 768
+// 23.8 / 24.2, 1024 27.5 / 29.1; 256 keeps the other kernel's LDS at 9 KB a workgroup.
 constexpr int kPlanThreads = 1024;
 __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(kvmi_fork_args a, BlockOf div) {
   extern __shared__ int plan_lds[];

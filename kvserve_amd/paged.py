@@ -748,15 +748,23 @@ def select_beams(logits: torch.Tensor, scores: torch.Tensor, beams: int, count: 
                after the other; any row stride, tokens adjacent
     scores     float32 [requests * beams]: sums of log-probabilities so far; -inf for a beam that is not
                in use (its logits do not matter)
-    count      beams <= count <= 64 candidates a request; default: beams, or with an end token twice that
-    end_token  candidates with this token are listed, but do not go on
+    count      beams <= count <= 64 candidates a request; default: beams, or with an end token twice that,
+               at most 64 (so that with more than 32 beams fewer than `beams` may go on: 64 less those
+               that end)
+    end_token  candidates with this token are listed, but do not go on; where several tokens end an
+               answer, choose those that go on from the `all_...` outputs
 
     Values are in 64 bits until their last rounding; among equal ones the lower beam comes first, then
     the larger logit, then the lower token (a row's sum is right to 1e-10 of it: beams whose values are closer
     than that may stand in either order, unless their logits are the same).  A value of -inf is no
-    candidate: behind the last stand parent and token -1 and score -inf.  So `parents` is what `fork_block_tables` takes: a row without
-    one gives its blocks back.  A beam with NaN or +inf in its score or logits has no candidates, and
-    the call raises ValueError where it checks.  No gradient flows back.
+    candidate: behind the last stand parent and token -1 and score -inf.  So `parents` is what
+    `fork_block_tables` takes: a row without one gives its blocks back.  A beam with NaN or +inf in its
+    score or logits has no candidates, and the call raises ValueError where it checks.  No gradient
+    flows back.
+
+    Banned tokens may hold -inf or the type's lowest value.  A beam with no token left is given a score of
+    -inf, or -inf throughout: a log-sum in 64 bits is right to 2^-53 of the row's largest logit, so a row of
+    bfloat16's or float32's lowest value throughout would give each token the beam's own score.
 
     `out`: the tensors of a `BeamChoice` to write into."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
